@@ -8,13 +8,18 @@
 #include <unordered_map>
 #include <vector>
 
+#include "api_common.cuh"
 #include "attention.cuh"
 #include "cache_ops.cuh"
 #include "nvtx.cuh"
 
-namespace {
+namespace b200 {
 
+namespace {
 thread_local std::string g_last_error;
+}  // namespace
+
+void set_last_error(const char* msg) { g_last_error = msg; }
 
 int cuda_fail(cudaError_t e, const char* where) {
   g_last_error = std::string(where) + ": " + cudaGetErrorString(e);
@@ -51,6 +56,15 @@ int num_sms() {
   }
   return n;
 }
+
+}  // namespace b200
+
+using b200::cuda_fail;
+using b200::esize_of;
+using b200::fail;
+using b200::num_sms;
+
+namespace {
 
 // ---- tensor maps -----------------------------------------------------------------------------
 // cuTensorMapEncodeTiled is fetched through the runtime's driver entry point, so the library
@@ -217,10 +231,6 @@ DecodePlan make_decode_plan(const B200DecodeParams& p) {
 
 }  // namespace
 
-namespace b200 {
-void set_last_error(const char* msg) { g_last_error = msg; }
-}  // namespace b200
-
 extern "C" {
 
 const char* b200_status_string(int status) {
@@ -236,7 +246,7 @@ const char* b200_status_string(int status) {
   }
 }
 
-const char* b200_last_error(void) { return g_last_error.c_str(); }
+const char* b200_last_error(void) { return b200::g_last_error.c_str(); }
 
 void b200_set_decode_split_tokens(int32_t tokens) {
   g_split_override.store(tokens > 0 ? ((tokens + 15) / 16) * 16 : 0, std::memory_order_relaxed);
