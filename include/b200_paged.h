@@ -40,6 +40,8 @@ extern "C" {
 #define B200_DEVICE_BAD_STEP 16   /* step metadata: bad sequence slot, negative start/count,
                                      or more tokens than the outputs hold                   */
 
+#define B200_DEVICE_BAD_SAMPLE 32 /* sampling: a row in which no token can be drawn          */
+
 /* ---- element types --------------------------------------------------------------------------- */
 #define B200_DTYPE_F32 0
 #define B200_DTYPE_BF16 1
@@ -373,6 +375,124 @@ int64_t b200_host_bytes_per_token(const B200HostAllocator* a);
 int64_t b200_host_pool_bytes(const B200HostAllocator* a);
 double b200_host_utilization(const B200HostAllocator* a);
 const char* b200_host_last_message(void);
+
+/* ============================================================================================
+ * 7. 8-bit paged cache: append, read back, decode and prefill
+ * ==========================================================================================*/
+
+/* Key and value caches of e4m3 numbers, (L, NB, BS, Hkv, D), with one fp32 scale per layer, block
+ * and KV head, (L, NB, Hkv): an entry stands for code * scale.  Half the bytes of a 16-bit cache
+ * plus 4 / (BS * D) of a byte per entry.  The appends below write powers of two as scales; a block
+ * that was never written has an undefined scale, which the append of its first slot replaces.
+ * All four arrays contiguous.  No counterpart in the reference (its caches hold the model's type). */
+typedef struct {
+  void* key_cache;
+  void* value_cache;
+  float* key_scale;
+  float* value_scale;
+  int32_t num_layers;
+  int32_t total_blocks;
+  int32_t block_size;    /* at most 1024 */
+  int32_t num_kv_heads;
+  int32_t head_dim;      /* at most 256 */
+  int32_t layer_idx;     /* the layer the call works on */
+} B200Fp8Cache;
+
+/* Bytes of device workspace the two appends need for num_tokens rows (0 for small calls). */
+size_t b200_append_fp8_workspace_bytes(const B200Fp8Cache* cache, int32_t num_tokens);
+
+/* b200_reshape_and_cache into an 8-bit cache; key and value rows are of `dtype`.  With m the
+ * largest finite |x| of a head over the call's rows in a block and need = the smallest power of
+ * two s (2^-100 at least) with m <= 448 s: the block's scale becomes need where the call writes the
+ * block's first slot (the block begins anew and what it held no longer counts), max(scale, need)
+ * elsewhere; where it grows, the entries that the block holds are rounded to the new scale.  Rows
+ * are rounded to the nearest code; infinities and NaN are held as NaN.  Rows may come in any
+ * order; of rows with the same slot the last one counts.  Slots < 0 are padding and skipped, slots
+ * >= NB*BS set B200_DEVICE_BAD_SLOT and are skipped.  Blocks of this call that other work reads
+ * or writes at the same time race. */
+int b200_reshape_and_cache_fp8(const B200Fp8Cache* cache, int32_t dtype, const void* key,
+                               int64_t k_stride_token, int64_t k_stride_head, const void* value,
+                               int64_t v_stride_token, int64_t v_stride_head,
+                               const int64_t* slot_mapping, int32_t num_tokens, void* workspace,
+                               size_t workspace_bytes, int32_t* status_word, void* stream);
+
+/* b200_rope_reshape_and_cache into an 8-bit cache: rotated q of `dtype` to q_out, rotated k and
+ * v to their slots as above.  Unlike the 16-bit form, angles are formed and reduced in 64 bits
+ * (exact at far positions) and rotated keys are rounded once, to their codes. */
+int b200_rope_reshape_and_cache_fp8(const B200Fp8Cache* cache, int32_t dtype, const void* qkv,
+                                    int64_t qkv_stride_token, int32_t num_tokens,
+                                    int32_t num_query_heads, const int64_t* positions,
+                                    const float* inv_freq, void* q_out,
+                                    int64_t q_out_stride_token, const int64_t* slot_mapping,
+                                    void* workspace, size_t workspace_bytes,
+                                    int32_t* status_word, void* stream);
+
+/* Read n slots back as values: k_out and v_out (n, Hkv, D) of `dtype`, contiguous.  Slots < 0 give
+ * zeros; slots >= NB*BS set B200_DEVICE_BAD_SLOT and give zeros.  Values beyond an f16's range
+ * become +-65504. */
+int b200_gather_cache_fp8(const B200Fp8Cache* cache, int32_t dtype, const int64_t* slots,
+                          int64_t n, void* k_out, void* v_out, int32_t* status_word,
+                          void* stream);
+
+typedef struct {
+  B200Fp8Cache cache;
+  const void* query;          /* [row][Hq][D] of `dtype`, strides in elements, D contiguous     */
+  int64_t q_stride_row;
+  int64_t q_stride_head;
+  void* out;                  /* [row][Hq][D] of `dtype`                                        */
+  int64_t o_stride_row;
+  int64_t o_stride_head;
+  int32_t dtype;              /* B200_DTYPE_* of query and out                                  */
+  int32_t num_query_heads;
+  const int32_t* block_tables; /* (S, block_table_stride)                                       */
+  int32_t block_table_stride;
+  const int32_t* context_lens; /* (S,)                                                          */
+  int32_t num_seqs;
+  int32_t max_context_len;    /* host upper bound of context_lens                               */
+  float scale;
+  const int32_t* query_rows;  /* decode: as in B200DecodeParams; prefill: unused                */
+  const int64_t* cu_seqlens;  /* prefill: as in B200PrefillParams; decode: unused               */
+  int32_t num_tokens;         /* prefill                                                        */
+  int32_t max_query_len;      /* prefill                                                        */
+  int32_t prefill_blocks;     /* prefill: host upper bound of the cache blocks that sequences with
+                                 more than one new token hold together; < 0: not known          */
+  int32_t* status_word;
+} B200AttentionFp8Params;
+
+size_t b200_paged_decode_fp8_workspace_bytes(const B200AttentionFp8Params* p);
+
+/* b200_paged_decode over an 8-bit cache.  A context of 0 gives zeros.  A page outside the pool
+ * sets B200_DEVICE_BAD_BLOCK and its positions do not take part. */
+int b200_paged_decode_fp8(const B200AttentionFp8Params* p, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+size_t b200_paged_prefill_fp8_workspace_bytes(const B200AttentionFp8Params* p);
+
+/* b200_paged_prefill over an 8-bit cache.  Rows of query behind the last sequence are left as
+ * they are in out. */
+int b200_paged_prefill_fp8(const B200AttentionFp8Params* p, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* ============================================================================================
+ * 8. Token sampling
+ * ==========================================================================================*/
+
+/* One token per row of logits (rows, vocab) of `dtype`, rows stride_row elements apart, drawn by
+ * the given uniform numbers in [0, 1).  With tokens ordered by decreasing logit (ties: the lower
+ * index first) and w = exp((logit - max) / temperature): top-k keeps the first k (<= 0: all);
+ * top-p keeps of those each token whose predecessors' sum of w is below top_p times their sum;
+ * min-p keeps tokens with w >= min_p; the first of all is always kept.  The token drawn is the
+ * first in index order whose cumulative w exceeds uniform times the kept sum; temperature 0 takes
+ * the first of all.  Parameters are device arrays of one entry per row; temperature, top_k, top_p
+ * and min_p may be NULL (1, off, 1, 0).  NaN logits count as -inf.  logprobs (may be NULL): the
+ * token's log probability at the row's temperature over the whole vocabulary.  A row in which no
+ * token can be drawn (all logits -inf, or a parameter that is NaN or out of range) gives -1 and
+ * NaN and sets B200_DEVICE_BAD_SAMPLE.  vocab <= 2^24.  Replaces the per-sequence host argmax of
+ * app/engine/llm_engine.py:200-204 for requests that are not greedy. */
+int b200_sample(const void* logits, int32_t dtype, int64_t stride_row, int32_t rows, int32_t vocab,
+                const float* uniform, const float* temperature, const int32_t* top_k,
+                const float* top_p, const float* min_p, int64_t* tokens, float* logprobs,
+                int32_t* status_word, void* stream);
 
 #ifdef __cplusplus
 }

@@ -27,6 +27,7 @@ DEVICE_BAD_SLOT = 2
 DEVICE_TIMEOUT = 4
 DEVICE_BAD_OP = 8
 DEVICE_BAD_STEP = 16
+DEVICE_BAD_SAMPLE = 32
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
@@ -69,6 +70,23 @@ class PrefillParams(ctypes.Structure):
         ("cu_seqlens", c_vp), ("context_lens", c_vp), ("num_seqs", c_i32), ("num_tokens", c_i32),
         ("max_query_len", c_i32), ("max_context_len", c_i32), ("scale", c_f), ("out", c_vp),
         ("o_stride_token", c_i64), ("o_stride_head", c_i64), ("status_word", c_vp),
+    ]
+
+
+class Fp8Cache(ctypes.Structure):
+    _fields_ = [(n, c_vp) for n in ("key_cache", "value_cache", "key_scale", "value_scale")] + [
+        (n, c_i32) for n in ("num_layers", "total_blocks", "block_size", "num_kv_heads", "head_dim",
+                             "layer_idx")]
+
+
+class AttentionFp8Params(ctypes.Structure):
+    _fields_ = [
+        ("cache", Fp8Cache), ("query", c_vp), ("q_stride_row", c_i64), ("q_stride_head", c_i64),
+        ("out", c_vp), ("o_stride_row", c_i64), ("o_stride_head", c_i64), ("dtype", c_i32),
+        ("num_query_heads", c_i32), ("block_tables", c_vp), ("block_table_stride", c_i32),
+        ("context_lens", c_vp), ("num_seqs", c_i32), ("max_context_len", c_i32), ("scale", c_f),
+        ("query_rows", c_vp), ("cu_seqlens", c_vp), ("num_tokens", c_i32),
+        ("max_query_len", c_i32), ("prefill_blocks", c_i32), ("status_word", c_vp),
     ]
 
 
@@ -139,6 +157,23 @@ SIGNATURES = [
     ("b200_host_pool_bytes", c_i64, [c_vp]),
     ("b200_host_utilization", ctypes.c_double, [c_vp]),
     ("b200_host_last_message", ctypes.c_char_p, []),
+    ("b200_sample", ctypes.c_int, [c_vp, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                   c_vp, c_vp, c_vp, c_vp]),
+    ("b200_append_fp8_workspace_bytes", c_sz, [ctypes.POINTER(Fp8Cache), c_i32]),
+    ("b200_reshape_and_cache_fp8", ctypes.c_int, [ctypes.POINTER(Fp8Cache), c_i32, c_vp, c_i64,
+                                                  c_i64, c_vp, c_i64, c_i64, c_vp, c_i32, c_vp,
+                                                  c_sz, c_vp, c_vp]),
+    ("b200_rope_reshape_and_cache_fp8", ctypes.c_int, [ctypes.POINTER(Fp8Cache), c_i32, c_vp,
+                                                       c_i64, c_i32, c_i32, c_vp, c_vp, c_vp,
+                                                       c_i64, c_vp, c_vp, c_sz, c_vp, c_vp]),
+    ("b200_gather_cache_fp8", ctypes.c_int, [ctypes.POINTER(Fp8Cache), c_i32, c_vp, c_i64, c_vp,
+                                             c_vp, c_vp, c_vp]),
+    ("b200_paged_decode_fp8_workspace_bytes", c_sz, [ctypes.POINTER(AttentionFp8Params)]),
+    ("b200_paged_decode_fp8", ctypes.c_int, [ctypes.POINTER(AttentionFp8Params), c_vp, c_sz,
+                                             c_vp]),
+    ("b200_paged_prefill_fp8_workspace_bytes", c_sz, [ctypes.POINTER(AttentionFp8Params)]),
+    ("b200_paged_prefill_fp8", ctypes.c_int, [ctypes.POINTER(AttentionFp8Params), c_vp, c_sz,
+                                              c_vp]),
 ]
 
 _LIB = None

@@ -1,0 +1,259 @@
+// C ABI of the 8-bit paged cache (include/b200_paged.h, section 7): argument checks and launches.
+#include "api_common.cuh"
+#include "fp8.cuh"
+#include "nvtx.cuh"
+
+using b200::cuda_fail;
+using b200::esize_of;
+using b200::fail;
+using b200::num_sms;
+
+namespace {
+
+int check_cache(const B200Fp8Cache* c, int dtype) {
+  if (c == nullptr) return fail(B200_ERR_INVALID_ARGUMENT, "null cache");
+  if (esize_of(dtype) == 0) return fail(B200_ERR_UNSUPPORTED, "unsupported dtype");
+  if (c->num_layers <= 0 || c->total_blocks <= 0 || c->block_size <= 0 || c->num_kv_heads <= 0 ||
+      c->head_dim <= 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "cache geometry must be positive");
+  if (c->layer_idx < 0 || c->layer_idx >= c->num_layers)
+    return fail(B200_ERR_INVALID_ARGUMENT, "layer_idx out of range");
+  if (c->block_size > 1024) return fail(B200_ERR_UNSUPPORTED, "block_size > 1024");
+  if (c->head_dim > 256) return fail(B200_ERR_UNSUPPORTED, "head_dim > 256");
+  if (c->num_kv_heads > 1024) return fail(B200_ERR_UNSUPPORTED, "num_kv_heads > 1024");
+  return B200_OK;
+}
+
+bool has_arrays(const B200Fp8Cache& c) {
+  return c.key_cache && c.value_cache && c.key_scale && c.value_scale;
+}
+
+// Cache side of an append, and its scratch in the caller's workspace.
+int append_args(const B200Fp8Cache& c, const int64_t* slots, int32_t n, void* workspace,
+                size_t workspace_bytes, int32_t* status, b200::AppendFp8Args* a) {
+  a->kc = static_cast<uint8_t*>(c.key_cache);
+  a->vc = static_cast<uint8_t*>(c.value_cache);
+  a->ks = c.key_scale;
+  a->vs = c.value_scale;
+  a->layer = c.layer_idx;
+  a->nb = c.total_blocks;
+  a->bs = c.block_size;
+  a->hkv = c.num_kv_heads;
+  a->head_dim = c.head_dim;
+  a->slots = slots;
+  a->num_tokens = n;
+  a->status = status;
+  const size_t need = b200::append_fp8_scratch_bytes(c.total_blocks, n);
+  if (need == 0) return B200_OK;
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(B200_ERR_INVALID_ARGUMENT, "append workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 4 != 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "append workspace must be 4-byte aligned");
+  a->count = static_cast<int32_t*>(workspace);
+  a->first = a->count + c.total_blocks;
+  a->num_runs = a->first + c.total_blocks;
+  a->runs = a->num_runs + 1;
+  return B200_OK;
+}
+
+int check_attention(const B200AttentionFp8Params* p) {
+  if (p == nullptr) return fail(B200_ERR_INVALID_ARGUMENT, "null params");
+  const int rc = check_cache(&p->cache, p->dtype);
+  if (rc != B200_OK) return rc;
+  if (p->num_query_heads <= 0 || p->num_query_heads % p->cache.num_kv_heads != 0)
+    return fail(B200_ERR_INVALID_ARGUMENT,
+                "num_query_heads must be a multiple of num_kv_heads for GQA");
+  if (p->num_seqs < 0 || p->num_tokens < 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "negative sizes");
+  if (p->block_table_stride < 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "negative block_table_stride");
+  return B200_OK;
+}
+
+b200::AttnFp8Args attention_args(const B200AttentionFp8Params& p) {
+  b200::AttnFp8Args a{};
+  const B200Fp8Cache& c = p.cache;
+  a.q = p.query;
+  a.q_srow = p.q_stride_row;
+  a.q_shead = p.q_stride_head;
+  a.kc = static_cast<const uint8_t*>(c.key_cache);
+  a.vc = static_cast<const uint8_t*>(c.value_cache);
+  a.ks = c.key_scale;
+  a.vs = c.value_scale;
+  a.layer = c.layer_idx;
+  a.nb = c.total_blocks;
+  a.bs = c.block_size;
+  a.hkv = c.num_kv_heads;
+  a.head_dim = c.head_dim;
+  a.hq = p.num_query_heads;
+  a.group = p.num_query_heads / c.num_kv_heads;
+  a.bt = p.block_tables;
+  a.bt_stride = p.block_table_stride;
+  a.ctx_lens = p.context_lens;
+  a.S = p.num_seqs;
+  a.scale = p.scale;
+  a.out = p.out;
+  a.o_srow = p.o_stride_row;
+  a.o_shead = p.o_stride_head;
+  a.status = p.status_word;
+  return a;
+}
+
+bool has_arrays(const B200AttentionFp8Params& p) {
+  return has_arrays(p.cache) && p.query && p.out && p.block_tables && p.context_lens;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t b200_append_fp8_workspace_bytes(const B200Fp8Cache* cache, int32_t num_tokens) {
+  if (cache == nullptr || cache->total_blocks <= 0 || num_tokens <= 0) return 0;
+  return b200::append_fp8_scratch_bytes(cache->total_blocks, num_tokens);
+}
+
+int b200_reshape_and_cache_fp8(const B200Fp8Cache* cache, int32_t dtype, const void* key,
+                               int64_t k_stride_token, int64_t k_stride_head, const void* value,
+                               int64_t v_stride_token, int64_t v_stride_head,
+                               const int64_t* slot_mapping, int32_t num_tokens, void* workspace,
+                               size_t workspace_bytes, int32_t* status_word, void* stream) {
+  b200::NvtxRange nvtx_range("b200_reshape_and_cache_fp8");
+  int rc = check_cache(cache, dtype);
+  if (rc != B200_OK) return rc;
+  if (num_tokens < 0) return fail(B200_ERR_INVALID_ARGUMENT, "num_tokens < 0");
+  if (num_tokens == 0) return B200_OK;
+  if (!has_arrays(*cache) || !key || !value || !slot_mapping)
+    return fail(B200_ERR_INVALID_ARGUMENT, "null pointer");
+  b200::AppendFp8Args a{};
+  rc = append_args(*cache, slot_mapping, num_tokens, workspace, workspace_bytes, status_word, &a);
+  if (rc != B200_OK) return rc;
+  a.key = key;
+  a.value = value;
+  a.k_stok = k_stride_token;
+  a.k_shead = k_stride_head;
+  a.v_stok = v_stride_token;
+  a.v_shead = v_stride_head;
+  cudaError_t e =
+      b200::launch_append_fp8(a, dtype, num_sms(), static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "reshape_and_cache_fp8");
+  return B200_OK;
+}
+
+int b200_rope_reshape_and_cache_fp8(const B200Fp8Cache* cache, int32_t dtype, const void* qkv,
+                                    int64_t qkv_stride_token, int32_t num_tokens,
+                                    int32_t num_query_heads, const int64_t* positions,
+                                    const float* inv_freq, void* q_out,
+                                    int64_t q_out_stride_token, const int64_t* slot_mapping,
+                                    void* workspace, size_t workspace_bytes,
+                                    int32_t* status_word, void* stream) {
+  b200::NvtxRange nvtx_range("b200_rope_reshape_and_cache_fp8");
+  int rc = check_cache(cache, dtype);
+  if (rc != B200_OK) return rc;
+  const int D = cache->head_dim, hkv = cache->num_kv_heads;
+  if (D % 2 != 0) return fail(B200_ERR_INVALID_ARGUMENT, "head_dim must be even");
+  if (num_query_heads <= 0 || num_query_heads % hkv != 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "num_query_heads must be a multiple of num_kv_heads");
+  if (num_tokens < 0) return fail(B200_ERR_INVALID_ARGUMENT, "num_tokens < 0");
+  if (num_tokens == 0) return B200_OK;
+  if (qkv_stride_token < static_cast<int64_t>(num_query_heads + 2 * hkv) * D && num_tokens > 1)
+    return fail(B200_ERR_INVALID_ARGUMENT, "qkv_stride_token shorter than a q,k,v row");
+  if (q_out_stride_token < static_cast<int64_t>(num_query_heads) * D && num_tokens > 1)
+    return fail(B200_ERR_INVALID_ARGUMENT, "q_out_stride_token shorter than a q row");
+  if (!has_arrays(*cache) || !qkv || !positions || !inv_freq || !q_out || !slot_mapping)
+    return fail(B200_ERR_INVALID_ARGUMENT, "null pointer");
+  b200::AppendFp8Args a{};
+  rc = append_args(*cache, slot_mapping, num_tokens, workspace, workspace_bytes, status_word, &a);
+  if (rc != B200_OK) return rc;
+  const int es = esize_of(dtype);
+  a.q_in = qkv;
+  a.q_stok = qkv_stride_token;
+  a.q_out = q_out;
+  a.qo_stok = q_out_stride_token;
+  a.hq = num_query_heads;
+  a.key = static_cast<const char*>(qkv) + static_cast<int64_t>(num_query_heads) * D * es;
+  a.value = static_cast<const char*>(a.key) + static_cast<int64_t>(hkv) * D * es;
+  a.k_stok = a.v_stok = qkv_stride_token;
+  a.k_shead = a.v_shead = D;
+  a.positions = positions;
+  a.inv_freq = inv_freq;
+  cudaError_t e =
+      b200::launch_append_fp8(a, dtype, num_sms(), static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "rope_reshape_and_cache_fp8");
+  return B200_OK;
+}
+
+int b200_gather_cache_fp8(const B200Fp8Cache* cache, int32_t dtype, const int64_t* slots,
+                          int64_t n, void* k_out, void* v_out, int32_t* status_word,
+                          void* stream) {
+  b200::NvtxRange nvtx_range("b200_gather_cache_fp8");
+  const int rc = check_cache(cache, dtype);
+  if (rc != B200_OK) return rc;
+  if (n < 0) return fail(B200_ERR_INVALID_ARGUMENT, "n < 0");
+  if (n == 0) return B200_OK;
+  if (!has_arrays(*cache) || !slots || !k_out || !v_out)
+    return fail(B200_ERR_INVALID_ARGUMENT, "null pointer");
+  b200::GatherFp8Args a{};
+  a.kc = static_cast<const uint8_t*>(cache->key_cache);
+  a.vc = static_cast<const uint8_t*>(cache->value_cache);
+  a.ks = cache->key_scale;
+  a.vs = cache->value_scale;
+  a.layer = cache->layer_idx;
+  a.nb = cache->total_blocks;
+  a.bs = cache->block_size;
+  a.hkv = cache->num_kv_heads;
+  a.head_dim = cache->head_dim;
+  a.slots = slots;
+  a.n = n;
+  a.k_out = k_out;
+  a.v_out = v_out;
+  a.status = status_word;
+  cudaError_t e =
+      b200::launch_gather_fp8(a, dtype, num_sms(), static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "gather_cache_fp8");
+  return B200_OK;
+}
+
+size_t b200_paged_decode_fp8_workspace_bytes(const B200AttentionFp8Params* p) {
+  (void)p;
+  return 0;
+}
+
+int b200_paged_decode_fp8(const B200AttentionFp8Params* p, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  b200::NvtxRange nvtx_range("b200_paged_decode_fp8");
+  (void)workspace;
+  (void)workspace_bytes;
+  const int rc = check_attention(p);
+  if (rc != B200_OK) return rc;
+  if (p->num_seqs == 0) return B200_OK;
+  if (!has_arrays(*p)) return fail(B200_ERR_INVALID_ARGUMENT, "null pointer");
+  b200::AttnFp8Args a = attention_args(*p);
+  a.query_rows = p->query_rows;
+  cudaError_t e = b200::launch_row_fp8(a, p->dtype, p->num_seqs, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "paged_decode_fp8");
+  return B200_OK;
+}
+
+size_t b200_paged_prefill_fp8_workspace_bytes(const B200AttentionFp8Params* p) {
+  (void)p;
+  return 0;
+}
+
+int b200_paged_prefill_fp8(const B200AttentionFp8Params* p, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  b200::NvtxRange nvtx_range("b200_paged_prefill_fp8");
+  (void)workspace;
+  (void)workspace_bytes;
+  const int rc = check_attention(p);
+  if (rc != B200_OK) return rc;
+  if (p->num_seqs == 0 || p->num_tokens == 0) return B200_OK;
+  if (!has_arrays(*p) || !p->cu_seqlens) return fail(B200_ERR_INVALID_ARGUMENT, "null pointer");
+  b200::AttnFp8Args a = attention_args(*p);
+  a.cu_q = p->cu_seqlens;
+  cudaError_t e =
+      b200::launch_row_fp8(a, p->dtype, p->num_tokens, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "paged_prefill_fp8");
+  return B200_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,435 @@
+// Append to, and read back from, an 8-bit paged cache (e4m3 numbers, one power-of-two scale per
+// layer, block and KV head).
+//
+// For block b and head h let R be the call's rows with a slot in b and m the largest finite |x| of
+// those rows (after rotation, for keys).  need = the smallest power of two s with m <= 448 s.
+//   new scale = need                    if R writes the block's first slot (the block begins anew)
+//             = max(old scale, need)    otherwise
+//   a held code c becomes rn(c * old / new) where the scale grew; a row's entry becomes rn(x / new).
+// Powers of two make both divisions exact, so each entry is rounded once (a held one again only
+// where it falls below e4m3's smallest normal number).
+//
+// One CTA owns a block: it lists the block's rows in the call, takes the maxima, rescales what the
+// block holds and writes the rows, so no two CTAs touch one scale.  In calls of up to
+// kAppendScanRows rows every row's CTA scans the call's slots for its block (the CTA of the first
+// such row goes on, the others leave); larger calls first count the rows of each block and list
+// the rows where a run of rows of one block starts.
+#include "fp8.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kAppendThreads = 256;
+constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kChunkRows = 16;    // rows of a block handled per pass
+constexpr int kMaxBlockSize = 1024;
+
+// cos and sin of pos * inv_freq, each in two parts (hi + lo).  The product is formed and reduced
+// to [-pi/4, pi/4] in 64 bits (at position 30,000 a 32-bit product alone is off by 1e-3 rad) and
+// the Taylor series there end with a remainder below 2e-14.
+struct Turn {
+  float ch, sh, cl, sl;
+};
+__device__ __forceinline__ Turn turn_of(int64_t pos, float inv_freq) {
+  const double a = static_cast<double>(pos) * static_cast<double>(inv_freq);
+  const double k = rint(a * 0.6366197723675814);                    // 2 / pi
+  double r = fma(-k, 1.5707963267948966, a);                        // pi / 2 in two parts
+  r = fma(-k, 6.123233995736766e-17, r);
+  const double z = r * r;
+  double s = 1.0 / 6227020800.0;                                    // 1 / 13!
+  s = fma(s, z, -1.0 / 39916800.0);
+  s = fma(s, z, 1.0 / 362880.0);
+  s = fma(s, z, -1.0 / 5040.0);
+  s = fma(s, z, 1.0 / 120.0);
+  s = fma(s, z, -1.0 / 6.0);
+  s = fma(s * z, r, r);
+  double c = -1.0 / 87178291200.0;                                  // -1 / 14!
+  c = fma(c, z, 1.0 / 479001600.0);
+  c = fma(c, z, -1.0 / 3628800.0);
+  c = fma(c, z, 1.0 / 40320.0);
+  c = fma(c, z, -1.0 / 720.0);
+  c = fma(c, z, 1.0 / 24.0);
+  c = fma(c, z, -0.5);
+  c = fma(c, z, 1.0);
+  const int quarter = static_cast<int>(static_cast<int64_t>(k) & 3);
+  if (quarter & 1) {
+    const double t = s;
+    s = c;
+    c = -t;
+  }
+  if (quarter & 2) {
+    s = -s;
+    c = -c;
+  }
+  Turn t;
+  t.ch = static_cast<float>(c);
+  t.cl = static_cast<float>(c - t.ch);
+  t.sh = static_cast<float>(s);
+  t.sl = static_cast<float>(s - t.sh);
+  return t;
+}
+
+// x * c + y * s rounded once from twice fp32's precision (products split by fma, two-sum), so that
+// a rotated key lands on the same code as its 64-bit value.
+__device__ __forceinline__ float mul_add2(float x, float ch, float cl, float y, float sh, float sl) {
+  const float p = __fmul_rn(x, ch), q = __fmul_rn(y, sh);
+  const float e = fmaf(x, cl, fmaf(x, ch, -p)) + fmaf(y, sl, fmaf(y, sh, -q));
+  const float d = __fadd_rn(p, q);
+  const float bb = __fsub_rn(d, p);
+  const float err = __fadd_rn(__fsub_rn(p, __fsub_rn(d, bb)), __fsub_rn(q, bb));
+  return __fadd_rn(d, err + e);
+}
+
+// Smallest power of two s with amax <= 448 s (448 = 1.75 * 2^8), at least 2^-100.
+__device__ __forceinline__ float scale_for(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  int e = static_cast<int>(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = max(e, 27);
+  return __uint_as_float(static_cast<uint32_t>(e) << 23);
+}
+
+__device__ __forceinline__ bool is_pow2(float s) {
+  return (__float_as_uint(s) & 0x7fffffu) == 0;
+}
+
+struct RowList {
+  int32_t row[kChunkRows];
+  int32_t off[kChunkRows];
+  int32_t n;
+  int32_t next;  // row to go on from
+};
+
+// The next rows (at most kChunkRows) of block slots [s0, s0 + bs) at or after row `pos`, in order;
+// stops early once `want` rows have been found.  Called by the whole CTA.
+__device__ void next_rows(const AppendFp8Args& a, int64_t s0, int pos, int want, RowList& list,
+                          int32_t* warp_n) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int found = 0;
+  while (pos < a.num_tokens && found < want && found < kChunkRows) {
+    const int r = pos + tid;
+    const int64_t slot = r < a.num_tokens ? a.slots[r] : -1;
+    const bool in = slot >= s0 && slot < s0 + a.bs;
+    const uint32_t m = __ballot_sync(0xffffffffu, in);
+    if (lane == 0) warp_n[warp] = __popc(m);
+    __syncthreads();
+    int before = found, total = 0;
+#pragma unroll
+    for (int w = 0; w < kAppendWarps; ++w) {
+      if (w < warp) before += warp_n[w];
+      total += warp_n[w];
+    }
+    const int at = before + __popc(m & ((1u << lane) - 1u));
+    if (in && at < kChunkRows) {
+      list.row[at] = r;
+      list.off[at] = static_cast<int32_t>(slot - s0);
+      if (at == kChunkRows - 1) list.next = r + 1;
+    }
+    if (found + total < kChunkRows && tid == 0) list.next = pos + kAppendThreads;
+    found += total;
+    pos += kAppendThreads;
+    __syncthreads();
+  }
+  if (tid == 0) list.n = min(found, kChunkRows);
+  __syncthreads();
+}
+
+template <typename T, bool ROPE>
+__global__ void __launch_bounds__(kAppendThreads) append_fp8_kernel(AppendFp8Args a, int q_ctas,
+                                                                    int q_rows) {
+  extern __shared__ __align__(16) float sm[];
+  __shared__ RowList list;
+  __shared__ int32_t warp_n[kAppendWarps];
+  __shared__ uint32_t written[kMaxBlockSize / 32];
+  __shared__ int32_t fresh_s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int D = a.head_dim, half = D / 2;
+
+  // ---- queries: rotated and rounded to the call's type ---------------------------------------
+  if (ROPE && static_cast<int>(blockIdx.x) < q_ctas) {
+    const int r0 = blockIdx.x * q_rows, r1 = min(a.num_tokens, r0 + q_rows);
+    float2* cs = reinterpret_cast<float2*>(sm);  // [q_rows][half]: cos, sin
+    for (int w = tid; w < (r1 - r0) * half; w += kAppendThreads) {
+      const int r = w / half, i = w - r * half;
+      const Turn t = turn_of(a.positions[r0 + r], a.inv_freq[i]);
+      cs[w] = make_float2(t.ch, t.sh);
+    }
+    __syncthreads();
+    const int per_row = a.hq * half;
+    for (int w = tid; w < (r1 - r0) * per_row; w += kAppendThreads) {
+      const int r = w / per_row, rem = w - r * per_row;
+      const int h = rem / half, i = rem - h * half;
+      const T* src = static_cast<const T*>(a.q_in) + (r0 + r) * a.q_stok + h * D;
+      T* dst = static_cast<T*>(a.q_out) + (r0 + r) * a.qo_stok + h * D;
+      const float x1 = to_f32<T>(src[i]), x2 = to_f32<T>(src[i + half]);
+      const float2 cv = cs[r * half + i];
+      dst[i] = from_f32<T>(x1 * cv.x - x2 * cv.y);
+      dst[i + half] = from_f32<T>(x2 * cv.x + x1 * cv.y);
+    }
+    return;
+  }
+
+  // ---- keys and values, block by block -------------------------------------------------------
+  const int64_t total_slots = static_cast<int64_t>(a.nb) * a.bs;
+  Turn* cs = reinterpret_cast<Turn*>(sm);              // [kChunkRows][half]
+  float* amax = sm + (ROPE ? kChunkRows * 2 * D : 0);  // [2 * hkv]
+  const bool scan = a.runs == nullptr;
+  const int unit0 = static_cast<int>(blockIdx.x) - q_ctas;
+  const int step = static_cast<int>(gridDim.x) - q_ctas;
+  const int units = scan ? a.num_tokens : *a.num_runs;
+  for (int unit = unit0; unit < units; unit += step) {
+    const int t = scan ? unit : a.runs[unit];
+    const int64_t slot = a.slots[t];
+    if (slot < 0 || slot >= total_slots) {
+      if (slot >= total_slots && tid == 0) flag_status(a.status, B200_DEVICE_BAD_SLOT);
+      continue;
+    }
+    const int64_t blk = slot / a.bs, s0 = blk * a.bs;
+    int want;
+    if (scan) {
+      bool earlier = false;
+      want = 0;
+      for (int r0 = 0; r0 < a.num_tokens; r0 += kAppendThreads) {
+        const int r = r0 + tid;
+        const int64_t o = r < a.num_tokens ? a.slots[r] : -1;
+        const bool in = o >= s0 && o < s0 + a.bs;
+        earlier |= in && r < t;
+        want += __syncthreads_count(in);
+      }
+      if (__syncthreads_or(earlier)) continue;  // the block's first row owns it
+    } else {
+      if (a.num_tokens - a.first[blk] != t) continue;
+      want = a.count[blk];
+    }
+
+    // maxima over all of the block's rows, kChunkRows at a time
+    for (int i = tid; i < 2 * a.hkv; i += kAppendThreads) amax[i] = 0.f;
+    for (int i = tid; i < (a.bs + 31) / 32; i += kAppendThreads) written[i] = 0u;
+    if (tid == 0) fresh_s = 0;
+    __syncthreads();
+    int pos = t, seen = 0, chunks = 0;
+    const auto load_chunk = [&]() {
+      next_rows(a, s0, pos, want - seen, list, warp_n);
+      pos = list.next;
+      seen += list.n;
+      if (ROPE) {
+        for (int w = tid; w < list.n * half; w += kAppendThreads) {
+          const int r = w / half, i = w - r * half;
+          cs[w] = turn_of(a.positions[list.row[r]], a.inv_freq[i]);
+        }
+      }
+      __syncthreads();
+    };
+    // entry d and (rotary keys) d + half of row r of the chunk, head h
+    const auto entry = [&](int task, int r, int d, float& x1, float& x2) {
+      const int h = task >> 1;
+      if (task & 1) {
+        const T* v = static_cast<const T*>(a.value) + list.row[r] * a.v_stok + h * a.v_shead;
+        x1 = to_f32<T>(v[d]);
+      } else {
+        const T* k = static_cast<const T*>(a.key) + list.row[r] * a.k_stok + h * a.k_shead;
+        x1 = to_f32<T>(k[d]);
+        if (ROPE) {
+          const float y = to_f32<T>(k[d + half]);
+          const Turn w = cs[r * half + d];
+          x2 = mul_add2(y, w.ch, w.cl, x1, w.sh, w.sl);
+          x1 = mul_add2(x1, w.ch, w.cl, -y, w.sh, w.sl);
+        }
+      }
+    };
+    do {
+      load_chunk();
+      ++chunks;
+      if (tid < list.n) {
+        atomicOr(&written[list.off[tid] >> 5], 1u << (list.off[tid] & 31));
+        if (list.off[tid] == 0) fresh_s = 1;
+      }
+      for (int task = warp; task < 2 * a.hkv; task += kAppendWarps) {
+        const bool pair = ROPE && !(task & 1);
+        float m = 0.f;
+        for (int r = 0; r < list.n; ++r)
+          for (int d = lane; d < (pair ? half : D); d += 32) {
+            float x1, x2 = 0.f;
+            entry(task, r, d, x1, x2);
+            x1 = fabsf(x1);
+            x2 = pair ? fabsf(x2) : 0.f;
+            if (x1 < INFINITY) m = fmaxf(m, x1);  // false for NaN too
+            if (x2 < INFINITY) m = fmaxf(m, x2);
+          }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) amax[task] = fmaxf(amax[task], m);
+      }
+      __syncthreads();
+    } while (seen < want);
+
+    const bool fresh = fresh_s != 0;
+    const bool one_chunk = chunks == 1;
+    const int64_t cache_blk = static_cast<int64_t>(a.layer) * a.nb + blk;
+    pos = t;
+    seen = 0;
+    for (int ch = 0; ch < chunks; ++ch) {
+      if (!one_chunk) load_chunk();
+      for (int task = warp; task < 2 * a.hkv; task += kAppendWarps) {
+        const int h = task >> 1;
+        const bool is_v = task & 1;
+        float* sp = (is_v ? a.vs : a.ks) + cache_blk * a.hkv + h;
+        uint8_t* codes = (is_v ? a.vc : a.kc) + (cache_blk * a.bs * a.hkv + h) * D;
+        const int64_t row_bytes = static_cast<int64_t>(a.hkv) * D;
+        float s_new;
+        if (ch == 0) {
+          float old = *sp;
+          if (!(old > 0.f) || isinf(old)) old = 0.f;  // never written
+          s_new = scale_for(amax[task]);
+          if (!fresh) {
+            s_new = fmaxf(s_new, old);
+            if (s_new != old) {
+              const float ratio = old / s_new;
+              for (int o = 0; o < a.bs; ++o) {
+                if ((written[o >> 5] >> (o & 31)) & 1u) continue;
+                for (int d = lane; d < D; d += 32) {
+                  uint8_t* c = codes + o * row_bytes + d;
+                  *c = f32_to_e4m3(e4m3_to_f32(*c) * ratio);
+                }
+              }
+            }
+          }
+          __syncwarp();
+          if (lane == 0) *sp = s_new;
+          if (lane == 0) amax[task] = s_new;  // for the chunks that follow
+        } else {
+          s_new = amax[task];
+        }
+        __syncwarp();
+        const bool pow2 = is_pow2(s_new);
+        const float inv = 1.f / s_new;
+        const bool pair = ROPE && !is_v;
+        for (int r = 0; r < list.n; ++r) {
+          uint8_t* c = codes + list.off[r] * row_bytes;
+          for (int d = lane; d < (pair ? half : D); d += 32) {
+            float x1, x2 = 0.f;
+            entry(task, r, d, x1, x2);
+            c[d] = f32_to_e4m3(pow2 ? x1 * inv : x1 / s_new);
+            if (pair) c[d + half] = f32_to_e4m3(pow2 ? x2 * inv : x2 / s_new);
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Rows per block, the first row of each block and the starts of runs of rows of one block.
+__global__ void __launch_bounds__(256) append_mark_kernel(AppendFp8Args a) {
+  const int64_t total_slots = static_cast<int64_t>(a.nb) * a.bs;
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r >= a.num_tokens) return;
+  const int64_t slot = a.slots[r];
+  if (slot < 0) return;
+  if (slot >= total_slots) {
+    flag_status(a.status, B200_DEVICE_BAD_SLOT);
+    return;
+  }
+  const int64_t blk = slot / a.bs;
+  atomicAdd(&a.count[blk], 1);
+  const int64_t prev = r > 0 ? a.slots[r - 1] : -1;
+  if (prev < blk * a.bs || prev >= (blk + 1) * a.bs) {
+    atomicMax(&a.first[blk], a.num_tokens - r);
+    a.runs[atomicAdd(a.num_runs, 1)] = r;
+  }
+}
+
+// ---- read back -------------------------------------------------------------------------------
+// code * scale in the output's type; what an f16 cannot hold becomes +-65504.
+template <typename T>
+__device__ __forceinline__ T value_of(uint8_t c, float scale) {
+  return from_f32<T>(e4m3_to_f32(c) * scale);
+}
+template <>
+__device__ __forceinline__ __half value_of<__half>(uint8_t c, float scale) {
+  const float x = e4m3_to_f32(c) * scale;
+  return __float2half_rn(fabsf(x) > 65504.f ? copysignf(65504.f, x) : x);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) gather_fp8_kernel(GatherFp8Args a) {
+  const int64_t per_row = static_cast<int64_t>(a.hkv) * a.head_dim;
+  const int64_t total = per_row * a.n;
+  const int64_t slots = static_cast<int64_t>(a.nb) * a.bs;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t r = i / per_row, e = i - r * per_row;
+    const int64_t slot = a.slots[r];
+    if (slot < 0 || slot >= slots) {
+      if (slot >= slots && e == 0) flag_status(a.status, B200_DEVICE_BAD_SLOT);
+      static_cast<T*>(a.k_out)[i] = from_f32<T>(0.f);
+      static_cast<T*>(a.v_out)[i] = from_f32<T>(0.f);
+      continue;
+    }
+    const int64_t blk = static_cast<int64_t>(a.layer) * a.nb + slot / a.bs;
+    const int64_t at = (static_cast<int64_t>(a.layer) * slots + slot) * per_row + e;
+    const int64_t sc = blk * a.hkv + e / a.head_dim;
+    static_cast<T*>(a.k_out)[i] = value_of<T>(a.kc[at], a.ks[sc]);
+    static_cast<T*>(a.v_out)[i] = value_of<T>(a.vc[at], a.vs[sc]);
+  }
+}
+
+template <typename T>
+cudaError_t launch_append_t(const AppendFp8Args& a, int num_sms, cudaStream_t stream) {
+  const bool rope = a.positions != nullptr;
+  const int q_rows = a.num_tokens > 2048 ? 8 : 1;
+  const int q_ctas = rope ? (a.num_tokens + q_rows - 1) / q_rows : 0;
+  int kv_ctas = a.num_tokens;
+  if (a.runs != nullptr && kv_ctas > num_sms * 8) kv_ctas = num_sms * 8;
+  const size_t smem = ((rope ? kChunkRows * 2 * a.head_dim : 0) + 2 * a.hkv) * sizeof(float);
+  if (rope)
+    append_fp8_kernel<T, true><<<q_ctas + kv_ctas, kAppendThreads, smem, stream>>>(a, q_ctas, q_rows);
+  else
+    append_fp8_kernel<T, false><<<kv_ctas, kAppendThreads, smem, stream>>>(a, 0, 1);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t append_fp8_scratch_bytes(int nb, int num_tokens) {
+  if (num_tokens <= kAppendScanRows) return 0;
+  return (2 * static_cast<size_t>(nb) + 1 + num_tokens) * sizeof(int32_t);
+}
+
+cudaError_t launch_append_fp8(const AppendFp8Args& a, int dtype, int num_sms,
+                              cudaStream_t stream) {
+  if (a.num_tokens <= 0) return cudaSuccess;
+  if (a.runs != nullptr) {
+    // count, first and num_runs are adjacent
+    cudaError_t e = cudaMemsetAsync(a.count, 0, (2 * static_cast<size_t>(a.nb) + 1) * 4, stream);
+    if (e != cudaSuccess) return e;
+    append_mark_kernel<<<(a.num_tokens + 255) / 256, 256, 0, stream>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  switch (dtype) {
+    case B200_DTYPE_BF16: return launch_append_t<__nv_bfloat16>(a, num_sms, stream);
+    case B200_DTYPE_F16: return launch_append_t<__half>(a, num_sms, stream);
+    case B200_DTYPE_F32: return launch_append_t<float>(a, num_sms, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_gather_fp8(const GatherFp8Args& a, int dtype, int num_sms,
+                              cudaStream_t stream) {
+  if (a.n <= 0) return cudaSuccess;
+  const int64_t total = a.n * a.hkv * a.head_dim;
+  int64_t blocks = (total + 255) / 256;
+  const int64_t cap = static_cast<int64_t>(num_sms) * 8;
+  if (blocks > cap) blocks = cap;
+  const int grid = static_cast<int>(blocks);
+  switch (dtype) {
+    case B200_DTYPE_BF16: gather_fp8_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a); break;
+    case B200_DTYPE_F16: gather_fp8_kernel<__half><<<grid, 256, 0, stream>>>(a); break;
+    case B200_DTYPE_F32: gather_fp8_kernel<float><<<grid, 256, 0, stream>>>(a); break;
+    default: return cudaErrorInvalidValue;
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace b200

@@ -309,6 +309,252 @@ def copy_blocks(src_key_cache: torch.Tensor, src_value_cache: Optional[torch.Ten
             _stream(dev)))
 
 
+# ---- 8-bit cache -------------------------------------------------------------------------------
+# Caches are float8_e4m3fn (L, NB, BS, Hkv, D) with fp32 scales (L, NB, Hkv): an entry stands for
+# code * scale of its layer, block and head.
+
+def fp8_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scale: torch.Tensor,
+              value_scale: torch.Tensor, layer_idx: int) -> N.Fp8Cache:
+    """The C struct of an 8-bit cache; checks types, shapes and layout."""
+    if key_cache.dim() != 5:
+        raise ValueError("key_cache must be 5-D (layers, blocks, block_size, heads, dim)")
+    if key_cache.dtype != torch.float8_e4m3fn or value_cache.dtype != torch.float8_e4m3fn:
+        raise ValueError("8-bit caches must be float8_e4m3fn")
+    if value_cache.shape != key_cache.shape:
+        raise ValueError("value_cache must have the key cache's shape and dtype")
+    L, NB, BS, H, D = key_cache.shape
+    want = (L, NB, H)
+    if key_scale.shape != want or value_scale.shape != want:
+        raise ValueError(f"scales must be (layers, blocks, heads) = {want}")
+    if key_scale.dtype != torch.float32 or value_scale.dtype != torch.float32:
+        raise ValueError("scales must be float32")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous() and
+            key_scale.is_contiguous() and value_scale.is_contiguous()):
+        raise ValueError("caches must be contiguous (L, NB, BS, Hkv, D), scales (L, NB, Hkv)")
+    return N.Fp8Cache(key_cache.data_ptr(), value_cache.data_ptr(), key_scale.data_ptr(),
+                      value_scale.data_ptr(), L, NB, BS, H, D, int(layer_idx))
+
+
+def _one_device(*tensors) -> torch.device:
+    """The CUDA device that all the tensors are on."""
+    _require_cuda(*tensors)
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors are on {dev} and on {t.device}")
+    return dev
+
+
+def _dtype_code(t: torch.Tensor, name: str) -> int:
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"unsupported {name} dtype {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _check_slots(slots: torch.Tensor, rows: Optional[int]) -> None:
+    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        raise ValueError("slots must be a contiguous int64 vector")
+    if rows is not None and slots.shape[0] != rows:
+        raise ValueError(f"{slots.shape[0]} slots for {rows} rows")
+
+
+def _append_workspace(c: N.Fp8Cache, n: int, dev: torch.device, stream: int):
+    need = N.lib().b200_append_fp8_workspace_bytes(ctypes.byref(c), n)
+    return _WORKSPACE.get(dev, need, stream) if need else None
+
+
+def reshape_and_cache_fp8(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+                          value_cache: torch.Tensor, key_scale: torch.Tensor,
+                          value_scale: torch.Tensor, layer_idx: int,
+                          slot_mapping: torch.Tensor) -> None:
+    """``reshape_and_cache`` into an 8-bit cache: key/value (Ntok, Hkv, D) of any float type and
+    strides (D contiguous).  A block's scale becomes the smallest power of two that holds the
+    call's rows when the call writes the block's first slot, and only ever grows after that (the
+    entries that the block holds are then rounded to the new scale)."""
+    c = fp8_cache(key_cache, value_cache, key_scale, value_scale, layer_idx)
+    if key.dim() != 3 or key.shape != value.shape or key.shape[1:] != key_cache.shape[3:]:
+        raise ValueError("key and value must be (tokens, Hkv, D) with the cache's heads and dim")
+    if key.dtype != value.dtype:
+        raise ValueError("key and value must have one dtype")
+    code = _dtype_code(key, "key")
+    _check_slots(slot_mapping, key.shape[0])
+    if key.stride(-1) != 1 or value.stride(-1) != 1:
+        raise ValueError("head dim must be contiguous")
+    dev = _one_device(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
+    with torch.cuda.device(dev):
+        stream = _stream(dev)
+        n = key.shape[0]
+        ws = _append_workspace(c, n, dev, stream)
+        N.check(N.lib().b200_reshape_and_cache_fp8(
+            ctypes.byref(c), code, key.data_ptr(), key.stride(0), key.stride(1),
+            value.data_ptr(), value.stride(0), value.stride(1), slot_mapping.data_ptr(), n,
+            _ptr(ws), 0 if ws is None else ws.numel(), status_word(dev).data_ptr(), stream))
+
+
+def rope_reshape_and_cache_fp8(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                               num_query_heads: int, key_cache: torch.Tensor,
+                               value_cache: torch.Tensor, key_scale: torch.Tensor,
+                               value_scale: torch.Tensor, layer_idx: int,
+                               slot_mapping: torch.Tensor,
+                               q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``rope_reshape_and_cache`` into an 8-bit cache: qkv (Ntok, (Hq + 2*Hkv) * D) rows
+    [q | k | v] of any float type; rotated k and v go to their slots as
+    ``reshape_and_cache_fp8`` stores them; returns the rotated q (Ntok, Hq, D) of qkv's type.
+    Angles are formed in 64 bits and a rotated key is rounded once, to its code."""
+    c = fp8_cache(key_cache, value_cache, key_scale, value_scale, layer_idx)
+    if qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise ValueError("qkv must be (tokens, row) with unit stride inside a row")
+    code = _dtype_code(qkv, "qkv")
+    n, hq = qkv.shape[0], int(num_query_heads)
+    _check_slots(slot_mapping, n)
+    if (positions.dtype != torch.int64 or positions.shape != (n,) or
+            not positions.is_contiguous()):
+        raise ValueError("positions must be a contiguous int64 vector of one entry per row")
+    if (inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or
+            inv_freq.numel() != c.head_dim // 2):
+        raise ValueError("inv_freq must be contiguous float32 with head_dim / 2 entries")
+    if qkv.shape[1] < (hq + 2 * c.num_kv_heads) * c.head_dim:
+        raise ValueError("qkv rows shorter than the q, k and v heads")
+    if q_out is None:
+        q_out = torch.empty((n, hq, c.head_dim), dtype=qkv.dtype, device=qkv.device)
+    elif q_out.shape != (n, hq, c.head_dim) or q_out.dtype != qkv.dtype:
+        raise ValueError("q_out must be (tokens, Hq, D) of qkv's dtype")
+    if q_out.stride(2) != 1 or (hq > 1 and q_out.stride(1) != c.head_dim):
+        raise ValueError("q_out must have contiguous heads")
+    dev = _one_device(qkv, positions, inv_freq, key_cache, value_cache, key_scale, value_scale,
+                      slot_mapping, q_out)
+    with torch.cuda.device(dev):
+        stream = _stream(dev)
+        ws = _append_workspace(c, n, dev, stream)
+        N.check(N.lib().b200_rope_reshape_and_cache_fp8(
+            ctypes.byref(c), code, qkv.data_ptr(), qkv.stride(0), n, hq, positions.data_ptr(),
+            inv_freq.data_ptr(), q_out.data_ptr(), q_out.stride(0), slot_mapping.data_ptr(),
+            _ptr(ws), 0 if ws is None else ws.numel(), status_word(dev).data_ptr(), stream))
+    return q_out
+
+
+def gather_cache_fp8(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scale: torch.Tensor,
+                     value_scale: torch.Tensor, layer_idx: int, slots: torch.Tensor,
+                     dtype: torch.dtype = torch.bfloat16):
+    """The values (code * scale) that an 8-bit cache holds in the given slots: key and value,
+    each (n, Hkv, D) of ``dtype``; zeros for slots below 0."""
+    c = fp8_cache(key_cache, value_cache, key_scale, value_scale, layer_idx)
+    if dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {dtype}")
+    _check_slots(slots, None)
+    dev = _one_device(key_cache, value_cache, key_scale, value_scale, slots)
+    out = torch.empty((2, slots.shape[0], c.num_kv_heads, c.head_dim), dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        N.check(N.lib().b200_gather_cache_fp8(
+            ctypes.byref(c), _DTYPES[dtype], slots.data_ptr(), slots.shape[0], out[0].data_ptr(),
+            out[1].data_ptr(), status_word(dev).data_ptr(), _stream(dev)))
+    return out[0], out[1]
+
+
+def attention_fp8_params(query, key_cache, value_cache, key_scale, value_scale, layer_idx,
+                         block_tables, context_lens, scale, out, max_context_len, query_rows=None,
+                         cu_seqlens=None, max_query_len=0, prefill_blocks=-1):
+    """The C struct of an attention call over an 8-bit cache; checks what the struct cannot say."""
+    p = N.AttentionFp8Params()
+    p.cache = fp8_cache(key_cache, value_cache, key_scale, value_scale, layer_idx)
+    if query.dim() != 3 or query.stride(-1) != 1:
+        raise ValueError("query must be (rows, Hq, D) with the head dim contiguous")
+    if query.shape[2] != p.cache.head_dim:
+        raise ValueError(f"query head dim {query.shape[2]} != cache head dim {p.cache.head_dim}")
+    p.dtype = _dtype_code(query, "query")
+    if out.dtype != query.dtype or out.shape != query.shape or out.stride(-1) != 1:
+        raise ValueError("out must have the query's shape and dtype, the head dim contiguous")
+    if block_tables.dtype != torch.int32 or context_lens.dtype != torch.int32:
+        raise ValueError("block_tables and context_lens must be int32")
+    if block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be (S, max_blocks) with unit stride along a row")
+    if context_lens.dim() != 1 or not context_lens.is_contiguous():
+        raise ValueError("context_lens must be a contiguous (S,) tensor")
+    S = context_lens.shape[0]
+    if block_tables.shape[0] < S:
+        raise ValueError("block_tables has fewer rows than context_lens has sequences")
+    if S > 1 and block_tables.stride(0) < block_tables.shape[1]:
+        raise ValueError("block_tables rows must not overlap")
+    if query_rows is not None and (query_rows.dtype != torch.int32 or query_rows.shape != (S,) or
+                                   not query_rows.is_contiguous()):
+        raise ValueError("query_rows must be int32 with one entry per sequence")
+    if cu_seqlens is None:
+        if query_rows is None and query.shape[0] < S:
+            raise ValueError(f"query has {query.shape[0]} rows, the batch needs {S}")
+    elif (cu_seqlens.dtype != torch.int64 or cu_seqlens.shape != (S + 1,) or
+          not cu_seqlens.is_contiguous()):
+        raise ValueError("cu_seqlens must be a contiguous int64 (S+1,) tensor")
+    p.query, p.q_stride_row, p.q_stride_head = query.data_ptr(), query.stride(0), query.stride(1)
+    p.out, p.o_stride_row, p.o_stride_head = out.data_ptr(), out.stride(0), out.stride(1)
+    p.num_query_heads = query.shape[1]
+    p.block_tables, p.block_table_stride = block_tables.data_ptr(), block_tables.shape[1]
+    if S > 1:
+        p.block_table_stride = block_tables.stride(0)
+    p.context_lens, p.num_seqs = context_lens.data_ptr(), S
+    # no sequence reaches past its row of the table
+    p.max_context_len = min(int(max_context_len), block_tables.shape[1] * p.cache.block_size)
+    p.scale = float(scale)
+    p.query_rows, p.cu_seqlens = _ptr(query_rows), _ptr(cu_seqlens)
+    p.num_tokens, p.max_query_len = query.shape[0], int(max_query_len)
+    p.prefill_blocks = int(prefill_blocks)
+    return p
+
+
+def paged_decode_fp8(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                     key_scale: torch.Tensor, value_scale: torch.Tensor, layer_idx: int,
+                     block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float,
+                     max_context_len: int, out: Optional[torch.Tensor] = None,
+                     query_rows: Optional[torch.Tensor] = None,
+                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_decode`` over an 8-bit cache: query (rows, Hq, D) of any float type, one row per
+    sequence (or ``query_rows``); returns out (rows, Hq, D) of the query's type."""
+    if out is None:
+        out = torch.empty_like(query)
+    p = attention_fp8_params(query, key_cache, value_cache, key_scale, value_scale, layer_idx,
+                             block_tables, context_lens, scale, out, max_context_len, query_rows)
+    dev = _one_device(query, key_cache, value_cache, key_scale, value_scale, block_tables,
+                      context_lens, out, query_rows, workspace)
+    p.status_word = status_word(dev).data_ptr()
+    L = N.lib()
+    with torch.cuda.device(dev):
+        stream = _stream(dev)
+        need = L.b200_paged_decode_fp8_workspace_bytes(ctypes.byref(p))
+        ws = workspace if workspace is not None else (
+            _WORKSPACE.get(dev, need, stream) if need else None)
+        N.check(L.b200_paged_decode_fp8(ctypes.byref(p), _ptr(ws),
+                                        0 if ws is None else ws.numel() * ws.element_size(),
+                                        stream))
+    return out
+
+
+def paged_prefill_fp8(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                      key_scale: torch.Tensor, value_scale: torch.Tensor, layer_idx: int,
+                      block_tables: torch.Tensor, cu_seqlens: torch.Tensor,
+                      context_lens: torch.Tensor, scale: float, max_query_len: int,
+                      max_context_len: int, out: Optional[torch.Tensor] = None,
+                      prefill_blocks: Optional[int] = None) -> torch.Tensor:
+    """``paged_prefill`` over an 8-bit cache (prefill chunks and mixed steps): query (Ntok, Hq, D)
+    of any float type.  ``prefill_blocks``: how many cache blocks the sequences with more than one
+    new token hold together, where the caller knows it; it bounds the call's scratch memory."""
+    if out is None:
+        out = torch.empty_like(query)
+    p = attention_fp8_params(query, key_cache, value_cache, key_scale, value_scale, layer_idx,
+                             block_tables, context_lens, scale, out, max_context_len,
+                             cu_seqlens=cu_seqlens, max_query_len=max_query_len,
+                             prefill_blocks=-1 if prefill_blocks is None else prefill_blocks)
+    dev = _one_device(query, key_cache, value_cache, key_scale, value_scale, block_tables,
+                      cu_seqlens, context_lens, out)
+    p.status_word = status_word(dev).data_ptr()
+    L = N.lib()
+    with torch.cuda.device(dev):
+        stream = _stream(dev)
+        need = L.b200_paged_prefill_fp8_workspace_bytes(ctypes.byref(p))
+        ws = _WORKSPACE.get(dev, need, stream) if need else None
+        N.check(L.b200_paged_prefill_fp8(ctypes.byref(p), _ptr(ws),
+                                         0 if ws is None else ws.numel(), stream))
+    return out
+
+
 def paged_attention_masked(query: torch.Tensor, key_cache: torch.Tensor,
                            value_cache: torch.Tensor, layer_idx: int, gather_slots: torch.Tensor,
                            attention_mask: torch.Tensor, scaling: float) -> torch.Tensor:
