@@ -57,23 +57,8 @@ int num_sms() {
   return n;
 }
 
-}  // namespace b200
-
-using b200::cuda_fail;
-using b200::esize_of;
-using b200::fail;
-using b200::num_sms;
-
-namespace {
-
-// ---- tensor maps -----------------------------------------------------------------------------
 // cuTensorMapEncodeTiled is fetched through the runtime's driver entry point, so the library
 // needs no link-time dependency on libcuda.
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
@@ -88,6 +73,18 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
+}  // namespace b200
+
+using b200::cuda_fail;
+using b200::encode_fn;
+using b200::EncodeTiledFn;
+using b200::esize_of;
+using b200::fail;
+using b200::num_sms;
+
+namespace {
+
+// ---- tensor maps -----------------------------------------------------------------------------
 struct MapKey {
   const void* ptr;
   int64_t rows;

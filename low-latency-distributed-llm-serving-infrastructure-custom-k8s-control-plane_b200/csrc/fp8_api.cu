@@ -1,6 +1,7 @@
 // C ABI of the 8-bit paged cache (include/b200_paged.h, section 7): argument checks and launches.
 #include "api_common.cuh"
 #include "fp8.cuh"
+#include "fp8_decode.cuh"
 #include "nvtx.cuh"
 
 using b200::cuda_fail;
@@ -97,6 +98,114 @@ b200::AttnFp8Args attention_args(const B200AttentionFp8Params& p) {
   a.o_shead = p.o_stride_head;
   a.status = p.status_word;
   return a;
+}
+
+size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+
+// One launch of the tensor-core decode (up to kDecodeFp8MaxSeqs sequences) and its workspace.
+struct DecodePlan {
+  bool tensor_cores;
+  int nchunks, grid;
+  int64_t max_ctx;
+  size_t off_ml, off_o, total;
+};
+
+DecodePlan decode_plan(const B200AttentionFp8Params& p) {
+  const B200Fp8Cache& c = p.cache;
+  DecodePlan pl{};
+  const int64_t rows = static_cast<int64_t>(c.num_layers) * c.total_blocks * c.block_size;
+  pl.tensor_cores = (c.head_dim == 64 || c.head_dim == 128) &&
+                    (c.block_size == 8 || c.block_size % 16 == 0) && rows < (int64_t(1) << 31) &&
+                    reinterpret_cast<uintptr_t>(c.key_cache) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(c.value_cache) % 16 == 0;
+  if (!pl.tensor_cores) return pl;
+  const int group = p.num_query_heads / c.num_kv_heads;
+  pl.nchunks = (group + 7) / 8;
+  const int S = p.num_seqs < b200::kDecodeFp8MaxSeqs ? p.num_seqs : b200::kDecodeFp8MaxSeqs;
+  // no sequence reaches past its row of the table
+  pl.max_ctx = p.max_context_len;
+  const int64_t most = static_cast<int64_t>(p.block_table_stride) * c.block_size;
+  if (pl.max_ctx > most) pl.max_ctx = most;
+  if (pl.max_ctx < 0) pl.max_ctx = 0;
+  pl.grid = b200::decode_fp8_grid(S, pl.max_ctx, c.num_kv_heads * pl.nchunks, p.dtype, num_sms());
+  const size_t parts = b200::decode_fp8_parts(pl.grid);
+  pl.off_ml = align256((S + 1) * sizeof(int32_t));
+  pl.off_o = pl.off_ml + align256(parts * 8 * sizeof(float2));
+  pl.total = pl.off_o + align256(parts * 8 * c.head_dim * sizeof(float));
+  return pl;
+}
+
+// A cache (L, NB, BS, Hkv, D) of bytes as (D, Hkv, L*NB*BS), box (D, 1, box_rows), swizzled over
+// the D bytes of a row.
+int code_map(const void* cache, const B200Fp8Cache& c, int box_rows, CUtensorMap* out) {
+  b200::EncodeTiledFn fn = b200::encode_fn();
+  if (fn == nullptr) return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t D = c.head_dim, H = c.num_kv_heads;
+  const cuuint64_t dims[3] = {D, H, static_cast<cuuint64_t>(c.num_layers) * c.total_blocks * c.block_size};
+  const cuuint64_t strides[2] = {D, H * D};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(D), 1, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r =
+      fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(cache), dims, strides, box, estr,
+         CU_TENSOR_MAP_INTERLEAVE_NONE,
+         c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+  return B200_OK;
+}
+
+// cu_q: mixed batch, only sequences with exactly one new token are decoded (row cu_q[s]).
+int run_decode(const B200AttentionFp8Params& p, const DecodePlan& pl, const int64_t* cu_q, char* ws,
+               cudaStream_t st) {
+  const B200Fp8Cache& c = p.cache;
+  CUtensorMap km, vm;
+  const int box_rows = c.block_size >= 16 ? 16 : 8;
+  int rc = code_map(c.key_cache, c, box_rows, &km);
+  if (rc == B200_OK) rc = code_map(c.value_cache, c, box_rows, &vm);
+  if (rc != B200_OK) return rc;
+  b200::DecodeFp8Args a{};
+  a.q_srow = p.q_stride_row;
+  a.q_shead = p.q_stride_head;
+  a.ks = c.key_scale;
+  a.vs = c.value_scale;
+  a.layer = c.layer_idx;
+  a.nb = c.total_blocks;
+  a.bs = c.block_size;
+  a.hkv = c.num_kv_heads;
+  a.head_dim = c.head_dim;
+  a.group = p.num_query_heads / c.num_kv_heads;
+  a.nchunks = pl.nchunks;
+  a.bt_stride = p.block_table_stride;
+  a.max_ctx = static_cast<int32_t>(pl.max_ctx);
+  a.scale_log2 = p.scale * b200::kLog2e;
+  a.o_srow = p.o_stride_row;
+  a.o_shead = p.o_stride_head;
+  a.status = p.status_word;
+  a.cu_units = reinterpret_cast<int32_t*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + pl.off_ml);
+  a.part_o = reinterpret_cast<float*>(ws + pl.off_o);
+  for (int s0 = 0; s0 < p.num_seqs; s0 += b200::kDecodeFp8MaxSeqs) {
+    a.S = p.num_seqs - s0 < b200::kDecodeFp8MaxSeqs ? p.num_seqs - s0 : b200::kDecodeFp8MaxSeqs;
+    a.bt = p.block_tables + static_cast<int64_t>(s0) * p.block_table_stride;
+    a.ctx_lens = p.context_lens + s0;
+    a.cu_q = cu_q ? cu_q + s0 : nullptr;
+    a.query_rows = !cu_q && p.query_rows ? p.query_rows + s0 : nullptr;
+    // without a map, sequence s reads and writes row s of the call
+    const int64_t shift = cu_q || p.query_rows ? 0 : s0;
+    a.q = static_cast<const char*>(p.query) + shift * p.q_stride_row * esize_of(p.dtype);
+    a.out = static_cast<char*>(p.out) + shift * p.o_stride_row * esize_of(p.dtype);
+    const cudaError_t e = b200::launch_decode_fp8(p.dtype, km, vm, a, pl.grid, st);
+    if (e != cudaSuccess) return cuda_fail(e, "paged_decode_fp8");
+  }
+  return B200_OK;
+}
+
+int check_workspace(const void* ws, size_t have, size_t need) {
+  if (need == 0) return B200_OK;
+  if (ws == nullptr || have < need) return fail(B200_ERR_INVALID_ARGUMENT, "attention workspace too small");
+  if (reinterpret_cast<uintptr_t>(ws) % 256 != 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "attention workspace must be 256-byte aligned");
+  return B200_OK;
 }
 
 bool has_arrays(const B200AttentionFp8Params& p) {
@@ -214,22 +323,27 @@ int b200_gather_cache_fp8(const B200Fp8Cache* cache, int32_t dtype, const int64_
 }
 
 size_t b200_paged_decode_fp8_workspace_bytes(const B200AttentionFp8Params* p) {
-  (void)p;
-  return 0;
+  if (check_attention(p) != B200_OK || p->num_seqs == 0) return 0;
+  return decode_plan(*p).total;
 }
 
 int b200_paged_decode_fp8(const B200AttentionFp8Params* p, void* workspace,
                           size_t workspace_bytes, void* stream) {
   b200::NvtxRange nvtx_range("b200_paged_decode_fp8");
-  (void)workspace;
-  (void)workspace_bytes;
-  const int rc = check_attention(p);
+  int rc = check_attention(p);
   if (rc != B200_OK) return rc;
   if (p->num_seqs == 0) return B200_OK;
   if (!has_arrays(*p)) return fail(B200_ERR_INVALID_ARGUMENT, "null pointer");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const DecodePlan pl = decode_plan(*p);
+  if (pl.tensor_cores) {
+    rc = check_workspace(workspace, workspace_bytes, pl.total);
+    if (rc != B200_OK) return rc;
+    return run_decode(*p, pl, nullptr, static_cast<char*>(workspace), st);
+  }
   b200::AttnFp8Args a = attention_args(*p);
   a.query_rows = p->query_rows;
-  cudaError_t e = b200::launch_row_fp8(a, p->dtype, p->num_seqs, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = b200::launch_row_fp8(a, p->dtype, p->num_seqs, st);
   if (e != cudaSuccess) return cuda_fail(e, "paged_decode_fp8");
   return B200_OK;
 }

@@ -1,0 +1,638 @@
+// Decode over an 8-bit paged cache on the tensor cores (mma.sync; one new token per sequence).
+//
+// The batch's work is one line of units of 16 tokens: sequence by sequence, KV head by KV head (and
+// tile of 8 query heads by tile).  Every warp of a persistent grid takes an equal share of that
+// line, so the shares differ by one unit at most however the context lengths are spread, and runs
+// by itself: its own TMA ring, its own softmax, no CTA-wide synchronisation.  A warp writes an
+// item (sequence, KV head, tile of query heads) that lies inside its share straight to the output;
+// of the first and the last item of its share it may hold only a part, which it leaves in the
+// workspace for the merge kernel that follows.
+//
+// Per unit: K (16 x D codes) by ldmatrix, four codes of a row per lane and register, widened to
+// f16 in registers (exact).  The order of the dims inside a k-step of 16 is free as long as Q has
+// it too, so a lane's four adjacent codes serve two k-columns each.  V by transposing ldmatrix on
+// pairs of codes (two adjacent dims as one 16-bit element) and one byte permutation.
+//   S^T = K Q^T and O^T += V^T P^T, m16n8k16 with f16 operands and fp32 sums.
+// Q is scaled to f16 by a power of two per head (exact for bf16 and f16 queries); fp32 queries and
+// weights are split in two f16 parts (22 bits), each with its own product.
+// The weights of P: p = 2^(x - m) with a lazily moved reference m (p <= 2^8), stored for the
+// product as p * vs * F: vs is the page's value scale and F a power of two per head that keeps the
+// products inside f16's normal range whatever the scales are (11 bits of every weight that is
+// within 2^-22 of the head's largest).
+//
+// Bound: HBM (4 * G flop per byte).  A unit is 32 * D bytes.
+#include <cuda.h>
+
+#include "fp8.cuh"
+#include "fp8_decode.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kMinShare = 4;   // units per warp at least: a shorter share costs more in the merge
+constexpr float kLazy = 8.f;   // log2 of how far p may exceed 1 before the reference moves
+
+template <int D>
+struct Ring {
+  static constexpr int kTile = 16 * D;       // codes of one unit of K (or V)
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kStages = 12288 / kStage;  // 12 KB per warp: 3 stages of D 128, 6 of D 64
+  static constexpr int kWarpBytes = kStages * kStage;
+};
+
+__device__ __forceinline__ uint32_t cvt_e4m3x2(uint32_t v) {  // low 16 bits -> f16x2
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t cvt_e4m3x2_hi(uint32_t v) {  // high 16 bits -> f16x2
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) { return MmaOp<__half>::pack(lo, hi); }
+
+// 16-byte chunk `c` of row `r` in a tile of rows of D bytes, as TMA swizzles it (128 B rows with
+// the 128 B pattern, 64 B rows with the 64 B pattern).
+template <int D>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  if (D == 128) return r * 128 + ((c ^ (r & 7)) << 4);
+  return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
+
+// 2^(up - e) with mx in [1, 2) * 2^e: an exact power of two, within fp32's normal range.
+__device__ __forceinline__ float pow2_inverse(float mx, int up) {
+  int e = static_cast<int>(__float_as_uint(mx) >> 23);
+  e = min(max(254 - e + up, 1), 253);
+  return __uint_as_float(static_cast<uint32_t>(e) << 23);
+}
+
+// Inclusive prefix sums of the sequences' units into cu[1..S], cu[0] = 0.  Whole CTA.
+__device__ void prefix_units(const DecodeFp8Args& a, int32_t* cu, int32_t* warp_sums) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int32_t carry = 0;
+  if (tid == 0) cu[0] = 0;
+  for (int base = 0; base < a.S; base += kThreads) {
+    const int s = base + tid;
+    int32_t n = 0;
+    if (s < a.S) {
+      const int32_t ctx = min(a.ctx_lens[s], a.max_ctx);
+      const bool decoded = a.cu_q == nullptr || a.cu_q[s + 1] - a.cu_q[s] == 1;
+      if (decoded && ctx > 0) n = (ctx + 15) >> 4;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t t = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += t;
+    }
+    if (lane == 31) warp_sums[warp] = n;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) n += warp_sums[w];
+    }
+    if (s < a.S) cu[s + 1] = carry + n;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) carry += warp_sums[w];
+    __syncthreads();
+  }
+}
+
+__device__ __forceinline__ int64_t share_of(int64_t total, int warps) {
+  const int64_t w = (total + warps - 1) / warps;
+  return w > kMinShare ? w : kMinShare;
+}
+
+// Up to 32 consecutive units of one item; lane i holds unit i's page(s) and scales.
+template <int NP>
+struct Seg {
+  int s, hc, u0, n, units, ctx;
+  int32_t blk[NP];
+  float ks[NP], vs[NP];
+};
+
+template <typename T, int D, int NP, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
+    decode_fp8_kernel(const __grid_constant__ CUtensorMap kmap,
+                      const __grid_constant__ CUtensorMap vmap, DecodeFp8Args a) {
+  using R = Ring<D>;
+  constexpr int NS = R::kStages;
+  constexpr int KS = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_u32 = smem_u32(smem_raw);
+  const uint32_t base_u32 = (raw_u32 + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base_u32 - raw_u32);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kWarps * R::kWarpBytes);
+  int32_t* warp_sums = reinterpret_cast<int32_t*>(bars + kWarps * NS);
+  int32_t* cu = warp_sums + kWarps;  // [S + 1]
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = lane >> 2, c = lane & 3;
+  if (tid == 0) {
+    for (int i = 0; i < kWarps * NS; ++i) mbar_init(&bars[i], 1);
+    fence_proxy_async_smem();
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+  }
+  prefix_units(a, cu, warp_sums);  // its barriers publish the mbarriers too
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= a.S; i += kThreads) a.cu_units[i] = cu[i];
+  __syncthreads();
+
+  const int ips = a.hkv * a.nchunks;
+  const int64_t total = static_cast<int64_t>(cu[a.S]) * ips;
+  const int64_t share = share_of(total, static_cast<int>(gridDim.x) * kWarps);
+  const int gw = blockIdx.x * kWarps + warp;
+  int64_t at = gw * share;  // next unit of the line to make a segment of
+  const int64_t end = min(total, at + share);
+  if (at >= end) return;
+  const int64_t begin = at;
+
+  uint8_t* ring = smem + warp * R::kWarpBytes;
+  const uint32_t ring_u32 = base_u32 + warp * R::kWarpBytes;
+  uint64_t* my_bars = bars + warp * NS;
+
+  int seq;  // sequence of `at`
+  {
+    int lo = 0, hi = a.S - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (static_cast<int64_t>(cu[mid + 1]) * ips > at) hi = mid; else lo = mid + 1;
+    }
+    seq = lo;
+  }
+  int64_t rem = at - static_cast<int64_t>(cu[seq]) * ips;
+  int hc_next = static_cast<int>(rem / (cu[seq + 1] - cu[seq]));
+  int u_next = static_cast<int>(rem - static_cast<int64_t>(hc_next) * (cu[seq + 1] - cu[seq]));
+
+  const auto load_seg = [&]() {
+    Seg<NP> g;
+    g.n = 0;
+    if (at >= end) return g;
+    while (cu[seq + 1] == cu[seq]) ++seq;
+    g.s = seq;
+    g.hc = hc_next;
+    g.u0 = u_next;
+    g.units = cu[seq + 1] - cu[seq];
+    g.ctx = min(a.ctx_lens[seq], a.max_ctx);
+    g.n = static_cast<int>(min(min(static_cast<int64_t>(g.units - u_next), end - at), static_cast<int64_t>(32)));
+    at += g.n;
+    u_next += g.n;
+    if (u_next == g.units) {
+      u_next = 0;
+      if (++hc_next == ips) {
+        hc_next = 0;
+        ++seq;
+      }
+    }
+    const int32_t* row = a.bt + static_cast<int64_t>(g.s) * a.bt_stride;
+    const int h = g.hc / a.nchunks;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int t = (g.u0 + lane) * 16 + p * 8;
+      g.blk[p] = -1;
+      g.ks[p] = g.vs[p] = 0.f;
+      if (lane < g.n && t < g.ctx) {
+        const int32_t b = row[t / a.bs];
+        if (b >= 0 && b < a.nb) {
+          g.blk[p] = b;
+          const int64_t sc = (static_cast<int64_t>(a.layer) * a.nb + b) * a.hkv + h;
+          g.ks[p] = a.ks[sc];
+          g.vs[p] = a.vs[sc];
+        } else {
+          flag_status(a.status, B200_DEVICE_BAD_BLOCK);
+        }
+      }
+    }
+    return g;
+  };
+
+  Seg<NP> cur = load_seg();
+  Seg<NP> nxt = load_seg();
+  uint32_t filled = 0, used = 0;  // units issued and consumed so far
+  int next_issue = 0;             // index of the next unit to issue, from cur's first
+
+  const auto issue_one = [&]() -> bool {
+    const bool in_cur = next_issue < cur.n;
+    const int i = in_cur ? next_issue : next_issue - cur.n;
+    if (!in_cur && i >= nxt.n) return false;
+    const int h = (in_cur ? cur.hc : nxt.hc) / a.nchunks;
+    const int u = (in_cur ? cur.u0 : nxt.u0) + i;
+    int32_t blk[NP];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) blk[p] = __shfl_sync(0xffffffffu, in_cur ? cur.blk[p] : nxt.blk[p], i);
+    if (lane == 0) {
+      const int st = filled % NS;
+      uint64_t* bar = &my_bars[st];
+      uint8_t* kdst = ring + st * R::kStage;
+      mbar_arrive_expect_tx(bar, R::kStage);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        // a page outside the pool (or past the context): the pool's first page is read instead and
+        // its rows are masked
+        const int32_t b = blk[p] < 0 ? 0 : blk[p];
+        const int32_t row = (a.layer * a.nb + b) * a.bs + (NP == 1 ? (u * 16) % a.bs : 0);
+        tma_load_3d(kdst + p * 8 * D, &kmap, bar, 0, h, row);
+        tma_load_3d(kdst + R::kTile + p * 8 * D, &vmap, bar, 0, h, row);
+      }
+    }
+    ++next_issue;
+    ++filled;
+    return true;
+  };
+  while (filled < NS && issue_one()) {
+  }
+
+  uint32_t qf[KS][2], ql[SPLIT ? KS : 1][2];
+  float acc[KS][4];
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, F0 = 0.f, F1 = 0.f, qscale0 = 0.f, qscale1 = 0.f;
+  int64_t qrow = 0;
+  int nh = 0, hq0 = 0;
+  bool fresh = true;  // the next unit begins an item (for this warp)
+  int64_t pos = begin;
+
+  while (cur.n > 0) {
+    if (fresh) {
+      fresh = false;
+      const int h = cur.hc / a.nchunks, cch = cur.hc - h * a.nchunks;
+      nh = min(8, a.group - cch * 8);
+      hq0 = h * a.group + cch * 8;
+      qrow = a.cu_q ? a.cu_q[cur.s] : (a.query_rows ? a.query_rows[cur.s] : cur.s);
+      float qv[KS][4];
+      float mx = 0.f;
+      const T* q = static_cast<const T*>(a.q) + qrow * a.q_srow + static_cast<int64_t>(hq0 + r) * a.q_shead;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          qv[k][j] = r < nh ? to_f32<T>(q[16 * k + 4 * c + j]) : 0.f;
+          mx = fmaxf(mx, fabsf(qv[k][j]));
+        }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // |q| below 2^11 after scaling: the smallest parts that matter stay normal f16 numbers
+      const float inv = pow2_inverse(mx, 10);
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float x = qv[k][2 * j] * inv, y = qv[k][2 * j + 1] * inv;
+          qf[k][j] = pack_f16(x, y);
+          if (SPLIT) {
+            const __half2 hi = *reinterpret_cast<__half2*>(&qf[k][j]);
+            ql[k][j] = pack_f16(x - __low2float(hi), y - __high2float(hi));
+          }
+        }
+      const float back = a.scale_log2 / inv;  // head r's; the scores are laid out by 2c, 2c + 1
+      qscale0 = __shfl_sync(0xffffffffu, back, 8 * c);
+      qscale1 = __shfl_sync(0xffffffffu, back, 8 * c + 4);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0.f;
+      m0 = m1 = -INFINITY;
+      l0 = l1 = 0.f;
+      F0 = F1 = 0.f;
+    }
+
+    for (int i = 0; i < cur.n; ++i) {
+      const int st = used % NS;
+      if (!mbar_wait_bounded(&my_bars[st], (used / NS) & 1u)) {
+        // wait (bounded) for every fill in flight, so that none lands after this CTA is gone
+        if (lane == 0) flag_status(a.status, B200_DEVICE_TIMEOUT);
+        for (uint32_t f = used + 1; f < filled; ++f) mbar_wait_bounded(&my_bars[f % NS], (f / NS) & 1u);
+        return;
+      }
+      const uint32_t kb = ring_u32 + st * R::kStage;
+      const uint32_t vb = kb + R::kTile;
+      const int tok0 = (cur.u0 + i) * 16;
+      float ks[2], vs[2];
+      bool good[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int pp = NP == 1 ? 0 : p;
+        ks[p] = __shfl_sync(0xffffffffu, cur.ks[pp], i);
+        vs[p] = __shfl_sync(0xffffffffu, cur.vs[pp], i);
+        good[p] = __shfl_sync(0xffffffffu, cur.blk[pp], i) >= 0;
+      }
+      const int valid = cur.ctx - tok0;  // tokens of the unit inside the context
+      const bool whole = valid >= 16 && good[0] && good[1];
+      if (!whole) {
+        // rows that do not take part may hold anything, NaN codes among it: their V is zeroed
+        uint8_t* v = ring + st * R::kStage + R::kTile;
+        for (int idx = lane; idx < 16 * (D / 16); idx += 32) {
+          const int row = idx / (D / 16), ch = idx % (D / 16);
+          if (row >= valid || !good[row >> 3])
+            *reinterpret_cast<uint4*>(v + tile_at<D>(row, ch)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+      }
+
+      // ---- S^T = K Q^T -------------------------------------------------------------------
+      float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
+      const int krow = (lane & 7) + 8 * ((lane >> 3) & 1);
+#pragma unroll
+      for (int k = 0; k < KS; k += 2) {
+        uint32_t x0, x1, x2, x3;
+        ldmatrix_x4(kb + tile_at<D>(krow, k + (lane >> 4)), x0, x1, x2, x3);
+        {
+          const uint32_t a0 = cvt_e4m3x2(x0), a1 = cvt_e4m3x2(x1), a2 = cvt_e4m3x2_hi(x0), a3 = cvt_e4m3x2_hi(x1);
+          MmaOp<__half>::run(sa, a0, a1, a2, a3, qf[k][0], qf[k][1]);
+          if (SPLIT) MmaOp<__half>::run(sa, a0, a1, a2, a3, ql[k][0], ql[k][1]);
+        }
+        {
+          const uint32_t a0 = cvt_e4m3x2(x2), a1 = cvt_e4m3x2(x3), a2 = cvt_e4m3x2_hi(x2), a3 = cvt_e4m3x2_hi(x3);
+          MmaOp<__half>::run(sb, a0, a1, a2, a3, qf[k + 1][0], qf[k + 1][1]);
+          if (SPLIT) MmaOp<__half>::run(sb, a0, a1, a2, a3, ql[k + 1][0], ql[k + 1][1]);
+        }
+      }
+      float x0 = (sa[0] + sb[0]) * (ks[0] * qscale0), x1 = (sa[1] + sb[1]) * (ks[0] * qscale1);
+      float x2 = (sa[2] + sb[2]) * (ks[1] * qscale0), x3 = (sa[3] + sb[3]) * (ks[1] * qscale1);
+      if (!whole) {
+        if (r >= valid || !good[0]) x0 = x1 = -INFINITY;
+        if (r + 8 >= valid || !good[1]) x2 = x3 = -INFINITY;
+      }
+
+      // ---- softmax with a lazily moved reference --------------------------------------------
+      const float vmax = fmaxf(vs[0], vs[1]);
+      const bool move = fmaxf(x0, x2) > m0 + kLazy || fmaxf(x1, x3) > m1 + kLazy ||
+                        !(vmax * F0 <= 128.f) || !(vmax * F1 <= 128.f) || F0 == 0.f || F1 == 0.f;
+      float u0 = m0, u1 = m1;
+      if (__any_sync(0xffffffffu, move)) {
+        float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+          t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+        }
+        const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+        u0 = n0 == -INFINITY ? 0.f : n0;
+        u1 = n1 == -INFINITY ? 0.f : n1;
+        float al0 = fast_exp2(m0 - u0), al1 = fast_exp2(m1 - u1);
+        l0 *= al0;
+        l1 *= al1;
+        m0 = n0;
+        m1 = n1;
+        // the largest product p * vs of the unit, per head
+        float w0 = fmaxf(fast_exp2(x0 - u0) * vs[0], fast_exp2(x2 - u0) * vs[1]);
+        float w1 = fmaxf(fast_exp2(x1 - u1) * vs[0], fast_exp2(x3 - u1) * vs[1]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          w0 = fmaxf(w0, __shfl_xor_sync(0xffffffffu, w0, o));
+          w1 = fmaxf(w1, __shfl_xor_sync(0xffffffffu, w1, o));
+        }
+        // F changes when unset or when a product would pass 2^15
+        const auto refit = [](float w, float& F, float& al) {
+          if (!(w > 0.f)) return;
+          if (F == 0.f || w * F > 32768.f) {
+            const float f = pow2_inverse(w, 8);  // p * vs * F in [2^8, 2^9)
+            al = F == 0.f ? 0.f : al * (f / F);
+            F = f;
+          }
+        };
+        refit(w0, F0, al0);
+        refit(w1, F1, al1);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          acc[k][0] *= al0;
+          acc[k][1] *= al1;
+          acc[k][2] *= al0;
+          acc[k][3] *= al1;
+        }
+      }
+      float p0 = fast_exp2(x0 - u0), p1 = fast_exp2(x1 - u1);
+      float p2 = fast_exp2(x2 - u0), p3 = fast_exp2(x3 - u1);
+      l0 += p0 + p2;
+      l1 += p1 + p3;
+      p0 *= vs[0] * F0;
+      p1 *= vs[0] * F1;
+      p2 *= vs[1] * F0;
+      p3 *= vs[1] * F1;
+      if (!whole) {  // 0 * (an unwritten page's scale) is not 0 when that is NaN
+        if (r >= valid || !good[0]) p0 = p1 = 0.f;
+        if (r + 8 >= valid || !good[1]) p2 = p3 = 0.f;
+      }
+      const uint32_t ph0 = pack_f16(p0, p1), ph1 = pack_f16(p2, p3);
+      const uint32_t pb0 = movmatrix_trans(ph0), pb1 = movmatrix_trans(ph1);
+      uint32_t pl0 = 0, pl1 = 0;
+      if (SPLIT) {
+        const __half2 h0 = *reinterpret_cast<const __half2*>(&ph0);
+        const __half2 h1 = *reinterpret_cast<const __half2*>(&ph1);
+        pl0 = movmatrix_trans(pack_f16(p0 - __low2float(h0), p1 - __high2float(h0)));
+        pl1 = movmatrix_trans(pack_f16(p2 - __low2float(h1), p3 - __high2float(h1)));
+      }
+
+      // ---- O^T += V^T P^T: row r of a 16-dim tile is dim 2r, row r + 8 dim 2r + 1 ------------
+#pragma unroll
+      for (int k = 0; k < KS; k += 2) {
+        uint32_t y0, y1, y2, y3;
+        ldmatrix_x4_trans(vb + tile_at<D>(krow, k + (lane >> 4)), y0, y1, y2, y3);
+        y0 = __byte_perm(y0, 0, 0x3120);
+        y1 = __byte_perm(y1, 0, 0x3120);
+        y2 = __byte_perm(y2, 0, 0x3120);
+        y3 = __byte_perm(y3, 0, 0x3120);
+        {
+          const uint32_t a0 = cvt_e4m3x2(y0), a1 = cvt_e4m3x2_hi(y0), a2 = cvt_e4m3x2(y1), a3 = cvt_e4m3x2_hi(y1);
+          MmaOp<__half>::run(acc[k], a0, a1, a2, a3, pb0, pb1);
+          if (SPLIT) MmaOp<__half>::run(acc[k], a0, a1, a2, a3, pl0, pl1);
+        }
+        {
+          const uint32_t a0 = cvt_e4m3x2(y2), a1 = cvt_e4m3x2_hi(y2), a2 = cvt_e4m3x2(y3), a3 = cvt_e4m3x2_hi(y3);
+          MmaOp<__half>::run(acc[k + 1], a0, a1, a2, a3, pb0, pb1);
+          if (SPLIT) MmaOp<__half>::run(acc[k + 1], a0, a1, a2, a3, pl0, pl1);
+        }
+      }
+      ++used;
+      __syncwarp();
+      if (lane == 0) fence_proxy_async_smem();  // this stage's reads and zeroing before its refill
+      issue_one();
+    }
+
+    // ---- the item's end, or the share's ---------------------------------------------------
+    const int item_end = cur.u0 + cur.n;
+    const bool done = item_end == cur.units;
+    const int64_t seg_end = pos + cur.n;
+    if (done || seg_end == end) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+      }
+      const int64_t item0 = seg_end - item_end;  // the line's unit where this item begins
+      if (done && item0 >= begin) {
+        const float f0 = F0 > 0.f ? 1.f / F0 : 0.f, f1 = F1 > 0.f ? 1.f / F1 : 0.f;
+        const float i0 = l0 != 0.f ? 1.f / l0 : 0.f, i1 = l1 != 0.f ? 1.f / l1 : 0.f;
+        T* o0 = static_cast<T*>(a.out) + qrow * a.o_srow + static_cast<int64_t>(hq0 + 2 * c) * a.o_shead;
+        T* o1 = o0 + a.o_shead;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const int d = 16 * k + 2 * r;
+          if (2 * c < nh) {
+            o0[d] = from_f32<T>(acc[k][0] * f0 * i0);
+            o0[d + 1] = from_f32<T>(acc[k][2] * f0 * i0);
+          }
+          if (2 * c + 1 < nh) {
+            o1[d] = from_f32<T>(acc[k][1] * f1 * i1);
+            o1[d + 1] = from_f32<T>(acc[k][3] * f1 * i1);
+          }
+        }
+      } else {
+        // a part of an item: sums relative to 2^m, the output sum as the values' (without F)
+        const int64_t slot = 2 * static_cast<int64_t>(gw) + (item0 <= begin ? 0 : 1);
+        float* po = a.part_o + slot * 8 * D;
+        float2* ml = a.part_ml + slot * 8;
+        const float i0 = F0 > 0.f ? 1.f / F0 : 0.f, i1 = F1 > 0.f ? 1.f / F1 : 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const int d = 16 * k + 2 * r;
+          if (2 * c < nh)
+            *reinterpret_cast<float2*>(po + (2 * c) * D + d) = make_float2(acc[k][0] * i0, acc[k][2] * i0);
+          if (2 * c + 1 < nh)
+            *reinterpret_cast<float2*>(po + (2 * c + 1) * D + d) = make_float2(acc[k][1] * i1, acc[k][3] * i1);
+        }
+        if (r == 0) {
+          ml[2 * c] = make_float2(m0, l0);
+          ml[2 * c + 1] = make_float2(m1, l1);
+        }
+      }
+      fresh = true;
+    }
+    pos = seg_end;
+    next_issue -= cur.n;
+    cur = nxt;
+    nxt = load_seg();
+    while (filled - used < NS && issue_one()) {
+    }
+  }
+}
+
+// Joins the parts of items that several warps shared, in the order of the warps, and writes zeros
+// for decoded sequences without context.  One CTA per item.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) merge_fp8_kernel(DecodeFp8Args a, int warps) {
+  __shared__ float4 sum_s[256];
+  __shared__ float2 ml_s[8][32];
+  const int tid = threadIdx.x;
+  const int ips = a.hkv * a.nchunks;
+  const int s = blockIdx.x / ips, hc = blockIdx.x - s * ips;
+  const int h = hc / a.nchunks, cch = hc - h * a.nchunks;
+  const int nh = min(8, a.group - cch * 8), hq0 = h * a.group + cch * 8;
+  const int units = a.cu_units[s + 1] - a.cu_units[s];
+  const int64_t qrow = a.cu_q ? a.cu_q[s] : (a.query_rows ? a.query_rows[s] : s);
+  T* out = static_cast<T*>(a.out) + qrow * a.o_srow + static_cast<int64_t>(hq0) * a.o_shead;
+  if (hc == 0 && tid == 0 && a.ctx_lens[s] > a.max_ctx) flag_status(a.status, B200_DEVICE_BAD_OP);
+  if (units == 0) {
+    if (a.cu_q == nullptr || a.cu_q[s + 1] - a.cu_q[s] == 1)
+      for (int i = tid; i < nh * D; i += 256) out[(i / D) * a.o_shead + i % D] = from_f32<T>(0.f);
+    return;
+  }
+  const int64_t total = static_cast<int64_t>(a.cu_units[a.S]) * ips;
+  const int64_t share = share_of(total, warps);
+  const int64_t first = static_cast<int64_t>(a.cu_units[s]) * ips + static_cast<int64_t>(hc) * units;
+  const int64_t w0 = first / share, w1 = (first + units - 1) / share;
+  if (w0 == w1) return;  // written by its warp
+  const int n = static_cast<int>(w1 - w0) + 1;
+  const auto slot_of = [&](int i) { return 2 * (w0 + i) + (i == 0 && first > w0 * share ? 1 : 0); };
+  // every head's largest reference, then each part's weight
+  constexpr int kVec = D / 4;                    // float4s of a head
+  const int lanes = nh * kVec;                   // at most 256
+  const int groups = 256 / lanes > 0 ? 256 / lanes : 1;
+  const int grp = tid / lanes, e = tid - grp * lanes;
+  const int hh = e / kVec;
+  float M = -INFINITY, L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (grp < groups) {
+    for (int i = grp; i < n; i += groups) {
+      const int64_t sl = slot_of(i);
+      const float2 ml = a.part_ml[sl * 8 + hh];
+      const float4 v = *reinterpret_cast<const float4*>(a.part_o + (sl * 8 + hh) * D + (e % kVec) * 4);
+      const float N = fmaxf(M, ml.x);
+      const float Nu = N == -INFINITY ? 0.f : N;
+      const float wa = fast_exp2(M - Nu), wb = fast_exp2(ml.x - Nu);
+      o.x = o.x * wa + v.x * wb;
+      o.y = o.y * wa + v.y * wb;
+      o.z = o.z * wa + v.z * wb;
+      o.w = o.w * wa + v.w * wb;
+      L = L * wa + ml.y * wb;
+      M = N;
+    }
+    sum_s[tid] = o;
+    if (e % kVec == 0) ml_s[hh][grp] = make_float2(M, L);
+  }
+  __syncthreads();
+  if (grp == 0) {
+    for (int g = 1; g < groups; ++g) {
+      const float2 ml = ml_s[hh][g];
+      const float4 v = sum_s[g * lanes + e];
+      const float N = fmaxf(M, ml.x);
+      const float Nu = N == -INFINITY ? 0.f : N;
+      const float wa = fast_exp2(M - Nu), wb = fast_exp2(ml.x - Nu);
+      o.x = o.x * wa + v.x * wb;
+      o.y = o.y * wa + v.y * wb;
+      o.z = o.z * wa + v.z * wb;
+      o.w = o.w * wa + v.w * wb;
+      L = L * wa + ml.y * wb;
+      M = N;
+    }
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+    T* d = out + static_cast<int64_t>(hh) * a.o_shead + (e % kVec) * 4;
+    d[0] = from_f32<T>(o.x * inv);
+    d[1] = from_f32<T>(o.y * inv);
+    d[2] = from_f32<T>(o.z * inv);
+    d[3] = from_f32<T>(o.w * inv);
+  }
+}
+
+template <int D>
+int smem_bytes(int S) {
+  using R = Ring<D>;
+  return 1024 + kWarps * R::kWarpBytes + kWarps * R::kStages * 8 + kWarps * 4 + (S + 1) * 4;
+}
+
+template <typename T, int D, int NP, bool SPLIT>
+cudaError_t launch_t(const CUtensorMap& km, const CUtensorMap& vm, const DecodeFp8Args& a, int grid,
+                     cudaStream_t stream) {
+  const int smem = smem_bytes<D>(a.S);
+  auto kern = decode_fp8_kernel<T, D, NP, SPLIT>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<grid, kThreads, smem, stream>>>(km, vm, a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  merge_fp8_kernel<T, D><<<a.S * a.hkv * a.nchunks, 256, 0, stream>>>(a, grid * kWarps);
+  return cudaGetLastError();
+}
+
+template <typename T, bool SPLIT>
+cudaError_t launch_d(const CUtensorMap& km, const CUtensorMap& vm, const DecodeFp8Args& a, int grid,
+                     cudaStream_t stream) {
+  if (a.head_dim == 128)
+    return a.bs == 8 ? launch_t<T, 128, 2, SPLIT>(km, vm, a, grid, stream)
+                     : launch_t<T, 128, 1, SPLIT>(km, vm, a, grid, stream);
+  return a.bs == 8 ? launch_t<T, 64, 2, SPLIT>(km, vm, a, grid, stream)
+                   : launch_t<T, 64, 1, SPLIT>(km, vm, a, grid, stream);
+}
+
+}  // namespace
+
+int decode_fp8_grid(int S, int64_t max_ctx, int ips, int dtype, int num_sms) {
+  const int64_t units = static_cast<int64_t>(S) * ((max_ctx + 15) / 16) * ips;
+  const int64_t need = (units + kMinShare * kWarps - 1) / (kMinShare * kWarps);
+  const int64_t most = static_cast<int64_t>(num_sms) * (dtype == B200_DTYPE_F32 ? 3 : 4);
+  return static_cast<int>(need < 1 ? 1 : need < most ? need : most);
+}
+
+int decode_fp8_parts(int grid) { return 2 * kWarps * grid; }
+
+cudaError_t launch_decode_fp8(int dtype, const CUtensorMap& km, const CUtensorMap& vm,
+                              const DecodeFp8Args& a, int grid, cudaStream_t stream) {
+  switch (dtype) {
+    case B200_DTYPE_F32: return launch_d<float, true>(km, vm, a, grid, stream);
+    case B200_DTYPE_BF16: return launch_d<__nv_bfloat16, false>(km, vm, a, grid, stream);
+    case B200_DTYPE_F16: return launch_d<__half, false>(km, vm, a, grid, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace b200
