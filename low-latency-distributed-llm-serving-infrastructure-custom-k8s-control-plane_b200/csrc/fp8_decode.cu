@@ -33,6 +33,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMinShare = 4;   // units per warp at least: a shorter share costs more in the merge
+constexpr float kUnset = 0x1p+126f;  // F before a page with a nonzero value scale: any scale moves it
 constexpr float kLazy = 8.f;   // log2 of how far p may exceed 1 before the reference moves
 
 template <int D>
@@ -101,16 +102,27 @@ __device__ void prefix_units(const DecodeFp8Args& a, int32_t* cu, int32_t* warp_
   }
 }
 
+// Items (KV heads, or tiles of query heads) that a team takes side by side.  A page's rows hold
+// the heads of a token one after another, so the warps of a team read adjacent pieces at about the
+// same time.
+__device__ __forceinline__ int team_of(int items) {
+  return items % 4 == 0 ? 4 : items % 2 == 0 ? 2 : 1;
+}
+
 __device__ __forceinline__ int64_t share_of(int64_t total, int warps) {
   const int64_t w = (total + warps - 1) / warps;
   return w > kMinShare ? w : kMinShare;
 }
 
-// Up to 32 consecutive units of one item; lane i holds unit i's page(s) and scales.
+// Up to 32 consecutive units of one item; lane i holds unit i's first cache row and scales (of its
+// two pages where a page holds 8 tokens).  A page that does not take part has kBad set: the row is
+// then one of the pool's first page.
+constexpr uint32_t kBad = 0x80000000u;
+
 template <int NP>
 struct Seg {
-  int s, hc, u0, n, units, ctx;
-  int32_t blk[NP];
+  int s, hc, h, u0, n, units, ctx;
+  uint32_t row[NP];
   float ks[NP], vs[NP];
 };
 
@@ -142,11 +154,12 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
     for (int i = tid; i <= a.S; i += kThreads) a.cu_units[i] = cu[i];
   __syncthreads();
 
-  const int ips = a.hkv * a.nchunks;
+  // teams of ts warps walk the line side by side, each warp with an item of its own
+  const int ts = team_of(a.hkv * a.nchunks), ips = a.hkv * a.nchunks / ts;
   const int64_t total = static_cast<int64_t>(cu[a.S]) * ips;
-  const int64_t share = share_of(total, static_cast<int>(gridDim.x) * kWarps);
+  const int64_t share = share_of(total, static_cast<int>(gridDim.x) * (kWarps / ts));
   const int gw = blockIdx.x * kWarps + warp;
-  int64_t at = gw * share;  // next unit of the line to make a segment of
+  int64_t at = gw / ts * share;  // next unit of the line to make a segment of
   const int64_t end = min(total, at + share);
   if (at >= end) return;
   const int64_t begin = at;
@@ -174,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
     if (at >= end) return g;
     while (cu[seq + 1] == cu[seq]) ++seq;
     g.s = seq;
-    g.hc = hc_next;
+    g.hc = hc_next * ts + warp % ts;
     g.u0 = u_next;
     g.units = cu[seq + 1] - cu[seq];
     g.ctx = min(a.ctx_lens[seq], a.max_ctx);
@@ -188,67 +201,82 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
         ++seq;
       }
     }
-    const int32_t* row = a.bt + static_cast<int64_t>(g.s) * a.bt_stride;
-    const int h = g.hc / a.nchunks;
+    g.h = g.hc / a.nchunks;
+    const int32_t* table = a.bt + static_cast<int64_t>(g.s) * a.bt_stride;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
       const int t = (g.u0 + lane) * 16 + p * 8;
-      g.blk[p] = -1;
+      const int page = t / a.bs;
+      int32_t b = 0;
+      uint32_t bad = kBad;
       g.ks[p] = g.vs[p] = 0.f;
       if (lane < g.n && t < g.ctx) {
-        const int32_t b = row[t / a.bs];
+        b = table[page];
         if (b >= 0 && b < a.nb) {
-          g.blk[p] = b;
-          const int64_t sc = (static_cast<int64_t>(a.layer) * a.nb + b) * a.hkv + h;
+          bad = 0;
+          const int64_t sc = (static_cast<int64_t>(a.layer) * a.nb + b) * a.hkv + g.h;
           g.ks[p] = a.ks[sc];
           g.vs[p] = a.vs[sc];
         } else {
+          b = 0;
           flag_status(a.status, B200_DEVICE_BAD_BLOCK);
         }
       }
+      g.row[p] = static_cast<uint32_t>((a.layer * a.nb + b) * a.bs + (t - page * a.bs)) | bad;
     }
     return g;
   };
 
   Seg<NP> cur = load_seg();
   Seg<NP> nxt = load_seg();
-  uint32_t filled = 0, used = 0;  // units issued and consumed so far
-  int next_issue = 0;             // index of the next unit to issue, from cur's first
+  // the producer's side: the segment it issues from (cur, or nxt), the next unit there, and the
+  // ring's next stage; units in flight
+  uint32_t prow[NP];
+#pragma unroll
+  for (int p = 0; p < NP; ++p) prow[p] = cur.row[p];
+  int ph = cur.h, pn = cur.n, pi = 0, pstage = 0, flight = 0;
+  bool on_next = false;
 
   const auto issue_one = [&]() -> bool {
-    const bool in_cur = next_issue < cur.n;
-    const int i = in_cur ? next_issue : next_issue - cur.n;
-    if (!in_cur && i >= nxt.n) return false;
-    const int h = (in_cur ? cur.hc : nxt.hc) / a.nchunks;
-    const int u = (in_cur ? cur.u0 : nxt.u0) + i;
-    int32_t blk[NP];
+    if (pi == pn) {
+      if (on_next || nxt.n == 0) return false;
+      on_next = true;
 #pragma unroll
-    for (int p = 0; p < NP; ++p) blk[p] = __shfl_sync(0xffffffffu, in_cur ? cur.blk[p] : nxt.blk[p], i);
+      for (int p = 0; p < NP; ++p) prow[p] = nxt.row[p];
+      ph = nxt.h;
+      pn = nxt.n;
+      pi = 0;
+    }
+    uint32_t row[NP];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) row[p] = __shfl_sync(0xffffffffu, prow[p], pi) & ~kBad;
     if (lane == 0) {
-      const int st = filled % NS;
-      uint64_t* bar = &my_bars[st];
-      uint8_t* kdst = ring + st * R::kStage;
+      uint64_t* bar = &my_bars[pstage];
+      uint8_t* dst = ring + pstage * R::kStage;
       mbar_arrive_expect_tx(bar, R::kStage);
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        // a page outside the pool (or past the context): the pool's first page is read instead and
-        // its rows are masked
-        const int32_t b = blk[p] < 0 ? 0 : blk[p];
-        const int32_t row = (a.layer * a.nb + b) * a.bs + (NP == 1 ? (u * 16) % a.bs : 0);
-        tma_load_3d(kdst + p * 8 * D, &kmap, bar, 0, h, row);
-        tma_load_3d(kdst + R::kTile + p * 8 * D, &vmap, bar, 0, h, row);
+        tma_load_3d(dst + p * 8 * D, &kmap, bar, 0, ph, static_cast<int32_t>(row[p]));
+        tma_load_3d(dst + R::kTile + p * 8 * D, &vmap, bar, 0, ph, static_cast<int32_t>(row[p]));
       }
     }
-    ++next_issue;
-    ++filled;
+    ++pi;
+    ++flight;
+    if (++pstage == NS) pstage = 0;
     return true;
   };
-  while (filled < NS && issue_one()) {
+  while (flight < NS && issue_one()) {
   }
+
+  int cstage = 0;          // the ring's next stage to read, and the phase of its barrier
+  uint32_t cphase = 0;
+  // ldmatrix: lane's row of the unit and 16-byte chunk 0 or 1, swizzled; chunk k is at ^ (k << 4)
+  const int krow = (lane & 7) + 8 * ((lane >> 3) & 1);
+  const uint32_t lane_at = tile_at<D>(krow, lane >> 4);
 
   uint32_t qf[KS][2], ql[SPLIT ? KS : 1][2];
   float acc[KS][4];
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, F0 = 0.f, F1 = 0.f, qscale0 = 0.f, qscale1 = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, F0 = kUnset, F1 = kUnset, qscale0 = 0.f, qscale1 = 0.f;
   int64_t qrow = 0;
   int nh = 0, hq0 = 0;
   bool fresh = true;  // the next unit begins an item (for this warp)
@@ -257,9 +285,9 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
   while (cur.n > 0) {
     if (fresh) {
       fresh = false;
-      const int h = cur.hc / a.nchunks, cch = cur.hc - h * a.nchunks;
+      const int cch = cur.hc - cur.h * a.nchunks;
       nh = min(8, a.group - cch * 8);
-      hq0 = h * a.group + cch * 8;
+      hq0 = cur.h * a.group + cch * 8;
       qrow = a.cu_q ? a.cu_q[cur.s] : (a.query_rows ? a.query_rows[cur.s] : cur.s);
       float qv[KS][4];
       float mx = 0.f;
@@ -293,49 +321,57 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
       for (int k = 0; k < KS; ++k) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0.f;
       m0 = m1 = -INFINITY;
       l0 = l1 = 0.f;
-      F0 = F1 = 0.f;
+      F0 = F1 = kUnset;
     }
 
     for (int i = 0; i < cur.n; ++i) {
-      const int st = used % NS;
-      if (!mbar_wait_bounded(&my_bars[st], (used / NS) & 1u)) {
+      if (!mbar_wait_bounded(&my_bars[cstage], cphase)) {
         // wait (bounded) for every fill in flight, so that none lands after this CTA is gone
         if (lane == 0) flag_status(a.status, B200_DEVICE_TIMEOUT);
-        for (uint32_t f = used + 1; f < filled; ++f) mbar_wait_bounded(&my_bars[f % NS], (f / NS) & 1u);
+        for (int f = 1; f < flight; ++f) {
+          if (++cstage == NS) {
+            cstage = 0;
+            cphase ^= 1u;
+          }
+          mbar_wait_bounded(&my_bars[cstage], cphase);
+        }
         return;
       }
-      const uint32_t kb = ring_u32 + st * R::kStage;
+      const uint32_t kb = ring_u32 + cstage * R::kStage + lane_at;
       const uint32_t vb = kb + R::kTile;
-      const int tok0 = (cur.u0 + i) * 16;
+      uint32_t row[NP];
       float ks[2], vs[2];
-      bool good[2];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int pp = NP == 1 ? 0 : p;
-        ks[p] = __shfl_sync(0xffffffffu, cur.ks[pp], i);
-        vs[p] = __shfl_sync(0xffffffffu, cur.vs[pp], i);
-        good[p] = __shfl_sync(0xffffffffu, cur.blk[pp], i) >= 0;
+      for (int p = 0; p < NP; ++p) {
+        row[p] = __shfl_sync(0xffffffffu, cur.row[p], i);
+        ks[p] = __shfl_sync(0xffffffffu, cur.ks[p], i);
+        vs[p] = __shfl_sync(0xffffffffu, cur.vs[p], i);
       }
-      const int valid = cur.ctx - tok0;  // tokens of the unit inside the context
-      const bool whole = valid >= 16 && good[0] && good[1];
+      if (NP == 1) {
+        ks[1] = ks[0];
+        vs[1] = vs[0];
+      }
+      const int valid = cur.ctx - (cur.u0 + i) * 16;  // tokens of the unit inside the context
+      const bool whole = valid >= 16 && !((row[0] | row[NP - 1]) & kBad);
+      const bool in0 = r < valid && !(row[0] & kBad);           // token r of the unit takes part
+      const bool in1 = r + 8 < valid && !(row[NP - 1] & kBad);  // token r + 8
       if (!whole) {
         // rows that do not take part may hold anything, NaN codes among it: their V is zeroed
-        uint8_t* v = ring + st * R::kStage + R::kTile;
+        uint8_t* v = ring + cstage * R::kStage + R::kTile;
         for (int idx = lane; idx < 16 * (D / 16); idx += 32) {
-          const int row = idx / (D / 16), ch = idx % (D / 16);
-          if (row >= valid || !good[row >> 3])
-            *reinterpret_cast<uint4*>(v + tile_at<D>(row, ch)) = make_uint4(0u, 0u, 0u, 0u);
+          const int rr = idx / (D / 16), ch = idx % (D / 16);
+          if (rr >= valid || (row[rr < 8 ? 0 : NP - 1] & kBad))
+            *reinterpret_cast<uint4*>(v + tile_at<D>(rr, ch)) = make_uint4(0u, 0u, 0u, 0u);
         }
         __syncwarp();
       }
 
       // ---- S^T = K Q^T -------------------------------------------------------------------
       float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
-      const int krow = (lane & 7) + 8 * ((lane >> 3) & 1);
 #pragma unroll
       for (int k = 0; k < KS; k += 2) {
         uint32_t x0, x1, x2, x3;
-        ldmatrix_x4(kb + tile_at<D>(krow, k + (lane >> 4)), x0, x1, x2, x3);
+        ldmatrix_x4(kb ^ (k << 4), x0, x1, x2, x3);
         {
           const uint32_t a0 = cvt_e4m3x2(x0), a1 = cvt_e4m3x2(x1), a2 = cvt_e4m3x2_hi(x0), a3 = cvt_e4m3x2_hi(x1);
           MmaOp<__half>::run(sa, a0, a1, a2, a3, qf[k][0], qf[k][1]);
@@ -347,36 +383,45 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
           if (SPLIT) MmaOp<__half>::run(sb, a0, a1, a2, a3, ql[k + 1][0], ql[k + 1][1]);
         }
       }
-      float x0 = (sa[0] + sb[0]) * (ks[0] * qscale0), x1 = (sa[1] + sb[1]) * (ks[0] * qscale1);
-      float x2 = (sa[2] + sb[2]) * (ks[1] * qscale0), x3 = (sa[3] + sb[3]) * (ks[1] * qscale1);
-      if (!whole) {
-        if (r >= valid || !good[0]) x0 = x1 = -INFINITY;
-        if (r + 8 >= valid || !good[1]) x2 = x3 = -INFINITY;
-      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sa[j] += sb[j];
+      const float c0 = ks[0] * qscale0, c1 = ks[0] * qscale1, c2 = ks[1] * qscale0, c3 = ks[1] * qscale1;
 
       // ---- softmax with a lazily moved reference --------------------------------------------
-      const float vmax = fmaxf(vs[0], vs[1]);
-      const bool move = fmaxf(x0, x2) > m0 + kLazy || fmaxf(x1, x3) > m1 + kLazy ||
-                        !(vmax * F0 <= 128.f) || !(vmax * F1 <= 128.f) || F0 == 0.f || F1 == 0.f;
-      float u0 = m0, u1 = m1;
+      float y0 = fmaf(sa[0], c0, -m0), y1 = fmaf(sa[1], c1, -m1);
+      float y2 = fmaf(sa[2], c2, -m0), y3 = fmaf(sa[3], c3, -m1);
+      if (!whole) {
+        if (!in0) y0 = y1 = -INFINITY;
+        if (!in1) y2 = y3 = -INFINITY;
+      }
+      const float vmax = NP == 1 ? vs[0] : fmaxf(vs[0], vs[1]);
+      const bool move = fmaxf(fmaxf(y0, y1), fmaxf(y2, y3)) > kLazy || vmax * fmaxf(F0, F1) > 128.f;
       if (__any_sync(0xffffffffu, move)) {
-        float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
+        y0 = in0 ? sa[0] * c0 : -INFINITY;
+        y1 = in0 ? sa[1] * c1 : -INFINITY;
+        y2 = in1 ? sa[2] * c2 : -INFINITY;
+        y3 = in1 ? sa[3] * c3 : -INFINITY;
+        float t0 = fmaxf(y0, y2), t1 = fmaxf(y1, y3);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
           t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
           t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
         }
-        const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-        u0 = n0 == -INFINITY ? 0.f : n0;
-        u1 = n1 == -INFINITY ? 0.f : n1;
+        t0 = fmaxf(m0, t0);
+        t1 = fmaxf(m1, t1);
+        const float u0 = t0 == -INFINITY ? 0.f : t0, u1 = t1 == -INFINITY ? 0.f : t1;
         float al0 = fast_exp2(m0 - u0), al1 = fast_exp2(m1 - u1);
         l0 *= al0;
         l1 *= al1;
-        m0 = n0;
-        m1 = n1;
+        m0 = t0;
+        m1 = t1;
+        y0 -= u0;
+        y1 -= u1;
+        y2 -= u0;
+        y3 -= u1;
         // the largest product p * vs of the unit, per head
-        float w0 = fmaxf(fast_exp2(x0 - u0) * vs[0], fast_exp2(x2 - u0) * vs[1]);
-        float w1 = fmaxf(fast_exp2(x1 - u1) * vs[0], fast_exp2(x3 - u1) * vs[1]);
+        float w0 = fmaxf(fast_exp2(y0) * vs[0], fast_exp2(y2) * vs[1]);
+        float w1 = fmaxf(fast_exp2(y1) * vs[0], fast_exp2(y3) * vs[1]);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
           w0 = fmaxf(w0, __shfl_xor_sync(0xffffffffu, w0, o));
@@ -384,12 +429,10 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
         }
         // F changes when unset or when a product would pass 2^15
         const auto refit = [](float w, float& F, float& al) {
-          if (!(w > 0.f)) return;
-          if (F == 0.f || w * F > 32768.f) {
-            const float f = pow2_inverse(w, 8);  // p * vs * F in [2^8, 2^9)
-            al = F == 0.f ? 0.f : al * (f / F);
-            F = f;
-          }
+          if (!(w > 0.f) || (F != kUnset && w * F <= 32768.f)) return;
+          const float f = pow2_inverse(w, 8);  // p * vs * F in [2^8, 2^9)
+          al *= f / F;
+          F = f;
         };
         refit(w0, F0, al0);
         refit(w1, F1, al1);
@@ -401,18 +444,13 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
           acc[k][3] *= al1;
         }
       }
-      float p0 = fast_exp2(x0 - u0), p1 = fast_exp2(x1 - u1);
-      float p2 = fast_exp2(x2 - u0), p3 = fast_exp2(x3 - u1);
+      float p0 = fast_exp2(y0), p1 = fast_exp2(y1), p2 = fast_exp2(y2), p3 = fast_exp2(y3);
       l0 += p0 + p2;
       l1 += p1 + p3;
       p0 *= vs[0] * F0;
       p1 *= vs[0] * F1;
       p2 *= vs[1] * F0;
       p3 *= vs[1] * F1;
-      if (!whole) {  // 0 * (an unwritten page's scale) is not 0 when that is NaN
-        if (r >= valid || !good[0]) p0 = p1 = 0.f;
-        if (r + 8 >= valid || !good[1]) p2 = p3 = 0.f;
-      }
       const uint32_t ph0 = pack_f16(p0, p1), ph1 = pack_f16(p2, p3);
       const uint32_t pb0 = movmatrix_trans(ph0), pb1 = movmatrix_trans(ph1);
       uint32_t pl0 = 0, pl1 = 0;
@@ -426,24 +464,28 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
       // ---- O^T += V^T P^T: row r of a 16-dim tile is dim 2r, row r + 8 dim 2r + 1 ------------
 #pragma unroll
       for (int k = 0; k < KS; k += 2) {
-        uint32_t y0, y1, y2, y3;
-        ldmatrix_x4_trans(vb + tile_at<D>(krow, k + (lane >> 4)), y0, y1, y2, y3);
-        y0 = __byte_perm(y0, 0, 0x3120);
-        y1 = __byte_perm(y1, 0, 0x3120);
-        y2 = __byte_perm(y2, 0, 0x3120);
-        y3 = __byte_perm(y3, 0, 0x3120);
+        uint32_t z0, z1, z2, z3;
+        ldmatrix_x4_trans(vb ^ (k << 4), z0, z1, z2, z3);
+        z0 = __byte_perm(z0, 0, 0x3120);
+        z1 = __byte_perm(z1, 0, 0x3120);
+        z2 = __byte_perm(z2, 0, 0x3120);
+        z3 = __byte_perm(z3, 0, 0x3120);
         {
-          const uint32_t a0 = cvt_e4m3x2(y0), a1 = cvt_e4m3x2_hi(y0), a2 = cvt_e4m3x2(y1), a3 = cvt_e4m3x2_hi(y1);
+          const uint32_t a0 = cvt_e4m3x2(z0), a1 = cvt_e4m3x2_hi(z0), a2 = cvt_e4m3x2(z1), a3 = cvt_e4m3x2_hi(z1);
           MmaOp<__half>::run(acc[k], a0, a1, a2, a3, pb0, pb1);
           if (SPLIT) MmaOp<__half>::run(acc[k], a0, a1, a2, a3, pl0, pl1);
         }
         {
-          const uint32_t a0 = cvt_e4m3x2(y2), a1 = cvt_e4m3x2_hi(y2), a2 = cvt_e4m3x2(y3), a3 = cvt_e4m3x2_hi(y3);
+          const uint32_t a0 = cvt_e4m3x2(z2), a1 = cvt_e4m3x2_hi(z2), a2 = cvt_e4m3x2(z3), a3 = cvt_e4m3x2_hi(z3);
           MmaOp<__half>::run(acc[k + 1], a0, a1, a2, a3, pb0, pb1);
           if (SPLIT) MmaOp<__half>::run(acc[k + 1], a0, a1, a2, a3, pl0, pl1);
         }
       }
-      ++used;
+      --flight;
+      if (++cstage == NS) {
+        cstage = 0;
+        cphase ^= 1u;
+      }
       __syncwarp();
       if (lane == 0) fence_proxy_async_smem();  // this stage's reads and zeroing before its refill
       issue_one();
@@ -461,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
       }
       const int64_t item0 = seg_end - item_end;  // the line's unit where this item begins
       if (done && item0 >= begin) {
-        const float f0 = F0 > 0.f ? 1.f / F0 : 0.f, f1 = F1 > 0.f ? 1.f / F1 : 0.f;
+        const float f0 = 1.f / F0, f1 = 1.f / F1;
         const float i0 = l0 != 0.f ? 1.f / l0 : 0.f, i1 = l1 != 0.f ? 1.f / l1 : 0.f;
         T* o0 = static_cast<T*>(a.out) + qrow * a.o_srow + static_cast<int64_t>(hq0 + 2 * c) * a.o_shead;
         T* o1 = o0 + a.o_shead;
@@ -482,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
         const int64_t slot = 2 * static_cast<int64_t>(gw) + (item0 <= begin ? 0 : 1);
         float* po = a.part_o + slot * 8 * D;
         float2* ml = a.part_ml + slot * 8;
-        const float i0 = F0 > 0.f ? 1.f / F0 : 0.f, i1 = F1 > 0.f ? 1.f / F1 : 0.f;
+        const float i0 = 1.f / F0, i1 = 1.f / F1;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           const int d = 16 * k + 2 * r;
@@ -499,10 +541,17 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
       fresh = true;
     }
     pos = seg_end;
-    next_issue -= cur.n;
     cur = nxt;
+    if (!on_next) {  // everything of the old segment is issued: go on with this one
+#pragma unroll
+      for (int p = 0; p < NP; ++p) prow[p] = cur.row[p];
+      ph = cur.h;
+      pn = cur.n;
+      pi = 0;
+    }
+    on_next = false;
     nxt = load_seg();
-    while (filled - used < NS && issue_one()) {
+    while (flight < NS && issue_one()) {
     }
   }
 }
@@ -527,13 +576,16 @@ __global__ void __launch_bounds__(256) merge_fp8_kernel(DecodeFp8Args a, int war
       for (int i = tid; i < nh * D; i += 256) out[(i / D) * a.o_shead + i % D] = from_f32<T>(0.f);
     return;
   }
-  const int64_t total = static_cast<int64_t>(a.cu_units[a.S]) * ips;
-  const int64_t share = share_of(total, warps);
-  const int64_t first = static_cast<int64_t>(a.cu_units[s]) * ips + static_cast<int64_t>(hc) * units;
+  const int ts = team_of(ips);
+  const int64_t total = static_cast<int64_t>(a.cu_units[a.S]) * (ips / ts);
+  const int64_t share = share_of(total, warps / ts);
+  const int64_t first = static_cast<int64_t>(a.cu_units[s]) * (ips / ts) + static_cast<int64_t>(hc / ts) * units;
   const int64_t w0 = first / share, w1 = (first + units - 1) / share;
-  if (w0 == w1) return;  // written by its warp
+  if (w0 == w1) return;  // written by its one warp
   const int n = static_cast<int>(w1 - w0) + 1;
-  const auto slot_of = [&](int i) { return 2 * (w0 + i) + (i == 0 && first > w0 * share ? 1 : 0); };
+  const auto slot_of = [&](int i) {
+    return 2 * ((w0 + i) * ts + hc % ts) + (i == 0 && first > w0 * share ? 1 : 0);
+  };
   // every head's largest reference, then each part's weight
   constexpr int kVec = D / 4;                    // float4s of a head
   const int lanes = nh * kVec;                   // at most 256
