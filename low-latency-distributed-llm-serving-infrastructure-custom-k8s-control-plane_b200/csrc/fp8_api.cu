@@ -127,7 +127,7 @@ DecodePlan decode_plan(const B200AttentionFp8Params& p) {
   const int64_t most = static_cast<int64_t>(p.block_table_stride) * c.block_size;
   if (pl.max_ctx > most) pl.max_ctx = most;
   if (pl.max_ctx < 0) pl.max_ctx = 0;
-  pl.grid = b200::decode_fp8_grid(S, pl.max_ctx, c.num_kv_heads * pl.nchunks, p.dtype, num_sms());
+  pl.grid = b200::decode_fp8_grid(S, pl.max_ctx, c.num_kv_heads * pl.nchunks, num_sms());
   const size_t parts = b200::decode_fp8_parts(pl.grid);
   pl.off_ml = align256((S + 1) * sizeof(int32_t));
   pl.off_o = pl.off_ml + align256(parts * 8 * sizeof(float2));

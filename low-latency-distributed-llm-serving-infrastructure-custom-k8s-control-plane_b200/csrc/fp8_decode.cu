@@ -1,6 +1,6 @@
 // Decode over an 8-bit paged cache on the tensor cores (mma.sync; one new token per sequence).
 //
-// The batch's work is one line of units of 16 tokens: sequence by sequence, KV head by KV head (and
+// The batch's work is one line of units of 32 tokens: sequence by sequence, KV head by KV head (and
 // tile of 8 query heads by tile).  Every warp of a persistent grid takes an equal share of that
 // line, so the shares differ by one unit at most however the context lengths are spread, and runs
 // by itself: its own TMA ring, its own softmax, no CTA-wide synchronisation.  A warp writes an
@@ -8,7 +8,7 @@
 // of the first and the last item of its share it may hold only a part, which it leaves in the
 // workspace for the merge kernel that follows.
 //
-// Per unit: K (16 x D codes) by ldmatrix, four codes of a row per lane and register, widened to
+// Per 16 tokens: K (16 x D codes) by ldmatrix, four codes of a row per lane and register, widened to
 // f16 in registers (exact).  The order of the dims inside a k-step of 16 is free as long as Q has
 // it too, so a lane's four adjacent codes serve two k-columns each.  V by transposing ldmatrix on
 // pairs of codes (two adjacent dims as one 16-bit element) and one byte permutation.
@@ -20,7 +20,7 @@
 // products inside f16's normal range whatever the scales are (11 bits of every weight that is
 // within 2^-22 of the head's largest).
 //
-// Bound: HBM (4 * G flop per byte).  A unit is 32 * D bytes.
+// Bound: HBM (4 * G flop per byte).  A unit is 64 * D bytes.
 #include <cuda.h>
 
 #include "fp8.cuh"
@@ -31,16 +31,18 @@ namespace b200 {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kCtasPerSm = 3;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kMinShare = 4;   // units per warp at least: a shorter share costs more in the merge
+constexpr int kUnit = 32;      // tokens
+constexpr int kMinShare = 2;   // units per warp at least: a shorter share costs more in the merge
 constexpr float kUnset = 0x1p+126f;  // F before a page with a nonzero value scale: any scale moves it
 constexpr float kLazy = 8.f;   // log2 of how far p may exceed 1 before the reference moves
 
 template <int D>
 struct Ring {
-  static constexpr int kTile = 16 * D;       // codes of one unit of K (or V)
+  static constexpr int kTile = kUnit * D;    // codes of one unit of K (or V)
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kStages = 12288 / kStage;  // 12 KB per warp: 3 stages of D 128, 6 of D 64
+  static constexpr int kStages = 16384 / kStage;  // 16 KB per warp: 2 stages of D 128, 4 of D 64
   static constexpr int kWarpBytes = kStages * kStage;
 };
 
@@ -82,7 +84,7 @@ __device__ void prefix_units(const DecodeFp8Args& a, int32_t* cu, int32_t* warp_
     if (s < a.S) {
       const int32_t ctx = min(a.ctx_lens[s], a.max_ctx);
       const bool decoded = a.cu_q == nullptr || a.cu_q[s + 1] - a.cu_q[s] == 1;
-      if (decoded && ctx > 0) n = (ctx + 15) >> 4;
+      if (decoded && ctx > 0) n = (ctx + kUnit - 1) / kUnit;
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -114,9 +116,9 @@ __device__ __forceinline__ int64_t share_of(int64_t total, int warps) {
   return w > kMinShare ? w : kMinShare;
 }
 
-// Up to 32 consecutive units of one item; lane i holds unit i's first cache row and scales (of its
-// two pages where a page holds 8 tokens).  A page that does not take part has kBad set: the row is
-// then one of the pool's first page.
+// Up to 32 consecutive units of one item; lane i holds the first cache rows and the scales of unit
+// i's NP pieces: halves of 16 tokens, or quarters of 8 where a page holds 8.  kBad marks a piece
+// that does not take part: behind the context, or on a page outside the pool.
 constexpr uint32_t kBad = 0x80000000u;
 
 template <int NP>
@@ -127,12 +129,13 @@ struct Seg {
 };
 
 template <typename T, int D, int NP, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
     decode_fp8_kernel(const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, DecodeFp8Args a) {
   using R = Ring<D>;
   constexpr int NS = R::kStages;
   constexpr int KS = D / 16;
+  constexpr int kPiece = kUnit / NP;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base_u32 = (raw_u32 + 1023u) & ~1023u;
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
     const int32_t* table = a.bt + static_cast<int64_t>(g.s) * a.bt_stride;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const int t = (g.u0 + lane) * 16 + p * 8;
+      const int t = (g.u0 + lane) * kUnit + p * kPiece;
       const int page = t / a.bs;
       int32_t b = 0;
       uint32_t bad = kBad;
@@ -248,16 +251,21 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
       pi = 0;
     }
     uint32_t row[NP];
+    uint32_t bytes = 0;
 #pragma unroll
-    for (int p = 0; p < NP; ++p) row[p] = __shfl_sync(0xffffffffu, prow[p], pi) & ~kBad;
+    for (int p = 0; p < NP; ++p) {
+      row[p] = __shfl_sync(0xffffffffu, prow[p], pi);
+      if (!(row[p] & kBad)) bytes += 2 * kPiece * D;
+    }
     if (lane == 0) {
       uint64_t* bar = &my_bars[pstage];
       uint8_t* dst = ring + pstage * R::kStage;
-      mbar_arrive_expect_tx(bar, R::kStage);
+      mbar_arrive_expect_tx(bar, bytes);
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        tma_load_3d(dst + p * 8 * D, &kmap, bar, 0, ph, static_cast<int32_t>(row[p]));
-        tma_load_3d(dst + R::kTile + p * 8 * D, &vmap, bar, 0, ph, static_cast<int32_t>(row[p]));
+        if (row[p] & kBad) continue;
+        tma_load_3d(dst + p * kPiece * D, &kmap, bar, 0, ph, static_cast<int32_t>(row[p]));
+        tma_load_3d(dst + R::kTile + p * kPiece * D, &vmap, bar, 0, ph, static_cast<int32_t>(row[p]));
       }
     }
     ++pi;
@@ -339,89 +347,111 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
       }
       const uint32_t kb = ring_u32 + cstage * R::kStage + lane_at;
       const uint32_t vb = kb + R::kTile;
-      uint32_t row[NP];
-      float ks[2], vs[2];
+      uint32_t bad = 0;
+      float ks[NP], vs[NP];
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        row[p] = __shfl_sync(0xffffffffu, cur.row[p], i);
+        bad |= (__shfl_sync(0xffffffffu, cur.row[p], i) >> 31) << p;
         ks[p] = __shfl_sync(0xffffffffu, cur.ks[p], i);
         vs[p] = __shfl_sync(0xffffffffu, cur.vs[p], i);
       }
-      if (NP == 1) {
-        ks[1] = ks[0];
-        vs[1] = vs[0];
-      }
-      const int valid = cur.ctx - (cur.u0 + i) * 16;  // tokens of the unit inside the context
-      const bool whole = valid >= 16 && !((row[0] | row[NP - 1]) & kBad);
-      const bool in0 = r < valid && !(row[0] & kBad);           // token r of the unit takes part
-      const bool in1 = r + 8 < valid && !(row[NP - 1] & kBad);  // token r + 8
+      const int valid = cur.ctx - (cur.u0 + i) * kUnit;  // tokens of the unit inside the context
+      const bool whole = valid >= kUnit && bad == 0;
+      // token t of the unit takes part
+      const auto takes_part = [&](int t) { return t < valid && !((bad >> (t / kPiece)) & 1u); };
       if (!whole) {
         // rows that do not take part may hold anything, NaN codes among it: their V is zeroed
         uint8_t* v = ring + cstage * R::kStage + R::kTile;
-        for (int idx = lane; idx < 16 * (D / 16); idx += 32) {
+        for (int idx = lane; idx < kUnit * (D / 16); idx += 32) {
           const int rr = idx / (D / 16), ch = idx % (D / 16);
-          if (rr >= valid || (row[rr < 8 ? 0 : NP - 1] & kBad))
+          if (!takes_part(rr))
             *reinterpret_cast<uint4*>(v + tile_at<D>(rr, ch)) = make_uint4(0u, 0u, 0u, 0u);
         }
         __syncwarp();
       }
 
-      // ---- S^T = K Q^T -------------------------------------------------------------------
-      float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
+      // ---- S^T = K Q^T: s[j] has tokens 16j + r (elements 0, 1) and 16j + r + 8 (2, 3) -----------
+      float s[2][4];
 #pragma unroll
-      for (int k = 0; k < KS; k += 2) {
-        uint32_t x0, x1, x2, x3;
-        ldmatrix_x4(kb ^ (k << 4), x0, x1, x2, x3);
-        {
-          const uint32_t a0 = cvt_e4m3x2(x0), a1 = cvt_e4m3x2(x1), a2 = cvt_e4m3x2_hi(x0), a3 = cvt_e4m3x2_hi(x1);
-          MmaOp<__half>::run(sa, a0, a1, a2, a3, qf[k][0], qf[k][1]);
-          if (SPLIT) MmaOp<__half>::run(sa, a0, a1, a2, a3, ql[k][0], ql[k][1]);
+      for (int j = 0; j < 2; ++j) {
+        float sb[4] = {0.f, 0.f, 0.f, 0.f};
+        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; k += 2) {
+          uint32_t x0, x1, x2, x3;
+          ldmatrix_x4((kb ^ (k << 4)) + j * 16 * D, x0, x1, x2, x3);
+          {
+            const uint32_t a0 = cvt_e4m3x2(x0), a1 = cvt_e4m3x2(x1), a2 = cvt_e4m3x2_hi(x0), a3 = cvt_e4m3x2_hi(x1);
+            MmaOp<__half>::run(s[j], a0, a1, a2, a3, qf[k][0], qf[k][1]);
+            if (SPLIT) MmaOp<__half>::run(s[j], a0, a1, a2, a3, ql[k][0], ql[k][1]);
+          }
+          {
+            const uint32_t a0 = cvt_e4m3x2(x2), a1 = cvt_e4m3x2(x3), a2 = cvt_e4m3x2_hi(x2), a3 = cvt_e4m3x2_hi(x3);
+            MmaOp<__half>::run(sb, a0, a1, a2, a3, qf[k + 1][0], qf[k + 1][1]);
+            if (SPLIT) MmaOp<__half>::run(sb, a0, a1, a2, a3, ql[k + 1][0], ql[k + 1][1]);
+          }
         }
-        {
-          const uint32_t a0 = cvt_e4m3x2(x2), a1 = cvt_e4m3x2(x3), a2 = cvt_e4m3x2_hi(x2), a3 = cvt_e4m3x2_hi(x3);
-          MmaOp<__half>::run(sb, a0, a1, a2, a3, qf[k + 1][0], qf[k + 1][1]);
-          if (SPLIT) MmaOp<__half>::run(sb, a0, a1, a2, a3, ql[k + 1][0], ql[k + 1][1]);
-        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] += sb[e];
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sa[j] += sb[j];
-      const float c0 = ks[0] * qscale0, c1 = ks[0] * qscale1, c2 = ks[1] * qscale0, c3 = ks[1] * qscale1;
 
-      // ---- softmax with a lazily moved reference --------------------------------------------
-      float y0 = fmaf(sa[0], c0, -m0), y1 = fmaf(sa[1], c1, -m1);
-      float y2 = fmaf(sa[2], c2, -m0), y3 = fmaf(sa[3], c3, -m1);
-      if (!whole) {
-        if (!in0) y0 = y1 = -INFINITY;
-        if (!in1) y2 = y3 = -INFINITY;
+      // ---- softmax with a lazily moved reference: y = score - m, in log2 units -------------------
+      float y[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float ka = ks[j * NP / 2], kc = ks[(j + 1) * NP / 2 - 1];  // of rows r and r + 8
+        y[j][0] = fmaf(s[j][0], ka * qscale0, -m0);
+        y[j][1] = fmaf(s[j][1], ka * qscale1, -m1);
+        y[j][2] = fmaf(s[j][2], kc * qscale0, -m0);
+        y[j][3] = fmaf(s[j][3], kc * qscale1, -m1);
+        if (!whole) {
+          if (!takes_part(16 * j + r)) y[j][0] = y[j][1] = -INFINITY;
+          if (!takes_part(16 * j + r + 8)) y[j][2] = y[j][3] = -INFINITY;
+        }
       }
-      const float vmax = NP == 1 ? vs[0] : fmaxf(vs[0], vs[1]);
-      const bool move = fmaxf(fmaxf(y0, y1), fmaxf(y2, y3)) > kLazy || vmax * fmaxf(F0, F1) > 128.f;
+      float vmax = vs[0], top = y[0][0];
+#pragma unroll
+      for (int p = 1; p < NP; ++p) vmax = fmaxf(vmax, vs[p]);
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, y[e >> 2][e & 3]);
+      const bool move = top > kLazy || vmax * fmaxf(F0, F1) > 128.f;
       if (__any_sync(0xffffffffu, move)) {
-        y0 = in0 ? sa[0] * c0 : -INFINITY;
-        y1 = in0 ? sa[1] * c1 : -INFINITY;
-        y2 = in1 ? sa[2] * c2 : -INFINITY;
-        y3 = in1 ? sa[3] * c3 : -INFINITY;
-        float t0 = fmaxf(y0, y2), t1 = fmaxf(y1, y3);
+        float t0 = m0, t1 = m1;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float ka = ks[j * NP / 2], kc = ks[(j + 1) * NP / 2 - 1];
+          y[j][0] = s[j][0] * (ka * qscale0);
+          y[j][1] = s[j][1] * (ka * qscale1);
+          y[j][2] = s[j][2] * (kc * qscale0);
+          y[j][3] = s[j][3] * (kc * qscale1);
+          if (!takes_part(16 * j + r)) y[j][0] = y[j][1] = -INFINITY;
+          if (!takes_part(16 * j + r + 8)) y[j][2] = y[j][3] = -INFINITY;
+          t0 = fmaxf(t0, fmaxf(y[j][0], y[j][2]));
+          t1 = fmaxf(t1, fmaxf(y[j][1], y[j][3]));
+        }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
           t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
           t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
         }
-        t0 = fmaxf(m0, t0);
-        t1 = fmaxf(m1, t1);
         const float u0 = t0 == -INFINITY ? 0.f : t0, u1 = t1 == -INFINITY ? 0.f : t1;
         float al0 = fast_exp2(m0 - u0), al1 = fast_exp2(m1 - u1);
         l0 *= al0;
         l1 *= al1;
         m0 = t0;
         m1 = t1;
-        y0 -= u0;
-        y1 -= u1;
-        y2 -= u0;
-        y3 -= u1;
         // the largest product p * vs of the unit, per head
-        float w0 = fmaxf(fast_exp2(y0) * vs[0], fast_exp2(y2) * vs[1]);
-        float w1 = fmaxf(fast_exp2(y1) * vs[0], fast_exp2(y3) * vs[1]);
+        float w0 = 0.f, w1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float va = vs[j * NP / 2], vc = vs[(j + 1) * NP / 2 - 1];
+          y[j][0] -= u0;
+          y[j][1] -= u1;
+          y[j][2] -= u0;
+          y[j][3] -= u1;
+          w0 = fmaxf(w0, fmaxf(fast_exp2(y[j][0]) * va, fast_exp2(y[j][2]) * vc));
+          w1 = fmaxf(w1, fmaxf(fast_exp2(y[j][1]) * va, fast_exp2(y[j][3]) * vc));
+        }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
           w0 = fmaxf(w0, __shfl_xor_sync(0xffffffffu, w0, o));
@@ -444,43 +474,50 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : 4)
           acc[k][3] *= al1;
         }
       }
-      float p0 = fast_exp2(y0), p1 = fast_exp2(y1), p2 = fast_exp2(y2), p3 = fast_exp2(y3);
-      l0 += p0 + p2;
-      l1 += p1 + p3;
-      p0 *= vs[0] * F0;
-      p1 *= vs[0] * F1;
-      p2 *= vs[1] * F0;
-      p3 *= vs[1] * F1;
-      const uint32_t ph0 = pack_f16(p0, p1), ph1 = pack_f16(p2, p3);
-      const uint32_t pb0 = movmatrix_trans(ph0), pb1 = movmatrix_trans(ph1);
-      uint32_t pl0 = 0, pl1 = 0;
-      if (SPLIT) {
-        const __half2 h0 = *reinterpret_cast<const __half2*>(&ph0);
-        const __half2 h1 = *reinterpret_cast<const __half2*>(&ph1);
-        pl0 = movmatrix_trans(pack_f16(p0 - __low2float(h0), p1 - __high2float(h0)));
-        pl1 = movmatrix_trans(pack_f16(p2 - __low2float(h1), p3 - __high2float(h1)));
+      uint32_t pb[2][2], pl[SPLIT ? 2 : 1][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float va = vs[j * NP / 2], vc = vs[(j + 1) * NP / 2 - 1];
+        float p0 = fast_exp2(y[j][0]), p1 = fast_exp2(y[j][1]), p2 = fast_exp2(y[j][2]), p3 = fast_exp2(y[j][3]);
+        l0 += p0 + p2;
+        l1 += p1 + p3;
+        p0 *= va * F0;
+        p1 *= va * F1;
+        p2 *= vc * F0;
+        p3 *= vc * F1;
+        const uint32_t ph0 = pack_f16(p0, p1), ph1 = pack_f16(p2, p3);
+        pb[j][0] = movmatrix_trans(ph0);
+        pb[j][1] = movmatrix_trans(ph1);
+        if (SPLIT) {
+          const __half2 h0 = *reinterpret_cast<const __half2*>(&ph0);
+          const __half2 h1 = *reinterpret_cast<const __half2*>(&ph1);
+          pl[j][0] = movmatrix_trans(pack_f16(p0 - __low2float(h0), p1 - __high2float(h0)));
+          pl[j][1] = movmatrix_trans(pack_f16(p2 - __low2float(h1), p3 - __high2float(h1)));
+        }
       }
 
       // ---- O^T += V^T P^T: row r of a 16-dim tile is dim 2r, row r + 8 dim 2r + 1 ------------
 #pragma unroll
-      for (int k = 0; k < KS; k += 2) {
-        uint32_t z0, z1, z2, z3;
-        ldmatrix_x4_trans(vb ^ (k << 4), z0, z1, z2, z3);
-        z0 = __byte_perm(z0, 0, 0x3120);
-        z1 = __byte_perm(z1, 0, 0x3120);
-        z2 = __byte_perm(z2, 0, 0x3120);
-        z3 = __byte_perm(z3, 0, 0x3120);
-        {
-          const uint32_t a0 = cvt_e4m3x2(z0), a1 = cvt_e4m3x2_hi(z0), a2 = cvt_e4m3x2(z1), a3 = cvt_e4m3x2_hi(z1);
-          MmaOp<__half>::run(acc[k], a0, a1, a2, a3, pb0, pb1);
-          if (SPLIT) MmaOp<__half>::run(acc[k], a0, a1, a2, a3, pl0, pl1);
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int k = 0; k < KS; k += 2) {
+          uint32_t z0, z1, z2, z3;
+          ldmatrix_x4_trans((vb ^ (k << 4)) + j * 16 * D, z0, z1, z2, z3);
+          z0 = __byte_perm(z0, 0, 0x3120);
+          z1 = __byte_perm(z1, 0, 0x3120);
+          z2 = __byte_perm(z2, 0, 0x3120);
+          z3 = __byte_perm(z3, 0, 0x3120);
+          {
+            const uint32_t a0 = cvt_e4m3x2(z0), a1 = cvt_e4m3x2_hi(z0), a2 = cvt_e4m3x2(z1), a3 = cvt_e4m3x2_hi(z1);
+            MmaOp<__half>::run(acc[k], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+            if (SPLIT) MmaOp<__half>::run(acc[k], a0, a1, a2, a3, pl[j][0], pl[j][1]);
+          }
+          {
+            const uint32_t a0 = cvt_e4m3x2(z2), a1 = cvt_e4m3x2_hi(z2), a2 = cvt_e4m3x2(z3), a3 = cvt_e4m3x2_hi(z3);
+            MmaOp<__half>::run(acc[k + 1], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+            if (SPLIT) MmaOp<__half>::run(acc[k + 1], a0, a1, a2, a3, pl[j][0], pl[j][1]);
+          }
         }
-        {
-          const uint32_t a0 = cvt_e4m3x2(z2), a1 = cvt_e4m3x2_hi(z2), a2 = cvt_e4m3x2(z3), a3 = cvt_e4m3x2_hi(z3);
-          MmaOp<__half>::run(acc[k + 1], a0, a1, a2, a3, pb0, pb1);
-          if (SPLIT) MmaOp<__half>::run(acc[k + 1], a0, a1, a2, a3, pl0, pl1);
-        }
-      }
       --flight;
       if (++cstage == NS) {
         cstage = 0;
@@ -660,18 +697,18 @@ template <typename T, bool SPLIT>
 cudaError_t launch_d(const CUtensorMap& km, const CUtensorMap& vm, const DecodeFp8Args& a, int grid,
                      cudaStream_t stream) {
   if (a.head_dim == 128)
-    return a.bs == 8 ? launch_t<T, 128, 2, SPLIT>(km, vm, a, grid, stream)
-                     : launch_t<T, 128, 1, SPLIT>(km, vm, a, grid, stream);
-  return a.bs == 8 ? launch_t<T, 64, 2, SPLIT>(km, vm, a, grid, stream)
-                   : launch_t<T, 64, 1, SPLIT>(km, vm, a, grid, stream);
+    return a.bs == 8 ? launch_t<T, 128, 4, SPLIT>(km, vm, a, grid, stream)
+                     : launch_t<T, 128, 2, SPLIT>(km, vm, a, grid, stream);
+  return a.bs == 8 ? launch_t<T, 64, 4, SPLIT>(km, vm, a, grid, stream)
+                   : launch_t<T, 64, 2, SPLIT>(km, vm, a, grid, stream);
 }
 
 }  // namespace
 
-int decode_fp8_grid(int S, int64_t max_ctx, int ips, int dtype, int num_sms) {
-  const int64_t units = static_cast<int64_t>(S) * ((max_ctx + 15) / 16) * ips;
+int decode_fp8_grid(int S, int64_t max_ctx, int ips, int num_sms) {
+  const int64_t units = static_cast<int64_t>(S) * ((max_ctx + kUnit - 1) / kUnit) * ips;
   const int64_t need = (units + kMinShare * kWarps - 1) / (kMinShare * kWarps);
-  const int64_t most = static_cast<int64_t>(num_sms) * (dtype == B200_DTYPE_F32 ? 3 : 4);
+  const int64_t most = static_cast<int64_t>(num_sms) * kCtasPerSm;
   return static_cast<int>(need < 1 ? 1 : need < most ? need : most);
 }
 

@@ -30,7 +30,7 @@ struct DecodeFp8Args {
 };
 
 // CTAs of a launch, and the parts that they may leave behind.
-int decode_fp8_grid(int S, int64_t max_ctx, int ips, int dtype, int num_sms);
+int decode_fp8_grid(int S, int64_t max_ctx, int ips, int num_sms);
 int decode_fp8_parts(int grid);
 cudaError_t launch_decode_fp8(int dtype, const CUtensorMap& km, const CUtensorMap& vm,
                               const DecodeFp8Args& a, int grid, cudaStream_t stream);
