@@ -193,6 +193,8 @@ int run_decode(const B200AttentionFp8Params& p, const DecodePlan& pl, const int6
     // without a map, sequence s reads and writes row s of the call
     const int64_t shift = cu_q || p.query_rows ? 0 : s0;
     a.q = static_cast<const char*>(p.query) + shift * p.q_stride_row * esize_of(p.dtype);
+    const size_t four = 4 * esize_of(p.dtype);
+    a.vec_q = reinterpret_cast<uintptr_t>(a.q) % four == 0 && a.q_srow % 4 == 0 && a.q_shead % 4 == 0;
     a.out = static_cast<char*>(p.out) + shift * p.o_stride_row * esize_of(p.dtype);
     const cudaError_t e = b200::launch_decode_fp8(p.dtype, km, vm, a, pl.grid, st);
     if (e != cudaSuccess) return cuda_fail(e, "paged_decode_fp8");

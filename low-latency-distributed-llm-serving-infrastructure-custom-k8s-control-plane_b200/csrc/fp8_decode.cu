@@ -25,16 +25,18 @@
 
 #include "fp8.cuh"
 #include "fp8_decode.cuh"
+#include "tc05.cuh"
 
 namespace b200 {
 
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;  // consumer warps
 constexpr int kCtasPerSm = 3;
-constexpr int kThreads = 32 * kWarps;
+constexpr int kThreads = 32 * (kWarps + 1);  // the last warp loads for the others
 constexpr int kUnit = 32;      // tokens
-constexpr int kMinShare = 2;   // units per warp at least: a shorter share costs more in the merge
+constexpr int kMinShare = 4;   // places on the line per warp at least: a shorter share costs more in the merge
+constexpr int kItemCost = 3;   // what beginning an item costs, in units: part of its length on the line
 constexpr float kUnset = 0x1p+126f;  // F before a page with a nonzero value scale: any scale moves it
 constexpr float kLazy = 8.f;   // log2 of how far p may exceed 1 before the reference moves
 
@@ -66,6 +68,23 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
   return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
+// Four adjacent elements of a query row (aligned to four elements).
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, bool take, float (&v)[4]) {
+  uint2 u = take ? *reinterpret_cast<const uint2*>(p) : make_uint2(0u, 0u);
+  const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = to_f32<T>(e[j]);
+}
+template <>
+__device__ __forceinline__ void load4<float>(const float* p, bool take, float (&v)[4]) {
+  const float4 u = take ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+  v[0] = u.x;
+  v[1] = u.y;
+  v[2] = u.z;
+  v[3] = u.w;
+}
+
 // 2^(up - e) with mx in [1, 2) * 2^e: an exact power of two, within fp32's normal range.
 __device__ __forceinline__ float pow2_inverse(float mx, int up) {
   int e = static_cast<int>(__float_as_uint(mx) >> 23);
@@ -73,7 +92,7 @@ __device__ __forceinline__ float pow2_inverse(float mx, int up) {
   return __uint_as_float(static_cast<uint32_t>(e) << 23);
 }
 
-// Inclusive prefix sums of the sequences' units into cu[1..S], cu[0] = 0.  Whole CTA.
+// Inclusive prefix sums of the lengths of the sequences' items (units and kItemCost) into cu[1..S], cu[0] = 0.  Whole CTA.
 __device__ void prefix_units(const DecodeFp8Args& a, int32_t* cu, int32_t* warp_sums) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int32_t carry = 0;
@@ -84,7 +103,7 @@ __device__ void prefix_units(const DecodeFp8Args& a, int32_t* cu, int32_t* warp_
     if (s < a.S) {
       const int32_t ctx = min(a.ctx_lens[s], a.max_ctx);
       const bool decoded = a.cu_q == nullptr || a.cu_q[s + 1] - a.cu_q[s] == 1;
-      if (decoded && ctx > 0) n = (ctx + kUnit - 1) / kUnit;
+      if (decoded && ctx > 0) n = (ctx + kUnit - 1) / kUnit + kItemCost;
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -94,12 +113,12 @@ __device__ void prefix_units(const DecodeFp8Args& a, int32_t* cu, int32_t* warp_
     if (lane == 31) warp_sums[warp] = n;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w <= kWarps; ++w) {
       if (w < warp) n += warp_sums[w];
     }
     if (s < a.S) cu[s + 1] = carry + n;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) carry += warp_sums[w];
+    for (int w = 0; w <= kWarps; ++w) carry += warp_sums[w];
     __syncthreads();
   }
 }
@@ -111,22 +130,96 @@ __device__ __forceinline__ int team_of(int items) {
   return items % 4 == 0 ? 4 : items % 2 == 0 ? 2 : 1;
 }
 
+// a / b (64-bit division only where it is needed: it costs some hundred cycles)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
 __device__ __forceinline__ int64_t share_of(int64_t total, int warps) {
-  const int64_t w = (total + warps - 1) / warps;
+  const int64_t w = quotient(total + warps - 1, warps);
   return w > kMinShare ? w : kMinShare;
 }
 
-// Up to 32 consecutive units of one item; lane i holds the first cache rows and the scales of unit
-// i's NP pieces: halves of 16 tokens, or quarters of 8 where a page holds 8.  kBad marks a piece
-// that does not take part: behind the context, or on a page outside the pool.
+// Non-blocking form of mbar_try_wait: the producer looks at several barriers in turn.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t phase) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(phase)
+      : "memory");
+  return ok != 0;
+}
+
+// What the producer tells a consumer about a unit: scales of its NP pieces (halves of 16 tokens, or
+// quarters of 8 where a page holds 8) and a bit for each piece that does not take part (behind the
+// context, or on a page outside the pool).
+struct UnitMeta {
+  float ks[4], vs[4];
+  uint32_t bad;
+  uint32_t pad[3];
+};
+
 constexpr uint32_t kBad = 0x80000000u;
 
-template <int NP>
-struct Seg {
-  int s, hc, h, u0, n, units, ctx;
-  uint32_t row[NP];
-  float ks[NP], vs[NP];
+// One warp's walk along its share of the line.
+struct Walk {
+  int64_t at, end;          // next unit and the end of the share
+  int seq, hc, u;           // where `at` is: sequence, team's item, place in the item
 };
+
+__device__ __forceinline__ Walk start_walk(const int32_t* cu, int S, int ips, int64_t at, int64_t end) {
+  Walk w{at, end, 0, 0, 0};
+  if (at >= end) return w;
+  int lo = 0, hi = S - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (static_cast<int64_t>(cu[mid + 1]) * ips > at) hi = mid; else lo = mid + 1;
+  }
+  w.seq = lo;
+  const int64_t rem = at - static_cast<int64_t>(cu[lo]) * ips;
+  const int length = cu[lo + 1] - cu[lo];
+  w.hc = static_cast<int>(rem / length);
+  w.u = static_cast<int>(rem - static_cast<int64_t>(w.hc) * length);
+  return w;
+}
+
+// Takes up to `most` units of one item: sequence, item, first unit and count (0 at the share's end).
+// The first kItemCost places of an item hold no unit.
+__device__ __forceinline__ int next_piece(Walk& w, const int32_t* cu, int ips, int most, int& s, int& hc,
+                                          int& u0) {
+  for (;;) {
+    if (w.at >= w.end) return 0;
+    const int length = cu[w.seq + 1] - cu[w.seq];
+    if (length == 0) {
+      ++w.seq;
+      continue;
+    }
+    if (w.u < kItemCost) {
+      const int skip = static_cast<int>(min(static_cast<int64_t>(kItemCost - w.u), w.end - w.at));
+      w.at += skip;
+      w.u += skip;
+      if (w.at >= w.end) return 0;
+    }
+    s = w.seq;
+    hc = w.hc;
+    u0 = w.u - kItemCost;
+    const int n = static_cast<int>(min(min(static_cast<int64_t>(length - w.u), w.end - w.at), static_cast<int64_t>(most)));
+    w.at += n;
+    w.u += n;
+    if (w.u == length) {
+      w.u = 0;
+      if (++w.hc == ips) {
+        w.hc = 0;
+        ++w.seq;
+      }
+    }
+    return n;
+  }
+}
 
 template <typename T, int D, int NP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
@@ -140,14 +233,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base_u32 = (raw_u32 + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base_u32 - raw_u32);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kWarps * R::kWarpBytes);
-  int32_t* warp_sums = reinterpret_cast<int32_t*>(bars + kWarps * NS);
-  int32_t* cu = warp_sums + kWarps;  // [S + 1]
+  UnitMeta* meta = reinterpret_cast<UnitMeta*>(smem + kWarps * R::kWarpBytes);  // [kWarps][NS]
+  uint64_t* full = reinterpret_cast<uint64_t*>(meta + kWarps * NS);             // [kWarps][NS]
+  uint64_t* empty = full + kWarps * NS;
+  int32_t* warp_sums = reinterpret_cast<int32_t*>(empty + kWarps * NS);
+  volatile int32_t* abort_s = warp_sums + kWarps + 1;
+  int32_t* cu = warp_sums + kWarps + 2;  // [S + 1]
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r = lane >> 2, c = lane & 3;
   if (tid == 0) {
-    for (int i = 0; i < kWarps * NS; ++i) mbar_init(&bars[i], 1);
+    *abort_s = 0;
+    for (int i = 0; i < kWarps * NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
     fence_proxy_async_smem();
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
@@ -157,159 +256,196 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     for (int i = tid; i <= a.S; i += kThreads) a.cu_units[i] = cu[i];
   __syncthreads();
 
+  asm volatile("griddepcontrol.launch_dependents;");
   // teams of ts warps walk the line side by side, each warp with an item of its own
   const int ts = team_of(a.hkv * a.nchunks), ips = a.hkv * a.nchunks / ts;
   const int64_t total = static_cast<int64_t>(cu[a.S]) * ips;
   const int64_t share = share_of(total, static_cast<int>(gridDim.x) * (kWarps / ts));
-  const int gw = blockIdx.x * kWarps + warp;
-  int64_t at = gw / ts * share;  // next unit of the line to make a segment of
-  const int64_t end = min(total, at + share);
-  if (at >= end) return;
-  const int64_t begin = at;
+  // this warp's share, or (producer) that of the consumer warp which this lane serves
+  const int who = warp < kWarps ? warp : lane >> 3;
+  const int gw = blockIdx.x * kWarps + who;
+  const int64_t begin = min(total, gw / ts * share), end = min(total, begin + share);
+  Walk walk = start_walk(cu, a.S, ips, begin, end);
 
-  uint8_t* ring = smem + warp * R::kWarpBytes;
-  const uint32_t ring_u32 = base_u32 + warp * R::kWarpBytes;
-  uint64_t* my_bars = bars + warp * NS;
+  if (warp == kWarps) {
+    // ======== producer: 8 lanes for each consumer warp ========================================
+    // Lane sl holds unit sl of the consumer's current 8 units (rows, scales) and of its next 8,
+    // whose page ids are asked for when the current 8 begin and whose scales two units later.
+    const int sl = lane & 7;
+    uint32_t row[NP], nrow[NP];
+    float ks[NP], vs[NP], nks[NP], nvs[NP];
+    int32_t nid[NP];
+    int h = 0, n = 0, i = 0;                       // current units: head, count, next to issue
+    int ns = 0, nhc = 0, nu0 = 0, nn = 0, nh = 0;  // next units
+    int nstate = 0;                                // 1: ids asked for, 2: scales asked for
+    uint8_t* ring = smem + who * R::kWarpBytes;
+    UnitMeta* my_meta = meta + who * NS;
+    uint64_t* my_full = full + who * NS;
+    uint64_t* my_empty = empty + who * NS;
+    int stage = 0;
+    uint32_t phase = 0, fills = 0;
 
-  int seq;  // sequence of `at`
-  {
-    int lo = 0, hi = a.S - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (static_cast<int64_t>(cu[mid + 1]) * ips > at) hi = mid; else lo = mid + 1;
-    }
-    seq = lo;
-  }
-  int64_t rem = at - static_cast<int64_t>(cu[seq]) * ips;
-  int hc_next = static_cast<int>(rem / (cu[seq + 1] - cu[seq]));
-  int u_next = static_cast<int>(rem - static_cast<int64_t>(hc_next) * (cu[seq + 1] - cu[seq]));
-
-  const auto load_seg = [&]() {
-    Seg<NP> g;
-    g.n = 0;
-    if (at >= end) return g;
-    while (cu[seq + 1] == cu[seq]) ++seq;
-    g.s = seq;
-    g.hc = hc_next * ts + warp % ts;
-    g.u0 = u_next;
-    g.units = cu[seq + 1] - cu[seq];
-    g.ctx = min(a.ctx_lens[seq], a.max_ctx);
-    g.n = static_cast<int>(min(min(static_cast<int64_t>(g.units - u_next), end - at), static_cast<int64_t>(32)));
-    at += g.n;
-    u_next += g.n;
-    if (u_next == g.units) {
-      u_next = 0;
-      if (++hc_next == ips) {
-        hc_next = 0;
-        ++seq;
-      }
-    }
-    g.h = g.hc / a.nchunks;
-    const int32_t* table = a.bt + static_cast<int64_t>(g.s) * a.bt_stride;
-#pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const int t = (g.u0 + lane) * kUnit + p * kPiece;
-      const int page = t / a.bs;
-      int32_t b = 0;
-      uint32_t bad = kBad;
-      g.ks[p] = g.vs[p] = 0.f;
-      if (lane < g.n && t < g.ctx) {
-        b = table[page];
-        if (b >= 0 && b < a.nb) {
-          bad = 0;
-          const int64_t sc = (static_cast<int64_t>(a.layer) * a.nb + b) * a.hkv + g.h;
-          g.ks[p] = a.ks[sc];
-          g.vs[p] = a.vs[sc];
-        } else {
-          b = 0;
-          flag_status(a.status, B200_DEVICE_BAD_BLOCK);
-        }
-      }
-      g.row[p] = static_cast<uint32_t>((a.layer * a.nb + b) * a.bs + (t - page * a.bs)) | bad;
-    }
-    return g;
-  };
-
-  Seg<NP> cur = load_seg();
-  Seg<NP> nxt = load_seg();
-  // the producer's side: the segment it issues from (cur, or nxt), the next unit there, and the
-  // ring's next stage; units in flight
-  uint32_t prow[NP];
-#pragma unroll
-  for (int p = 0; p < NP; ++p) prow[p] = cur.row[p];
-  int ph = cur.h, pn = cur.n, pi = 0, pstage = 0, flight = 0;
-  bool on_next = false;
-
-  const auto issue_one = [&]() -> bool {
-    if (pi == pn) {
-      if (on_next || nxt.n == 0) return false;
-      on_next = true;
-#pragma unroll
-      for (int p = 0; p < NP; ++p) prow[p] = nxt.row[p];
-      ph = nxt.h;
-      pn = nxt.n;
-      pi = 0;
-    }
-    uint32_t row[NP];
-    uint32_t bytes = 0;
-#pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      row[p] = __shfl_sync(0xffffffffu, prow[p], pi);
-      if (!(row[p] & kBad)) bytes += 2 * kPiece * D;
-    }
-    if (lane == 0) {
-      uint64_t* bar = &my_bars[pstage];
-      uint8_t* dst = ring + pstage * R::kStage;
-      mbar_arrive_expect_tx(bar, bytes);
+    const auto ask_ids = [&]() {
+      nn = next_piece(walk, cu, ips, 8, ns, nhc, nu0);
+      nstate = 1;
+      const int hc = nhc * ts + who % ts;
+      nh = hc / a.nchunks;
+      const int32_t ctx = nn > 0 ? min(a.ctx_lens[ns], a.max_ctx) : 0;
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        if (row[p] & kBad) continue;
-        tma_load_3d(dst + p * kPiece * D, &kmap, bar, 0, ph, static_cast<int32_t>(row[p]));
-        tma_load_3d(dst + R::kTile + p * kPiece * D, &vmap, bar, 0, ph, static_cast<int32_t>(row[p]));
+        const int t = (nu0 + sl) * kUnit + p * kPiece;
+        nid[p] = sl < nn && t < ctx ? a.bt[static_cast<int64_t>(ns) * a.bt_stride + t / a.bs] : -1;
+        if (sl < nn && t < ctx && (nid[p] < 0 || nid[p] >= a.nb)) flag_status(a.status, B200_DEVICE_BAD_BLOCK);
+      }
+      if (nn > 0 && (nu0 == 0 || fills == 0)) {
+        // the item's queries, on their way to L2 before the consumer asks for them
+        const int cch = hc - nh * a.nchunks;
+        const int64_t qrow = a.cu_q ? a.cu_q[ns] : (a.query_rows ? a.query_rows[ns] : ns);
+        if (cch * 8 + sl < a.group) {
+          const T* q = static_cast<const T*>(a.q) + qrow * a.q_srow +
+                       static_cast<int64_t>(nh * a.group + cch * 8 + sl) * a.q_shead;
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(q + D - 1));
+        }
+      }
+    };
+    const auto ask_scales = [&]() {
+      nstate = 2;
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const bool good = nid[p] >= 0 && nid[p] < a.nb;
+        const int32_t b = good ? nid[p] : 0;
+        const int t = (nu0 + sl) * kUnit + p * kPiece;
+        const int64_t sc = (static_cast<int64_t>(a.layer) * a.nb + b) * a.hkv + nh;
+        nks[p] = good ? a.ks[sc] : 0.f;
+        nvs[p] = good ? a.vs[sc] : 0.f;
+        nrow[p] = static_cast<uint32_t>((a.layer * a.nb + b) * a.bs + t % a.bs) | (good ? 0u : kBad);
+      }
+    };
+
+    ask_ids();
+    uint64_t idle_since = globaltimer_ns();
+    for (;;) {
+      if (i == n) {
+        if (nn > 0) {
+          if (nstate == 1) ask_scales();
+          n = nn;
+          h = nh;
+          i = 0;
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            row[p] = nrow[p];
+            ks[p] = nks[p];
+            vs[p] = nvs[p];
+          }
+          ask_ids();
+        }
+      } else if (nstate == 1 && i >= 2) {
+        ask_scales();
+      }
+      const bool left = i < n;
+      if (!__any_sync(0xffffffffu, left)) break;
+      const bool can = left && (fills < NS || mbar_test(&my_empty[stage], phase ^ 1u));
+      // one decision for the consumer's 8 lanes
+      const bool go = __shfl_sync(0xffffffffu, can ? 1 : 0, 0, 8) != 0;
+      uint32_t irow[NP], bad = 0, bytes = 0;
+      float iks[NP], ivs[NP];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        irow[p] = __shfl_sync(0xffffffffu, row[p], i & 7, 8);
+        iks[p] = __shfl_sync(0xffffffffu, ks[p], i & 7, 8);
+        ivs[p] = __shfl_sync(0xffffffffu, vs[p], i & 7, 8);
+        bad |= (irow[p] >> 31) << p;
+        if (!(irow[p] & kBad)) bytes += 2 * kPiece * D;
+      }
+      if (go) {
+        if (sl == 0) {
+          UnitMeta& m = my_meta[stage];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            m.ks[p] = iks[p];
+            m.vs[p] = ivs[p];
+          }
+          m.bad = bad;
+          uint8_t* dst = ring + stage * R::kStage;
+          mbar_arrive_expect_tx(&my_full[stage], bytes);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            if (irow[p] & kBad) continue;
+            tma_load_3d(dst + p * kPiece * D, &kmap, &my_full[stage], 0, h, static_cast<int32_t>(irow[p]));
+            tma_load_3d(dst + R::kTile + p * kPiece * D, &vmap, &my_full[stage], 0, h, static_cast<int32_t>(irow[p]));
+          }
+        }
+        ++i;
+        ++fills;
+        if (++stage == NS) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (__any_sync(0xffffffffu, go)) {
+        idle_since = globaltimer_ns();
+      } else if (*abort_s || globaltimer_ns() - idle_since > kWaitLimitNs) {
+        if (!*abort_s && lane == 0) flag_status(a.status, B200_DEVICE_TIMEOUT);
+        break;
       }
     }
-    ++pi;
-    ++flight;
-    if (++pstage == NS) pstage = 0;
-    return true;
-  };
-  while (flight < NS && issue_one()) {
+    // no load may land after the CTA is gone: wait (bounded) for the last fill of each stage
+    for (uint32_t k = 0; k < NS; ++k) {
+      if (stage == 0) phase ^= 1u;
+      stage = stage == 0 ? NS - 1 : stage - 1;
+      if (k < fills) mbar_wait_bounded(&my_full[stage], phase);
+    }
+    return;
   }
 
-  int cstage = 0;          // the ring's next stage to read, and the phase of its barrier
-  uint32_t cphase = 0;
-  // ldmatrix: lane's row of the unit and 16-byte chunk 0 or 1, swizzled; chunk k is at ^ (k << 4)
+  // ======== consumers ==========================================================================
+  const int r = lane >> 2, c = lane & 3;
+  uint8_t* ring = smem + warp * R::kWarpBytes;
+  const uint32_t ring_u32 = base_u32 + warp * R::kWarpBytes;
+  const UnitMeta* my_meta = meta + warp * NS;
+  uint64_t* my_full = full + warp * NS;
+  uint64_t* my_empty = empty + warp * NS;
+  int stage = 0;
+  uint32_t phase = 0;
+  // ldmatrix: lane's row of 16 tokens and 16-byte chunk 0 or 1, swizzled; chunk k is at ^ (k << 4)
   const int krow = (lane & 7) + 8 * ((lane >> 3) & 1);
   const uint32_t lane_at = tile_at<D>(krow, lane >> 4);
 
-  uint32_t qf[KS][2], ql[SPLIT ? KS : 1][2];
-  float acc[KS][4];
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, F0 = kUnset, F1 = kUnset, qscale0 = 0.f, qscale1 = 0.f;
-  int64_t qrow = 0;
-  int nh = 0, hq0 = 0;
-  bool fresh = true;  // the next unit begins an item (for this warp)
-  int64_t pos = begin;
+  for (;;) {
+    int seq, hct, u0;
+    const int n = next_piece(walk, cu, ips, 0x7fffffff, seq, hct, u0);
+    if (n == 0) break;
+    const int hc = hct * ts + warp % ts;
+    const int h = hc / a.nchunks, cch = hc - h * a.nchunks;
+    const int units = cu[seq + 1] - cu[seq] - kItemCost;
+    const int ctx = min(a.ctx_lens[seq], a.max_ctx);
+    const int nh = min(8, a.group - cch * 8);
+    const int hq0 = h * a.group + cch * 8;
+    const int64_t qrow = a.cu_q ? a.cu_q[seq] : (a.query_rows ? a.query_rows[seq] : seq);
 
-  while (cur.n > 0) {
-    if (fresh) {
-      fresh = false;
-      const int cch = cur.hc - cur.h * a.nchunks;
-      nh = min(8, a.group - cch * 8);
-      hq0 = cur.h * a.group + cch * 8;
-      qrow = a.cu_q ? a.cu_q[cur.s] : (a.query_rows ? a.query_rows[cur.s] : cur.s);
+    // ---- Q of head r, scaled to f16; |q| below 2^11: the parts that matter stay normal numbers ----
+    uint32_t qf[KS][2], ql[SPLIT ? KS : 1][2];
+    float qscale0, qscale1;
+    {
       float qv[KS][4];
       float mx = 0.f;
-      const T* q = static_cast<const T*>(a.q) + qrow * a.q_srow + static_cast<int64_t>(hq0 + r) * a.q_shead;
+      const T* q = static_cast<const T*>(a.q) + qrow * a.q_srow + static_cast<int64_t>(hq0 + r) * a.q_shead + 4 * c;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if (a.vec_q) {
+          load4<T>(q + 16 * k, r < nh, qv[k]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) qv[k][j] = r < nh ? to_f32<T>(q[16 * k + j]) : 0.f;
+        }
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          qv[k][j] = r < nh ? to_f32<T>(q[16 * k + 4 * c + j]) : 0.f;
-          mx = fmaxf(mx, fabsf(qv[k][j]));
-        }
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fabsf(qv[k][j]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      // |q| below 2^11 after scaling: the smallest parts that matter stay normal f16 numbers
       const float inv = pow2_inverse(mx, 10);
 #pragma unroll
       for (int k = 0; k < KS; ++k)
@@ -325,48 +461,41 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       const float back = a.scale_log2 / inv;  // head r's; the scores are laid out by 2c, 2c + 1
       qscale0 = __shfl_sync(0xffffffffu, back, 8 * c);
       qscale1 = __shfl_sync(0xffffffffu, back, 8 * c + 4);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0.f;
-      m0 = m1 = -INFINITY;
-      l0 = l1 = 0.f;
-      F0 = F1 = kUnset;
     }
+    float acc[KS][4];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, F0 = kUnset, F1 = kUnset;
 
-    for (int i = 0; i < cur.n; ++i) {
-      if (!mbar_wait_bounded(&my_bars[cstage], cphase)) {
-        // wait (bounded) for every fill in flight, so that none lands after this CTA is gone
+    for (int i = 0; i < n; ++i) {
+      if (!mbar_wait_bounded(&my_full[stage], phase)) {
         if (lane == 0) flag_status(a.status, B200_DEVICE_TIMEOUT);
-        for (int f = 1; f < flight; ++f) {
-          if (++cstage == NS) {
-            cstage = 0;
-            cphase ^= 1u;
-          }
-          mbar_wait_bounded(&my_bars[cstage], cphase);
-        }
+        *abort_s = 1;  // the producer sees to what is in flight
         return;
       }
-      const uint32_t kb = ring_u32 + cstage * R::kStage + lane_at;
+      const uint32_t kb = ring_u32 + stage * R::kStage + lane_at;
       const uint32_t vb = kb + R::kTile;
-      uint32_t bad = 0;
+      const UnitMeta& m = my_meta[stage];
+      const uint32_t bad = m.bad;
       float ks[NP], vs[NP];
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        bad |= (__shfl_sync(0xffffffffu, cur.row[p], i) >> 31) << p;
-        ks[p] = __shfl_sync(0xffffffffu, cur.ks[p], i);
-        vs[p] = __shfl_sync(0xffffffffu, cur.vs[p], i);
+        ks[p] = m.ks[p];
+        vs[p] = m.vs[p];
       }
-      const int valid = cur.ctx - (cur.u0 + i) * kUnit;  // tokens of the unit inside the context
+      const int valid = ctx - (u0 + i) * kUnit;  // tokens of the unit inside the context
       const bool whole = valid >= kUnit && bad == 0;
       // token t of the unit takes part
       const auto takes_part = [&](int t) { return t < valid && !((bad >> (t / kPiece)) & 1u); };
       if (!whole) {
         // rows that do not take part may hold anything, NaN codes among it: their V is zeroed
-        uint8_t* v = ring + cstage * R::kStage + R::kTile;
+        uint8_t* v = ring + stage * R::kStage + R::kTile;
         for (int idx = lane; idx < kUnit * (D / 16); idx += 32) {
           const int rr = idx / (D / 16), ch = idx % (D / 16);
           if (!takes_part(rr))
             *reinterpret_cast<uint4*>(v + tile_at<D>(rr, ch)) = make_uint4(0u, 0u, 0u, 0u);
         }
+        fence_proxy_async_smem();  // before the stage's next fill
         __syncwarp();
       }
 
@@ -518,124 +647,125 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             if (SPLIT) MmaOp<__half>::run(acc[k + 1], a0, a1, a2, a3, pl[j][0], pl[j][1]);
           }
         }
-      --flight;
-      if (++cstage == NS) {
-        cstage = 0;
-        cphase ^= 1u;
-      }
       __syncwarp();
-      if (lane == 0) fence_proxy_async_smem();  // this stage's reads and zeroing before its refill
-      issue_one();
+      if (lane == 0) tc05::mbar_arrive(&my_empty[stage]);
+      if (++stage == NS) {
+        stage = 0;
+        phase ^= 1u;
+      }
     }
 
     // ---- the item's end, or the share's ---------------------------------------------------
-    const int item_end = cur.u0 + cur.n;
-    const bool done = item_end == cur.units;
-    const int64_t seg_end = pos + cur.n;
-    if (done || seg_end == end) {
+    const bool done = u0 + n == units;
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-      }
-      const int64_t item0 = seg_end - item_end;  // the line's unit where this item begins
-      if (done && item0 >= begin) {
-        const float f0 = 1.f / F0, f1 = 1.f / F1;
-        const float i0 = l0 != 0.f ? 1.f / l0 : 0.f, i1 = l1 != 0.f ? 1.f / l1 : 0.f;
-        T* o0 = static_cast<T*>(a.out) + qrow * a.o_srow + static_cast<int64_t>(hq0 + 2 * c) * a.o_shead;
-        T* o1 = o0 + a.o_shead;
+    for (int o = 4; o < 32; o <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+    }
+    const int64_t item0 = walk.at - n - u0;  // the line's place of the item's first unit
+    if (done && item0 >= begin) {
+      const float f0 = 1.f / F0, f1 = 1.f / F1;
+      const float i0 = l0 != 0.f ? 1.f / l0 : 0.f, i1 = l1 != 0.f ? 1.f / l1 : 0.f;
+      T* o0 = static_cast<T*>(a.out) + qrow * a.o_srow + static_cast<int64_t>(hq0 + 2 * c) * a.o_shead;
+      T* o1 = o0 + a.o_shead;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const int d = 16 * k + 2 * r;
-          if (2 * c < nh) {
-            o0[d] = from_f32<T>(acc[k][0] * f0 * i0);
-            o0[d + 1] = from_f32<T>(acc[k][2] * f0 * i0);
-          }
-          if (2 * c + 1 < nh) {
-            o1[d] = from_f32<T>(acc[k][1] * f1 * i1);
-            o1[d + 1] = from_f32<T>(acc[k][3] * f1 * i1);
-          }
+      for (int k = 0; k < KS; ++k) {
+        const int d = 16 * k + 2 * r;
+        if (2 * c < nh) {
+          o0[d] = from_f32<T>(acc[k][0] * f0 * i0);
+          o0[d + 1] = from_f32<T>(acc[k][2] * f0 * i0);
         }
-      } else {
-        // a part of an item: sums relative to 2^m, the output sum as the values' (without F)
-        const int64_t slot = 2 * static_cast<int64_t>(gw) + (item0 <= begin ? 0 : 1);
-        float* po = a.part_o + slot * 8 * D;
-        float2* ml = a.part_ml + slot * 8;
-        const float i0 = 1.f / F0, i1 = 1.f / F1;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const int d = 16 * k + 2 * r;
-          if (2 * c < nh)
-            *reinterpret_cast<float2*>(po + (2 * c) * D + d) = make_float2(acc[k][0] * i0, acc[k][2] * i0);
-          if (2 * c + 1 < nh)
-            *reinterpret_cast<float2*>(po + (2 * c + 1) * D + d) = make_float2(acc[k][1] * i1, acc[k][3] * i1);
-        }
-        if (r == 0) {
-          ml[2 * c] = make_float2(m0, l0);
-          ml[2 * c + 1] = make_float2(m1, l1);
+        if (2 * c + 1 < nh) {
+          o1[d] = from_f32<T>(acc[k][1] * f1 * i1);
+          o1[d + 1] = from_f32<T>(acc[k][3] * f1 * i1);
         }
       }
-      fresh = true;
-    }
-    pos = seg_end;
-    cur = nxt;
-    if (!on_next) {  // everything of the old segment is issued: go on with this one
+    } else {
+      // a part of an item: sums relative to 2^m, the output sum as the values' (without F)
+      const int64_t slot = 2 * static_cast<int64_t>(gw) + (item0 <= begin ? 0 : 1);
+      float* po = a.part_o + slot * 8 * D;
+      float2* ml = a.part_ml + slot * 8;
+      const float i0 = 1.f / F0, i1 = 1.f / F1;
 #pragma unroll
-      for (int p = 0; p < NP; ++p) prow[p] = cur.row[p];
-      ph = cur.h;
-      pn = cur.n;
-      pi = 0;
-    }
-    on_next = false;
-    nxt = load_seg();
-    while (flight < NS && issue_one()) {
+      for (int k = 0; k < KS; ++k) {
+        const int d = 16 * k + 2 * r;
+        if (2 * c < nh)
+          *reinterpret_cast<float2*>(po + (2 * c) * D + d) = make_float2(acc[k][0] * i0, acc[k][2] * i0);
+        if (2 * c + 1 < nh)
+          *reinterpret_cast<float2*>(po + (2 * c + 1) * D + d) = make_float2(acc[k][1] * i1, acc[k][3] * i1);
+      }
+      if (r == 0) {
+        ml[2 * c] = make_float2(m0, l0);
+        ml[2 * c + 1] = make_float2(m1, l1);
+      }
     }
   }
 }
 
-// Joins the parts of items that several warps shared, in the order of the warps, and writes zeros
-// for decoded sequences without context.  One CTA per item.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) merge_fp8_kernel(DecodeFp8Args a, int warps) {
-  __shared__ float4 sum_s[256];
-  __shared__ float2 ml_s[8][32];
-  const int tid = threadIdx.x;
-  const int ips = a.hkv * a.nchunks;
-  const int s = blockIdx.x / ips, hc = blockIdx.x - s * ips;
+// The merge: joins the parts of items that several warps shared, in the order of the warps, and
+// writes zeros for decoded sequences without context.  Launched while the decode still runs; its
+// first statement waits for the decode's results.
+
+// An item as the merge sees it.
+struct MergeItem {
+  int64_t qrow, w0, share, first;  // output row; first warp team, the share, the place of the first unit
+  int n, h0, nh, sub, ts;          // parts (1: the warp wrote the output), query heads, warp in the team
+};
+
+// Item `hc` of sequence s; false where nothing is left to do but zeros (n = 0) or nothing (n = 1).
+__device__ __forceinline__ MergeItem merge_item(const DecodeFp8Args& a, int s, int hc, int warps) {
+  MergeItem it;
+  const int items = a.hkv * a.nchunks;
+  const int begin = a.cu_units[s], length = a.cu_units[s + 1] - begin, all = a.cu_units[a.S];
+  const bool decoded = a.cu_q == nullptr || a.cu_q[s + 1] - a.cu_q[s] == 1;
+  it.qrow = a.cu_q ? a.cu_q[s] : (a.query_rows ? a.query_rows[s] : s);
   const int h = hc / a.nchunks, cch = hc - h * a.nchunks;
-  const int nh = min(8, a.group - cch * 8), hq0 = h * a.group + cch * 8;
-  const int units = a.cu_units[s + 1] - a.cu_units[s];
-  const int64_t qrow = a.cu_q ? a.cu_q[s] : (a.query_rows ? a.query_rows[s] : s);
-  T* out = static_cast<T*>(a.out) + qrow * a.o_srow + static_cast<int64_t>(hq0) * a.o_shead;
-  if (hc == 0 && tid == 0 && a.ctx_lens[s] > a.max_ctx) flag_status(a.status, B200_DEVICE_BAD_OP);
-  if (units == 0) {
-    if (a.cu_q == nullptr || a.cu_q[s + 1] - a.cu_q[s] == 1)
-      for (int i = tid; i < nh * D; i += 256) out[(i / D) * a.o_shead + i % D] = from_f32<T>(0.f);
-    return;
-  }
-  const int ts = team_of(ips);
-  const int64_t total = static_cast<int64_t>(a.cu_units[a.S]) * (ips / ts);
-  const int64_t share = share_of(total, warps / ts);
-  const int64_t first = static_cast<int64_t>(a.cu_units[s]) * (ips / ts) + static_cast<int64_t>(hc / ts) * units;
-  const int64_t w0 = first / share, w1 = (first + units - 1) / share;
-  if (w0 == w1) return;  // written by its one warp
-  const int n = static_cast<int>(w1 - w0) + 1;
-  const auto slot_of = [&](int i) {
-    return 2 * ((w0 + i) * ts + hc % ts) + (i == 0 && first > w0 * share ? 1 : 0);
-  };
-  // every head's largest reference, then each part's weight
-  constexpr int kVec = D / 4;                    // float4s of a head
-  const int lanes = nh * kVec;                   // at most 256
-  const int groups = 256 / lanes > 0 ? 256 / lanes : 1;
-  const int grp = tid / lanes, e = tid - grp * lanes;
-  const int hh = e / kVec;
-  float M = -INFINITY, L = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (grp < groups) {
-    for (int i = grp; i < n; i += groups) {
-      const int64_t sl = slot_of(i);
-      const float2 ml = a.part_ml[sl * 8 + hh];
-      const float4 v = *reinterpret_cast<const float4*>(a.part_o + (sl * 8 + hh) * D + (e % kVec) * 4);
+  it.nh = min(8, a.group - cch * 8);
+  it.h0 = h * a.group + cch * 8;
+  it.ts = team_of(items);
+  it.sub = hc % it.ts;
+  it.n = decoded ? 0 : 1;
+  if (length == 0) return it;
+  const int ips = items / it.ts;
+  it.share = share_of(static_cast<int64_t>(all) * ips, warps / it.ts);
+  const int64_t end = static_cast<int64_t>(begin) * ips + static_cast<int64_t>(hc / it.ts + 1) * length;
+  it.first = end - length + kItemCost;
+  it.w0 = quotient(it.first, it.share);
+  it.n = static_cast<int>(quotient(end - 1, it.share) - it.w0) + 1;
+  return it;
+}
+
+__device__ __forceinline__ int64_t merge_slot(const MergeItem& it, int i) {
+  return 2 * ((it.w0 + i) * it.ts + it.sub) + (i == 0 && it.first > it.w0 * it.share ? 1 : 0);
+}
+
+// Few parts an item: one warp per item.
+constexpr int kMergeWarps = 4;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kMergeWarps) merge_few_kernel(DecodeFp8Args a, int warps) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int items = a.hkv * a.nchunks;
+  const int idx = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+  if (idx >= a.S * items) return;
+  const int s = idx / items, hc = idx - s * items;
+  if (hc == 0 && lane == 0 && a.ctx_lens[s] > a.max_ctx) flag_status(a.status, B200_DEVICE_BAD_OP);
+  const MergeItem it = merge_item(a, s, hc, warps);
+  if (it.n == 1) return;
+  T* out = static_cast<T*>(a.out) + it.qrow * a.o_srow + static_cast<int64_t>(it.h0) * a.o_shead;
+  constexpr int kVec = D / 4, kPer = 32 / kVec;  // float4s of a head, heads at a time
+  const int e = lane % kVec;
+#pragma unroll 4
+  for (int hb = 0; hb < it.nh; hb += kPer) {
+    const int hh = hb + lane / kVec;
+    const bool live = hh < it.nh;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = -INFINITY, L = 0.f;
+    for (int i = 0; i < it.n; ++i) {
+      const int64_t sl = merge_slot(it, i);
+      const float2 ml = live ? a.part_ml[sl * 8 + hh] : make_float2(-INFINITY, 0.f);
+      const float4 v = live ? *reinterpret_cast<const float4*>(a.part_o + (sl * 8 + hh) * D + e * 4) : o;
       const float N = fmaxf(M, ml.x);
       const float Nu = N == -INFINITY ? 0.f : N;
       const float wa = fast_exp2(M - Nu), wb = fast_exp2(ml.x - Nu);
@@ -646,25 +776,108 @@ __global__ void __launch_bounds__(256) merge_fp8_kernel(DecodeFp8Args a, int war
       L = L * wa + ml.y * wb;
       M = N;
     }
-    sum_s[tid] = o;
-    if (e % kVec == 0) ml_s[hh][grp] = make_float2(M, L);
+    if (!live) continue;
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+    T* d = out + static_cast<int64_t>(hh) * a.o_shead + e * 4;
+    d[0] = from_f32<T>(o.x * inv);
+    d[1] = from_f32<T>(o.y * inv);
+    d[2] = from_f32<T>(o.z * inv);
+    d[3] = from_f32<T>(o.w * inv);
   }
+}
+
+// Many parts an item: one CTA per item.
+constexpr int kMergeThreads = 512;
+constexpr int kMergeParts = 128;  // parts joined per pass
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeThreads) merge_many_kernel(DecodeFp8Args a, int warps) {
+  __shared__ float4 sum_s[kMergeThreads];
+  __shared__ float wt[8][kMergeParts];
+  __shared__ float m_s[8], l_s[8], al_s[8];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int items = a.hkv * a.nchunks;
+  const int s = blockIdx.x / items, hc = blockIdx.x - s * items;
+  if (hc == 0 && tid == 0 && a.ctx_lens[s] > a.max_ctx) flag_status(a.status, B200_DEVICE_BAD_OP);
+  const MergeItem it = merge_item(a, s, hc, warps);
+  const int n = it.n, nh = it.nh;
+  if (n == 1) return;
+  T* out = static_cast<T*>(a.out) + it.qrow * a.o_srow + static_cast<int64_t>(it.h0) * a.o_shead;
+  if (n == 0) {
+    for (int i = tid; i < nh * D; i += kMergeThreads) out[(i / D) * a.o_shead + i % D] = from_f32<T>(0.f);
+    return;
+  }
+  constexpr int kVec = D / 4;       // float4s of a head
+  const int lanes = nh * kVec;
+  const int groups = kMergeThreads / lanes;
+  const int grp = tid / lanes, e = tid - grp * lanes;
+  const int hh = e / kVec;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < n; p0 += kMergeParts) {
+    const int np = min(kMergeParts, n - p0);
+    for (int w8 = warp; w8 < nh; w8 += kMergeThreads / 32) {
+      // head w8's reference, the parts' weights, the sum of p
+      float mine[kMergeParts / 32], l[kMergeParts / 32];
+      float M = p0 == 0 ? -INFINITY : m_s[w8];
+      const float M_old = M;
+#pragma unroll
+      for (int j = 0; j < kMergeParts / 32; ++j) {
+        const int i = lane + 32 * j;
+        const float2 ml = i < np ? a.part_ml[merge_slot(it, p0 + i) * 8 + w8] : make_float2(-INFINITY, 0.f);
+        mine[j] = ml.x;
+        l[j] = ml.y;
+        M = fmaxf(M, ml.x);
+      }
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+      const float Mu = M == -INFINITY ? 0.f : M;
+      float L = 0.f;
+#pragma unroll
+      for (int j = 0; j < kMergeParts / 32; ++j) {
+        const float w = fast_exp2(mine[j] - Mu);
+        wt[w8][lane + 32 * j] = w;
+        L += w * l[j];
+      }
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+      if (lane == 0) {
+        const float al = fast_exp2(M_old - Mu);
+        m_s[w8] = M;
+        al_s[w8] = al;
+        l_s[w8] = (p0 == 0 ? 0.f : l_s[w8] * al) + L;
+      }
+    }
+    __syncthreads();
+    if (grp < groups) {
+      const float al = p0 == 0 ? 0.f : al_s[hh];
+      o.x *= al;
+      o.y *= al;
+      o.z *= al;
+      o.w *= al;
+#pragma unroll 4
+      for (int i = grp; i < np; i += groups) {
+        const float4 v = *reinterpret_cast<const float4*>(a.part_o + (merge_slot(it, p0 + i) * 8 + hh) * D + (e % kVec) * 4);
+        const float w = wt[hh][i];
+        o.x = fmaf(v.x, w, o.x);
+        o.y = fmaf(v.y, w, o.y);
+        o.z = fmaf(v.z, w, o.z);
+        o.w = fmaf(v.w, w, o.w);
+      }
+    }
+    __syncthreads();
+  }
+  sum_s[tid] = o;
   __syncthreads();
   if (grp == 0) {
     for (int g = 1; g < groups; ++g) {
-      const float2 ml = ml_s[hh][g];
       const float4 v = sum_s[g * lanes + e];
-      const float N = fmaxf(M, ml.x);
-      const float Nu = N == -INFINITY ? 0.f : N;
-      const float wa = fast_exp2(M - Nu), wb = fast_exp2(ml.x - Nu);
-      o.x = o.x * wa + v.x * wb;
-      o.y = o.y * wa + v.y * wb;
-      o.z = o.z * wa + v.z * wb;
-      o.w = o.w * wa + v.w * wb;
-      L = L * wa + ml.y * wb;
-      M = N;
+      o.x += v.x;
+      o.y += v.y;
+      o.z += v.z;
+      o.w += v.w;
     }
-    const float inv = L != 0.f ? 1.f / L : 0.f;
+    const float inv = l_s[hh] != 0.f ? 1.f / l_s[hh] : 0.f;
     T* d = out + static_cast<int64_t>(hh) * a.o_shead + (e % kVec) * 4;
     d[0] = from_f32<T>(o.x * inv);
     d[1] = from_f32<T>(o.y * inv);
@@ -676,7 +889,8 @@ __global__ void __launch_bounds__(256) merge_fp8_kernel(DecodeFp8Args a, int war
 template <int D>
 int smem_bytes(int S) {
   using R = Ring<D>;
-  return 1024 + kWarps * R::kWarpBytes + kWarps * R::kStages * 8 + kWarps * 4 + (S + 1) * 4;
+  return 1024 + kWarps * R::kWarpBytes + kWarps * R::kStages * (sizeof(UnitMeta) + 16) + (kWarps + 2) * 4 +
+         (S + 1) * 4;
 }
 
 template <typename T, int D, int NP, bool SPLIT>
@@ -689,8 +903,25 @@ cudaError_t launch_t(const CUtensorMap& km, const CUtensorMap& vm, const DecodeF
   kern<<<grid, kThreads, smem, stream>>>(km, vm, a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  merge_fp8_kernel<T, D><<<a.S * a.hkv * a.nchunks, 256, 0, stream>>>(a, grid * kWarps);
-  return cudaGetLastError();
+  // the merge's launch overlaps the decode's end
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  const int items = a.hkv * a.nchunks;
+  // the parts of an item, on average: a warp joins few of them while a CTA would still start up
+  const int64_t parts = static_cast<int64_t>(grid) * kWarps / (static_cast<int64_t>(a.S) * items) + 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (parts > 6) {
+    cfg.gridDim = dim3(a.S * items);
+    cfg.blockDim = dim3(kMergeThreads);
+    return cudaLaunchKernelEx(&cfg, merge_many_kernel<T, D>, a, grid * kWarps);
+  }
+  cfg.gridDim = dim3((a.S * items + kMergeWarps - 1) / kMergeWarps);
+  cfg.blockDim = dim3(32 * kMergeWarps);
+  return cudaLaunchKernelEx(&cfg, merge_few_kernel<T, D>, a, grid * kWarps);
 }
 
 template <typename T, bool SPLIT>
@@ -706,8 +937,8 @@ cudaError_t launch_d(const CUtensorMap& km, const CUtensorMap& vm, const DecodeF
 }  // namespace
 
 int decode_fp8_grid(int S, int64_t max_ctx, int ips, int num_sms) {
-  const int64_t units = static_cast<int64_t>(S) * ((max_ctx + kUnit - 1) / kUnit) * ips;
-  const int64_t need = (units + kMinShare * kWarps - 1) / (kMinShare * kWarps);
+  const int64_t line = static_cast<int64_t>(S) * ((max_ctx + kUnit - 1) / kUnit + kItemCost) * ips;
+  const int64_t need = (line + kMinShare * kWarps - 1) / (kMinShare * kWarps);
   const int64_t most = static_cast<int64_t>(num_sms) * kCtasPerSm;
   return static_cast<int>(need < 1 ? 1 : need < most ? need : most);
 }

@@ -10,6 +10,7 @@ constexpr int kDecodeFp8MaxSeqs = 1024;  // sequences of one launch (their unit 
 struct DecodeFp8Args {
   const void* q;
   int64_t q_srow, q_shead;
+  int32_t vec_q;  // query rows and heads are aligned to four elements
   const int32_t* query_rows;
   const int64_t* cu_q;  // mixed batch: only sequences with exactly one new token, row cu_q[s]
   const float* ks;
