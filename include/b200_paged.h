@@ -468,8 +468,14 @@ int b200_paged_decode_fp8(const B200AttentionFp8Params* p, void* workspace,
 
 size_t b200_paged_prefill_fp8_workspace_bytes(const B200AttentionFp8Params* p);
 
-/* b200_paged_prefill over an 8-bit cache.  Rows of query behind the last sequence are left as
- * they are in out. */
+/* b200_paged_prefill over an 8-bit cache.  bf16 and f16 queries whose shapes the tensor-core prefill
+ * covers run on it, over a 16-bit copy of the pages that the sequences with more than one new token
+ * hold (exact for bf16 with power-of-two scales; f16 values beyond its range become +-65504); the
+ * copy takes 4 bytes per cached entry of prefill_blocks blocks in the workspace.  If those
+ * sequences hold more blocks than prefill_blocks, B200_DEVICE_BAD_STEP is set and the rows of the
+ * ones that do not fit are not meaningful.  A page outside the pool sets B200_DEVICE_BAD_BLOCK; the
+ * rows of a sequence with such a page are not meaningful, the others are not touched by it.  Rows
+ * of query behind the last sequence are left as they are in out. */
 int b200_paged_prefill_fp8(const B200AttentionFp8Params* p, void* workspace,
                            size_t workspace_bytes, void* stream);
 

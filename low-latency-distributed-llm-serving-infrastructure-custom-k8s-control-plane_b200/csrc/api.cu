@@ -480,7 +480,8 @@ static B200DecodeParams decode_leg(const B200PrefillParams& p) {
   return d;
 }
 
-static PrefillPlan make_prefill_plan(const B200PrefillParams& p) {
+// chunks_only: sequences with one new token are left out (someone else decodes them).
+static PrefillPlan make_prefill_plan(const B200PrefillParams& p, bool chunks_only = false) {
   PrefillPlan pl{};
   const int G = p.num_query_heads / p.geom.num_kv_heads;
   const int es = esize_of(p.geom.dtype);
@@ -495,9 +496,11 @@ static PrefillPlan make_prefill_plan(const B200PrefillParams& p) {
                             p.geom.block_size < (int64_t(1) << 31);
   pl.tq = G > 0 ? 128 / G : 128;
   pl.max_work = static_cast<int64_t>(p.num_tokens) / (pl.tq > 0 ? pl.tq : 1) + p.num_seqs;
-  const DecodePlan dpl = make_decode_plan(decode_leg(p));
-  pl.split_decodes = pl.tensor_cores && dpl.tensor_cores;
-  pl.decode_bytes = pl.split_decodes ? align256(dpl.total) : 0;
+  if (!chunks_only) {
+    const DecodePlan dpl = make_decode_plan(decode_leg(p));
+    pl.split_decodes = pl.tensor_cores && dpl.tensor_cores;
+    pl.decode_bytes = pl.split_decodes ? align256(dpl.total) : 0;
+  }
   pl.off_hdr = pl.decode_bytes;
   pl.off_work = pl.off_hdr + align256(sizeof(b200::PrefillHeader));
   pl.total = pl.tensor_cores ? pl.off_work + align256(pl.max_work * sizeof(int2)) : 0;
@@ -525,6 +528,88 @@ static int query_tensor_map(const void* q, int64_t stride_tok, int64_t stride_he
   return B200_OK;
 }
 
+// The tensor-core prefill of a planned batch (and the decode of its one-token sequences, where the
+// plan splits them off).
+static int run_prefill_tc(const B200PrefillParams& p, const PrefillPlan& pl, bool chunks_only,
+                          void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  const int G = p.num_query_heads / p.geom.num_kv_heads;
+  if (workspace == nullptr || workspace_bytes < pl.total)
+    return fail(B200_ERR_INVALID_ARGUMENT, "prefill workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "prefill workspace must be 256-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  if (pl.split_decodes) {
+    int rc = run_decode(decode_leg(p), p.cu_seqlens, ws, pl.decode_bytes, st);
+    if (rc != B200_OK) return rc;
+  }
+  auto* hdr = reinterpret_cast<b200::PrefillHeader*>(ws + pl.off_hdr);
+  auto* work = reinterpret_cast<int2*>(ws + pl.off_work);
+  CUtensorMap qm, km, vm;
+  int rc = query_tensor_map(p.query, p.q_stride_token, p.q_stride_head, p.num_query_heads,
+                        p.num_tokens, p.geom.head_dim, p.geom.dtype, pl.tq, &qm);
+  if (rc != B200_OK) return rc;
+  rc = cache_tensor_map(p.key_cache, p.geom, 16, &km);
+  if (rc != B200_OK) return rc;
+  rc = cache_tensor_map(p.value_cache, p.geom, 16, &vm);
+  if (rc != B200_OK) return rc;
+  // 0: one query tile per item (prefill.cu); 1: two tiles per item (prefill_q2.cu), which
+  // takes query tiles in pairs (the work list, sized for single tiles, holds the pairs as
+  // well); 2: two independent streams per CTA (prefill_ds.cu)
+  const int kernel = g_prefill_kernel.load(std::memory_order_relaxed);
+  const bool two_tiles = kernel == 1;
+  b200::PrefillPlanArgs pa{};
+  pa.cu_q = p.cu_seqlens;
+  pa.ctx_lens = p.context_lens;
+  pa.skip_single = pl.split_decodes || chunks_only ? 1 : 0;
+  pa.S = p.num_seqs;
+  pa.tq = two_tiles ? 2 * pl.tq : pl.tq;
+  pa.hkv = p.geom.num_kv_heads;
+  pa.max_work = static_cast<int32_t>(pl.max_work);
+  pa.status = p.status_word;
+  pa.hdr = hdr;
+  pa.work = work;
+  cudaError_t e = b200::launch_prefill_plan(pa, st);
+  if (e != cudaSuccess) return cuda_fail(e, "prefill plan");
+  b200::PrefillArgs a{};
+  a.layer = p.layer_idx;
+  a.nb = p.geom.total_blocks;
+  a.bs = p.geom.block_size;
+  a.hkv = p.geom.num_kv_heads;
+  a.hq = p.num_query_heads;
+  a.group = G;
+  a.tq = pl.tq;
+  a.bt = p.block_tables;
+  a.bt_stride = p.block_table_stride;
+  a.cu_q = p.cu_seqlens;
+  a.ctx_lens = p.context_lens;
+  a.S = p.num_seqs;
+  a.scale_log2 = p.scale * b200::kLog2e;
+  a.out = p.out;
+  a.o_stok = p.o_stride_token;
+  a.o_shead = p.o_stride_head;
+  a.vec_out = (reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.o_stride_token % 8 == 0 &&
+               p.o_stride_head % 8 == 0)
+                  ? 1
+                  : 0;
+  a.status = p.status_word;
+  a.hdr = hdr;
+  a.work = work;
+  const int64_t max_items = pl.max_work * p.geom.num_kv_heads;
+  const int items = static_cast<int>(max_items < (1 << 30) ? max_items : (1 << 30));
+  const int poly = g_prefill_poly_exp.load(std::memory_order_relaxed);
+  if (kernel == 2)
+    e = b200::launch_prefill_ds(p.geom.dtype, p.geom.head_dim, qm, km, vm, a, items, num_sms(),
+                                poly, st);
+  else if (two_tiles)
+    e = b200::launch_prefill_q2(p.geom.dtype, p.geom.head_dim, qm, km, vm, a, items, num_sms(),
+                                poly, st);
+  else
+    e = b200::launch_prefill_tc(p.geom.dtype, p.geom.head_dim, qm, km, vm, a, items, num_sms(),
+                                st);
+  if (e != cudaSuccess) return cuda_fail(e, "prefill");
+  return B200_OK;
+}
+
 size_t b200_paged_prefill_workspace_bytes(const B200PrefillParams* p) {
   if (p == nullptr || p->num_seqs <= 0 || p->geom.num_kv_heads <= 0 ||
       p->num_query_heads % p->geom.num_kv_heads != 0)
@@ -545,83 +630,8 @@ int b200_paged_prefill(const B200PrefillParams* pp, void* workspace, size_t work
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int G = p.num_query_heads / p.geom.num_kv_heads;
   const PrefillPlan pl = make_prefill_plan(p);
-  if (pl.tensor_cores && !g_force_cuda_core_prefill.load(std::memory_order_relaxed)) {
-    if (workspace == nullptr || workspace_bytes < pl.total)
-      return fail(B200_ERR_INVALID_ARGUMENT, "prefill workspace too small");
-    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
-      return fail(B200_ERR_INVALID_ARGUMENT, "prefill workspace must be 256-byte aligned");
-    char* ws = static_cast<char*>(workspace);
-    if (pl.split_decodes) {
-      rc = run_decode(decode_leg(p), p.cu_seqlens, ws, pl.decode_bytes, st);
-      if (rc != B200_OK) return rc;
-    }
-    auto* hdr = reinterpret_cast<b200::PrefillHeader*>(ws + pl.off_hdr);
-    auto* work = reinterpret_cast<int2*>(ws + pl.off_work);
-    CUtensorMap qm, km, vm;
-    rc = query_tensor_map(p.query, p.q_stride_token, p.q_stride_head, p.num_query_heads,
-                          p.num_tokens, p.geom.head_dim, p.geom.dtype, pl.tq, &qm);
-    if (rc != B200_OK) return rc;
-    rc = cache_tensor_map(p.key_cache, p.geom, 16, &km);
-    if (rc != B200_OK) return rc;
-    rc = cache_tensor_map(p.value_cache, p.geom, 16, &vm);
-    if (rc != B200_OK) return rc;
-    // 0: one query tile per item (prefill.cu); 1: two tiles per item (prefill_q2.cu), which
-    // takes query tiles in pairs (the work list, sized for single tiles, holds the pairs as
-    // well); 2: two independent streams per CTA (prefill_ds.cu)
-    const int kernel = g_prefill_kernel.load(std::memory_order_relaxed);
-    const bool two_tiles = kernel == 1;
-    b200::PrefillPlanArgs pa{};
-    pa.cu_q = p.cu_seqlens;
-    pa.ctx_lens = p.context_lens;
-    pa.skip_single = pl.split_decodes ? 1 : 0;
-    pa.S = p.num_seqs;
-    pa.tq = two_tiles ? 2 * pl.tq : pl.tq;
-    pa.hkv = p.geom.num_kv_heads;
-    pa.max_work = static_cast<int32_t>(pl.max_work);
-    pa.status = p.status_word;
-    pa.hdr = hdr;
-    pa.work = work;
-    cudaError_t e = b200::launch_prefill_plan(pa, st);
-    if (e != cudaSuccess) return cuda_fail(e, "prefill plan");
-    b200::PrefillArgs a{};
-    a.layer = p.layer_idx;
-    a.nb = p.geom.total_blocks;
-    a.bs = p.geom.block_size;
-    a.hkv = p.geom.num_kv_heads;
-    a.hq = p.num_query_heads;
-    a.group = G;
-    a.tq = pl.tq;
-    a.bt = p.block_tables;
-    a.bt_stride = p.block_table_stride;
-    a.cu_q = p.cu_seqlens;
-    a.ctx_lens = p.context_lens;
-    a.S = p.num_seqs;
-    a.scale_log2 = p.scale * b200::kLog2e;
-    a.out = p.out;
-    a.o_stok = p.o_stride_token;
-    a.o_shead = p.o_stride_head;
-    a.vec_out = (reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.o_stride_token % 8 == 0 &&
-                 p.o_stride_head % 8 == 0)
-                    ? 1
-                    : 0;
-    a.status = p.status_word;
-    a.hdr = hdr;
-    a.work = work;
-    const int64_t max_items = pl.max_work * p.geom.num_kv_heads;
-    const int items = static_cast<int>(max_items < (1 << 30) ? max_items : (1 << 30));
-    const int poly = g_prefill_poly_exp.load(std::memory_order_relaxed);
-    if (kernel == 2)
-      e = b200::launch_prefill_ds(p.geom.dtype, p.geom.head_dim, qm, km, vm, a, items, num_sms(),
-                                  poly, st);
-    else if (two_tiles)
-      e = b200::launch_prefill_q2(p.geom.dtype, p.geom.head_dim, qm, km, vm, a, items, num_sms(),
-                                  poly, st);
-    else
-      e = b200::launch_prefill_tc(p.geom.dtype, p.geom.head_dim, qm, km, vm, a, items, num_sms(),
-                                  st);
-    if (e != cudaSuccess) return cuda_fail(e, "prefill");
-    return B200_OK;
-  }
+  if (pl.tensor_cores && !g_force_cuda_core_prefill.load(std::memory_order_relaxed))
+    return run_prefill_tc(p, pl, false, workspace, workspace_bytes, st);
   b200::RowArgs a{};
   a.mode = b200::kRowBlockTable;
   a.q = p.query;
@@ -650,6 +660,23 @@ int b200_paged_prefill(const B200PrefillParams* pp, void* workspace, size_t work
   if (e != cudaSuccess) return cuda_fail(e, "paged_prefill(row)");
   return B200_OK;
 }
+
+}  // extern "C"
+
+namespace b200 {
+
+size_t prefill_chunks_workspace_bytes(const B200PrefillParams& p) {
+  return make_prefill_plan(p, true).total;
+}
+
+int prefill_chunks(const B200PrefillParams& p, void* workspace, size_t workspace_bytes,
+                   cudaStream_t st) {
+  return run_prefill_tc(p, make_prefill_plan(p, true), true, workspace, workspace_bytes, st);
+}
+
+}  // namespace b200
+
+extern "C" {
 
 void b200_set_prefill_poly_exp(int32_t mode) {
   g_prefill_poly_exp.store(mode < 0 || mode > 2 ? 1 : mode, std::memory_order_relaxed);

@@ -19,4 +19,10 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn encode_fn();
 
+// The tensor-core prefill over a 16-bit cache for the sequences with more than one new token only.
+// The workspace size is 0 for parameters that it does not cover.
+size_t prefill_chunks_workspace_bytes(const B200PrefillParams& p);
+int prefill_chunks(const B200PrefillParams& p, void* workspace, size_t workspace_bytes,
+                   cudaStream_t st);
+
 }  // namespace b200

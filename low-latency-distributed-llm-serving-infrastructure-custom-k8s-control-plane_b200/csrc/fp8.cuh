@@ -83,6 +83,30 @@ struct AttnFp8Args {
 
 cudaError_t launch_row_fp8(const AttnFp8Args& a, int dtype, int rows, cudaStream_t stream);
 
+// Copy of the pages of the sequences with more than one new token in 16 bits, for the tensor-core
+// prefill: a cache (1, scratch_blocks, BS, Hkv, D) with its block table and clamped lengths.
+struct ExpandFp8Args {
+  const uint8_t* kc;
+  const uint8_t* vc;
+  const float* ks;
+  const float* vs;
+  int32_t layer, nb, bs, hkv, head_dim;
+  const int32_t* bt;
+  int32_t bt_stride;
+  const int32_t* ctx_lens;
+  const int64_t* cu_q;
+  int32_t S, max_ctx;
+  int32_t scratch_blocks, scratch_stride;
+  int32_t* offsets;        // (S + 1): first scratch block of each sequence
+  int32_t* scratch_ctx;    // (S)
+  int32_t* scratch_table;  // (S, scratch_stride)
+  void* k16;
+  void* v16;
+  int32_t* status;
+};
+
+cudaError_t launch_expand_fp8(const ExpandFp8Args& a, int dtype, int num_sms, cudaStream_t stream);
+
 // One e4m3 code as fp32 (exact).
 __device__ __forceinline__ float e4m3_to_f32(uint8_t c) {
   const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);

@@ -210,6 +210,111 @@ int check_workspace(const void* ws, size_t have, size_t need) {
   return B200_OK;
 }
 
+// A prefill on the tensor cores: the decode's workspace, the 16-bit copy of the pages of the
+// sequences with more than one new token, and the 16-bit prefill's own workspace.
+struct PrefillPlan {
+  bool tensor_cores;
+  DecodePlan decode;
+  int32_t blocks, stride, max_ctx;
+  size_t off_offsets, off_ctx, off_table, off_chunks, chunk_bytes, off_k, off_v, total;
+};
+
+// The 16-bit prefill's parameters over the copy at `ws`.
+B200PrefillParams chunk_params(const B200AttentionFp8Params& p, const PrefillPlan& pl, char* ws) {
+  B200PrefillParams c{};
+  c.query = p.query;
+  c.q_stride_token = p.q_stride_row;
+  c.q_stride_head = p.q_stride_head;
+  c.key_cache = ws + pl.off_k;
+  c.value_cache = ws + pl.off_v;
+  c.geom = {1, pl.blocks, p.cache.block_size, p.cache.num_kv_heads, p.cache.head_dim, p.dtype};
+  c.layer_idx = 0;
+  c.num_query_heads = p.num_query_heads;
+  c.block_tables = reinterpret_cast<int32_t*>(ws + pl.off_table);
+  c.block_table_stride = pl.stride;
+  c.cu_seqlens = p.cu_seqlens;
+  c.context_lens = reinterpret_cast<int32_t*>(ws + pl.off_ctx);
+  c.num_seqs = p.num_seqs;
+  c.num_tokens = p.num_tokens;
+  c.max_query_len = p.max_query_len;
+  c.max_context_len = pl.max_ctx;
+  c.scale = p.scale;
+  c.out = p.out;
+  c.o_stride_token = p.o_stride_row;
+  c.o_stride_head = p.o_stride_head;
+  c.status_word = p.status_word;
+  return c;
+}
+
+PrefillPlan prefill_plan(const B200AttentionFp8Params& p) {
+  PrefillPlan pl{};
+  pl.decode = decode_plan(p);
+  const B200Fp8Cache& c = p.cache;
+  if (!pl.decode.tensor_cores || p.dtype == B200_DTYPE_F32) return pl;
+  pl.max_ctx = static_cast<int32_t>(pl.decode.max_ctx);
+  pl.stride = (pl.max_ctx + c.block_size - 1) / c.block_size;
+  if (pl.stride < 1) pl.stride = 1;
+  // at most half of the new tokens begin a sequence with more than one
+  const int64_t seqs = p.num_seqs < p.num_tokens / 2 ? p.num_seqs : p.num_tokens / 2;
+  int64_t blocks = seqs * pl.stride;
+  if (p.prefill_blocks >= 0 && p.prefill_blocks < blocks) blocks = p.prefill_blocks;
+  const int64_t block_bytes = static_cast<int64_t>(c.block_size) * c.num_kv_heads * c.head_dim * 2;
+  if (blocks > (int64_t(1) << 31) / c.block_size - 1) return pl;  // rows of the copy pass 31 bits
+  pl.blocks = blocks < 1 ? 1 : static_cast<int32_t>(blocks);
+  pl.chunk_bytes = b200::prefill_chunks_workspace_bytes(chunk_params(p, pl, nullptr));
+  if (pl.chunk_bytes == 0) return pl;
+  pl.tensor_cores = true;
+  size_t off = align256(pl.decode.total);
+  const auto take = [&off](size_t bytes) {
+    const size_t at = off;
+    off += align256(bytes);
+    return at;
+  };
+  pl.off_offsets = take((static_cast<size_t>(p.num_seqs) + 1) * 4);
+  pl.off_ctx = take(static_cast<size_t>(p.num_seqs) * 4);
+  pl.off_table = take(static_cast<size_t>(p.num_seqs) * pl.stride * 4);
+  pl.off_chunks = take(pl.chunk_bytes);
+  pl.off_k = take(static_cast<size_t>(pl.blocks) * block_bytes);
+  pl.off_v = take(static_cast<size_t>(pl.blocks) * block_bytes);
+  pl.total = off;
+  return pl;
+}
+
+// Decode of the one-token sequences, the copy, and the prefill of the others over it.  Copying
+// costs 3 bytes of traffic per cached entry once, against 4 G D flops per entry and new token.
+int run_prefill(const B200AttentionFp8Params& p, const PrefillPlan& pl, char* ws, cudaStream_t st) {
+  int rc = run_decode(p, pl.decode, p.cu_seqlens, ws, st);
+  if (rc != B200_OK || p.num_tokens < 2 || p.max_query_len < 2 || p.prefill_blocks == 0) return rc;
+  const B200Fp8Cache& c = p.cache;
+  b200::ExpandFp8Args a{};
+  a.kc = static_cast<const uint8_t*>(c.key_cache);
+  a.vc = static_cast<const uint8_t*>(c.value_cache);
+  a.ks = c.key_scale;
+  a.vs = c.value_scale;
+  a.layer = c.layer_idx;
+  a.nb = c.total_blocks;
+  a.bs = c.block_size;
+  a.hkv = c.num_kv_heads;
+  a.head_dim = c.head_dim;
+  a.bt = p.block_tables;
+  a.bt_stride = p.block_table_stride;
+  a.ctx_lens = p.context_lens;
+  a.cu_q = p.cu_seqlens;
+  a.S = p.num_seqs;
+  a.max_ctx = pl.max_ctx;
+  a.scratch_blocks = pl.blocks;
+  a.scratch_stride = pl.stride;
+  a.offsets = reinterpret_cast<int32_t*>(ws + pl.off_offsets);
+  a.scratch_ctx = reinterpret_cast<int32_t*>(ws + pl.off_ctx);
+  a.scratch_table = reinterpret_cast<int32_t*>(ws + pl.off_table);
+  a.k16 = ws + pl.off_k;
+  a.v16 = ws + pl.off_v;
+  a.status = p.status_word;
+  const cudaError_t e = b200::launch_expand_fp8(a, p.dtype, num_sms(), st);
+  if (e != cudaSuccess) return cuda_fail(e, "prefill_fp8 copy");
+  return b200::prefill_chunks(chunk_params(p, pl, ws), ws + pl.off_chunks, pl.chunk_bytes, st);
+}
+
 bool has_arrays(const B200AttentionFp8Params& p) {
   return has_arrays(p.cache) && p.query && p.out && p.block_tables && p.context_lens;
 }
@@ -351,23 +456,27 @@ int b200_paged_decode_fp8(const B200AttentionFp8Params* p, void* workspace,
 }
 
 size_t b200_paged_prefill_fp8_workspace_bytes(const B200AttentionFp8Params* p) {
-  (void)p;
-  return 0;
+  if (check_attention(p) != B200_OK || p->num_seqs == 0 || p->num_tokens == 0) return 0;
+  return prefill_plan(*p).total;
 }
 
 int b200_paged_prefill_fp8(const B200AttentionFp8Params* p, void* workspace,
                            size_t workspace_bytes, void* stream) {
   b200::NvtxRange nvtx_range("b200_paged_prefill_fp8");
-  (void)workspace;
-  (void)workspace_bytes;
-  const int rc = check_attention(p);
+  int rc = check_attention(p);
   if (rc != B200_OK) return rc;
   if (p->num_seqs == 0 || p->num_tokens == 0) return B200_OK;
   if (!has_arrays(*p) || !p->cu_seqlens) return fail(B200_ERR_INVALID_ARGUMENT, "null pointer");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const PrefillPlan pl = prefill_plan(*p);
+  if (pl.tensor_cores) {
+    rc = check_workspace(workspace, workspace_bytes, pl.total);
+    if (rc != B200_OK) return rc;
+    return run_prefill(*p, pl, static_cast<char*>(workspace), st);
+  }
   b200::AttnFp8Args a = attention_args(*p);
   a.cu_q = p->cu_seqlens;
-  cudaError_t e =
-      b200::launch_row_fp8(a, p->dtype, p->num_tokens, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = b200::launch_row_fp8(a, p->dtype, p->num_tokens, st);
   if (e != cudaSuccess) return cuda_fail(e, "paged_prefill_fp8");
   return B200_OK;
 }

@@ -1,5 +1,8 @@
 // Attention over an 8-bit paged cache:  o = sum_j softmax_j(scale * q.k_j) v_j  with
 // k_j = code * key scale of the block, v_j = code * value scale of the block.
+#include <type_traits>
+
+#include "cache_ops.cuh"
 #include "fp8.cuh"
 
 namespace b200 {
@@ -146,7 +149,121 @@ cudaError_t launch_row_t(const AttnFp8Args& a, int rows, cudaStream_t stream) {
   return cudaErrorInvalidValue;
 }
 
+// ---- the 16-bit copy of a prefill's pages -----------------------------------------------------
+
+// Scratch blocks of each sequence with more than one new token: one CTA.
+__global__ void __launch_bounds__(1024) expand_plan_kernel(ExpandFp8Args a) {
+  __shared__ int64_t warp_buf[32];
+  __shared__ int64_t total;
+  int64_t carry = 0;
+  for (int base = 0; base < a.S; base += 1024) {
+    const int s = base + threadIdx.x;
+    int64_t n = 0;
+    if (s < a.S) {
+      int32_t ctx = a.ctx_lens[s];
+      if (ctx > a.max_ctx) {
+        flag_status(a.status, B200_DEVICE_BAD_OP);
+        ctx = a.max_ctx;
+      }
+      a.scratch_ctx[s] = ctx;
+      if (a.cu_q[s + 1] - a.cu_q[s] > 1 && ctx > 0) n = (ctx + a.bs - 1) / a.bs;
+    }
+    const int64_t before = block_exclusive_scan_1024(n, warp_buf, &total) + carry;
+    if (s < a.S) a.offsets[s] = static_cast<int32_t>(before < a.scratch_blocks ? before : a.scratch_blocks);
+    carry += total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    if (carry > a.scratch_blocks) flag_status(a.status, B200_DEVICE_BAD_STEP);
+    a.offsets[a.S] = static_cast<int32_t>(carry < a.scratch_blocks ? carry : a.scratch_blocks);
+  }
+}
+
+// 16 codes at scale s in 16 bits: exact for bf16 with power-of-two scales; f16 values beyond its
+// range become +-65504.
+template <typename T>
+__device__ __forceinline__ void widen16(uint4 c, float s, uint4 (&out)[2]) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w[i >> 1] >> (16 * (i & 1))) & 0xffffu), __NV_E4M3);
+    const float2 f = __half22float2(__half2(h));
+    float x = f.x * s, y = f.y * s;
+    if (std::is_same<T, __half>::value) {
+      x = fabsf(x) > 65504.f ? copysignf(65504.f, x) : x;
+      y = fabsf(y) > 65504.f ? copysignf(65504.f, y) : y;
+    }
+    o[i] = MmaOp<T>::pack(x, y);
+  }
+  out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+  out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// Each CTA copies an equal share of the scratch blocks, 16 codes per thread and step.  Bound by
+// memory: 1 byte read and 2 written per entry.
+template <typename T>
+__global__ void __launch_bounds__(256) expand_kernel(ExpandFp8Args a) {
+  const int total = a.offsets[a.S];
+  const int per = (total + gridDim.x - 1) / gridDim.x;
+  const int b0 = blockIdx.x * per, b1 = min(total, b0 + per);
+  if (b0 >= b1) return;
+  int lo = 0, hi = a.S - 1;  // the sequence of b0: the last one that begins at or before it
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.offsets[mid] <= b0) lo = mid; else hi = mid - 1;
+  }
+  int seq = lo;
+  const int64_t block_bytes = static_cast<int64_t>(a.bs) * a.hkv * a.head_dim;
+  const int chunks = static_cast<int>(block_bytes / 16);
+  const int head_chunks = a.head_dim / 16;
+  for (int b = b0; b < b1; ++b) {
+    while (a.offsets[seq + 1] <= b) ++seq;
+    const int j = b - a.offsets[seq];
+    int32_t src = a.bt[static_cast<int64_t>(seq) * a.bt_stride + j];
+    const bool good = src >= 0 && src < a.nb;
+    if (threadIdx.x == 0) {
+      a.scratch_table[static_cast<int64_t>(seq) * a.scratch_stride + j] = b;
+      if (!good) flag_status(a.status, B200_DEVICE_BAD_BLOCK);
+    }
+    if (!good) src = 0;
+    const int64_t at = static_cast<int64_t>(a.layer) * a.nb + src;
+    const uint4* k = reinterpret_cast<const uint4*>(a.kc + at * block_bytes);
+    const uint4* v = reinterpret_cast<const uint4*>(a.vc + at * block_bytes);
+    uint4* ko = static_cast<uint4*>(a.k16) + static_cast<int64_t>(b) * chunks * 2;
+    uint4* vo = static_cast<uint4*>(a.v16) + static_cast<int64_t>(b) * chunks * 2;
+#pragma unroll 4
+    for (int c = threadIdx.x; c < chunks; c += 256) {
+      const int h = (c / head_chunks) % a.hkv;
+      uint4 kc = k[c], vc = v[c];
+      float ks = a.ks[at * a.hkv + h], vs = a.vs[at * a.hkv + h];
+      if (!good) {  // a page outside the pool: zeros
+        kc = vc = make_uint4(0u, 0u, 0u, 0u);
+        ks = vs = 0.f;
+      }
+      uint4 o[2];
+      widen16<T>(kc, ks, o);
+      ko[2 * c] = o[0];
+      ko[2 * c + 1] = o[1];
+      widen16<T>(vc, vs, o);
+      vo[2 * c] = o[0];
+      vo[2 * c + 1] = o[1];
+    }
+  }
+}
+
 }  // namespace
+
+cudaError_t launch_expand_fp8(const ExpandFp8Args& a, int dtype, int num_sms, cudaStream_t stream) {
+  expand_plan_kernel<<<1, 1024, 0, stream>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int grid = a.scratch_blocks < num_sms * 8 ? a.scratch_blocks : num_sms * 8;
+  if (dtype == B200_DTYPE_BF16) expand_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a);
+  else if (dtype == B200_DTYPE_F16) expand_kernel<__half><<<grid, 256, 0, stream>>>(a);
+  else return cudaErrorInvalidValue;
+  return cudaGetLastError();
+}
 
 cudaError_t launch_row_fp8(const AttnFp8Args& a, int dtype, int rows, cudaStream_t stream) {
   if (rows <= 0) return cudaSuccess;

@@ -237,10 +237,12 @@ def test_prefill(ops, dtype, case, bound):
     assert (out[-extra:] == 5.0).all()
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_prefill_bad_pages_do_not_take_part(ops, dtype):
+@pytest.mark.parametrize("dtype", ALL)
+def test_prefill_bad_pages_leave_other_sequences_alone(ops, dtype):
+    """A page outside the pool is flagged and read nowhere; the other sequences, a decode of this
+    one's like included, keep their results."""
     from llm_serving_b200 import _native as N
-    ctx, new, hq, H, D, BS = [100, 60, 50], [80, 60, 1], 8, 2, 128, 16
+    ctx, new, hq, H, D, BS = [100, 60, 50, 77], [80, 60, 1, 33], 8, 2, 128, 16
     q, cache, tables, cu, lens = _batch(ctx, new, hq, H, D, BS, dtype, seed=8)
     tables[0, 2] = -1
     tables[1, 3] = cache[0].shape[1]
@@ -248,7 +250,22 @@ def test_prefill_bad_pages_do_not_take_part(ops, dtype):
     ref = R.attend(q, *cache, 1, tables, cu, ctx, 0.1)
     got = ops.paged_prefill_fp8(q.cuda(), *[t.cuda() for t in cache], 1, tables.cuda(), cu.cuda(), lens.cuda(), 0.1, 80, 100)
     assert ops.read_status(torch.device("cuda")) & N.DEVICE_BAD_BLOCK
-    _close(got, dtype, ref, ctx, D, PREFILL_BITS[dtype])
+    _close(got[140:], dtype, tuple(t[140:] for t in ref), ctx, D, PREFILL_BITS[dtype])
+    assert got.isfinite().all()
+
+
+def test_prefill_bound_too_small_is_flagged(ops):
+    from llm_serving_b200 import _native as N
+    ctx, new = [40, 100], [40, 100]
+    q, cache, tables, cu, lens = _batch(ctx, new, 8, 2, 64, 16, torch.bfloat16, seed=2)
+    ref = R.attend(q, *cache, 0, tables, cu, ctx, 0.1)
+    args = (q.cuda(), *[t.cuda() for t in cache], 0, tables.cuda(), cu.cuda(), lens.cuda(), 0.1, 100, 100)
+    got = ops.paged_prefill_fp8(*args, prefill_blocks=5)  # ten blocks are needed
+    assert ops.read_status(torch.device("cuda")) & N.DEVICE_BAD_STEP
+    _close(got[:40], torch.bfloat16, tuple(t[:40] for t in ref), ctx, 64, PREFILL_BITS[torch.bfloat16])
+    got = ops.paged_prefill_fp8(*args, prefill_blocks=10)
+    assert ops.read_status(torch.device("cuda")) == 0
+    _close(got, torch.bfloat16, ref, ctx, 64, PREFILL_BITS[torch.bfloat16])
 
 
 def test_append_then_decode_then_prefill(ops):
