@@ -2,6 +2,7 @@
 // k_j = code * key scale of the block, v_j = code * value scale of the block.
 #include <type_traits>
 
+#include "api_common.cuh"
 #include "cache_ops.cuh"
 #include "fp8.cuh"
 
@@ -135,18 +136,17 @@ cudaError_t launch_row_t(const AttnFp8Args& a, int rows, cudaStream_t stream) {
   const dim3 grid(rows, a.hkv * nchunks);
   const int npl = (a.head_dim + 31) / 32;
   const size_t smem = (kRowWarps * 8 * a.head_dim + 2 * kRowWarps * 8) * sizeof(float);
-  const auto launch = [&](auto kern) -> cudaError_t {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 68 * 1024);
+  if (npl <= 1) row_fp8_kernel<T, 1><<<grid, kRowWarps * 32, smem, stream>>>(a, nchunks);
+  else if (npl <= 2) row_fp8_kernel<T, 2><<<grid, kRowWarps * 32, smem, stream>>>(a, nchunks);
+  else if (npl <= 4) row_fp8_kernel<T, 4><<<grid, kRowWarps * 32, smem, stream>>>(a, nchunks);
+  else if (npl <= 8) {
+    const cudaError_t e = allow_smem<row_fp8_kernel<T, 8>>(68 * 1024);
     if (e != cudaSuccess) return e;
-    kern<<<grid, kRowWarps * 32, smem, stream>>>(a, nchunks);
-    return cudaGetLastError();
-  };
-  if (npl <= 1) return launch(row_fp8_kernel<T, 1>);
-  if (npl <= 2) return launch(row_fp8_kernel<T, 2>);
-  if (npl <= 4) return launch(row_fp8_kernel<T, 4>);
-  if (npl <= 8) return launch(row_fp8_kernel<T, 8>);
-  return cudaErrorInvalidValue;
+    row_fp8_kernel<T, 8><<<grid, kRowWarps * 32, smem, stream>>>(a, nchunks);
+  } else {
+    return cudaErrorInvalidValue;
+  }
+  return cudaGetLastError();
 }
 
 // ---- the 16-bit copy of a prefill's pages -----------------------------------------------------

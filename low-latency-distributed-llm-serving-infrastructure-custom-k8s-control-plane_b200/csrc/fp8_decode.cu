@@ -23,6 +23,7 @@
 // Bound: HBM (4 * G flop per byte).  A unit is 64 * D bytes.
 #include <cuda.h>
 
+#include "api_common.cuh"
 #include "fp8.cuh"
 #include "fp8_decode.cuh"
 #include "tc05.cuh"
@@ -898,7 +899,7 @@ cudaError_t launch_t(const CUtensorMap& km, const CUtensorMap& vm, const DecodeF
                      cudaStream_t stream) {
   const int smem = smem_bytes<D>(a.S);
   auto kern = decode_fp8_kernel<T, D, NP, SPLIT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<decode_fp8_kernel<T, D, NP, SPLIT>>(smem_bytes<D>(kDecodeFp8MaxSeqs));
   if (e != cudaSuccess) return e;
   kern<<<grid, kThreads, smem, stream>>>(km, vm, a);
   e = cudaGetLastError();

@@ -6,6 +6,7 @@ fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional
 
@@ -24,6 +25,29 @@ def _require_cuda(*tensors):
 
 def _stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_NOTHING = contextlib.nullcontext()
+_STATUS_PTR = {}
+
+
+def _on(dev: torch.device):
+    """Makes ``dev`` the current device where it is not (entering torch's own guard costs some
+    microseconds even where it is)."""
+    return _NOTHING if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+
+
+def _raw_stream(dev: torch.device) -> int:
+    """``_stream`` of a device with an index, without building a stream object."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _status_ptr(dev: torch.device) -> int:
+    """Address of ``status_word`` of a device with an index."""
+    at = _STATUS_PTR.get(dev.index)
+    if at is None:
+        at = _STATUS_PTR[dev.index] = status_word(dev).data_ptr()
+    return at
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -337,10 +361,12 @@ def fp8_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scale: tor
 
 def _one_device(*tensors) -> torch.device:
     """The CUDA device that all the tensors are on."""
-    _require_cuda(*tensors)
     dev = tensors[0].device
+    if dev.type != "cuda":
+        _require_cuda(*tensors)
     for t in tensors:
         if t is not None and t.device != dev:
+            _require_cuda(t)
             raise ValueError(f"tensors are on {dev} and on {t.device}")
     return dev
 
@@ -381,14 +407,14 @@ def reshape_and_cache_fp8(key: torch.Tensor, value: torch.Tensor, key_cache: tor
     if key.stride(-1) != 1 or value.stride(-1) != 1:
         raise ValueError("head dim must be contiguous")
     dev = _one_device(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
-    with torch.cuda.device(dev):
-        stream = _stream(dev)
+    with _on(dev):
+        stream = _raw_stream(dev)
         n = key.shape[0]
         ws = _append_workspace(c, n, dev, stream)
         N.check(N.lib().b200_reshape_and_cache_fp8(
             ctypes.byref(c), code, key.data_ptr(), key.stride(0), key.stride(1),
             value.data_ptr(), value.stride(0), value.stride(1), slot_mapping.data_ptr(), n,
-            _ptr(ws), 0 if ws is None else ws.numel(), status_word(dev).data_ptr(), stream))
+            _ptr(ws), 0 if ws is None else ws.numel(), _status_ptr(dev), stream))
 
 
 def rope_reshape_and_cache_fp8(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -423,13 +449,13 @@ def rope_reshape_and_cache_fp8(qkv: torch.Tensor, positions: torch.Tensor, inv_f
         raise ValueError("q_out must have contiguous heads")
     dev = _one_device(qkv, positions, inv_freq, key_cache, value_cache, key_scale, value_scale,
                       slot_mapping, q_out)
-    with torch.cuda.device(dev):
-        stream = _stream(dev)
+    with _on(dev):
+        stream = _raw_stream(dev)
         ws = _append_workspace(c, n, dev, stream)
         N.check(N.lib().b200_rope_reshape_and_cache_fp8(
             ctypes.byref(c), code, qkv.data_ptr(), qkv.stride(0), n, hq, positions.data_ptr(),
             inv_freq.data_ptr(), q_out.data_ptr(), q_out.stride(0), slot_mapping.data_ptr(),
-            _ptr(ws), 0 if ws is None else ws.numel(), status_word(dev).data_ptr(), stream))
+            _ptr(ws), 0 if ws is None else ws.numel(), _status_ptr(dev), stream))
     return q_out
 
 
@@ -444,10 +470,10 @@ def gather_cache_fp8(key_cache: torch.Tensor, value_cache: torch.Tensor, key_sca
     _check_slots(slots, None)
     dev = _one_device(key_cache, value_cache, key_scale, value_scale, slots)
     out = torch.empty((2, slots.shape[0], c.num_kv_heads, c.head_dim), dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         N.check(N.lib().b200_gather_cache_fp8(
             ctypes.byref(c), _DTYPES[dtype], slots.data_ptr(), slots.shape[0], out[0].data_ptr(),
-            out[1].data_ptr(), status_word(dev).data_ptr(), _stream(dev)))
+            out[1].data_ptr(), _status_ptr(dev), _raw_stream(dev)))
     return out[0], out[1]
 
 
@@ -514,10 +540,10 @@ def paged_decode_fp8(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
                              block_tables, context_lens, scale, out, max_context_len, query_rows)
     dev = _one_device(query, key_cache, value_cache, key_scale, value_scale, block_tables,
                       context_lens, out, query_rows, workspace)
-    p.status_word = status_word(dev).data_ptr()
+    p.status_word = _status_ptr(dev)
     L = N.lib()
-    with torch.cuda.device(dev):
-        stream = _stream(dev)
+    with _on(dev):
+        stream = _raw_stream(dev)
         need = L.b200_paged_decode_fp8_workspace_bytes(ctypes.byref(p))
         ws = workspace if workspace is not None else (
             _WORKSPACE.get(dev, need, stream) if need else None)
@@ -544,10 +570,10 @@ def paged_prefill_fp8(query: torch.Tensor, key_cache: torch.Tensor, value_cache:
                              prefill_blocks=-1 if prefill_blocks is None else prefill_blocks)
     dev = _one_device(query, key_cache, value_cache, key_scale, value_scale, block_tables,
                       cu_seqlens, context_lens, out)
-    p.status_word = status_word(dev).data_ptr()
+    p.status_word = _status_ptr(dev)
     L = N.lib()
-    with torch.cuda.device(dev):
-        stream = _stream(dev)
+    with _on(dev):
+        stream = _raw_stream(dev)
         need = L.b200_paged_prefill_fp8_workspace_bytes(ctypes.byref(p))
         ws = _WORKSPACE.get(dev, need, stream) if need else None
         N.check(L.b200_paged_prefill_fp8(ctypes.byref(p), _ptr(ws),

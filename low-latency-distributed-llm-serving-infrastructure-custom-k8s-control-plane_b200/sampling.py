@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native as N
-from .paged_ops import _DTYPES, _one_device, _ptr, _stream, status_word
+from .paged_ops import _DTYPES, _on, _one_device, _ptr, _raw_stream, _status_ptr
 
 
 @dataclass
@@ -70,9 +70,9 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor,
     dev = _one_device(logits, uniform, temperature, top_k, top_p, min_p)
     tokens = torch.empty(rows, dtype=torch.int64, device=dev)
     logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         N.check(N.lib().b200_sample(
             logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), rows, vocab,
             uniform.data_ptr(), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
-            tokens.data_ptr(), logprobs.data_ptr(), status_word(dev).data_ptr(), _stream(dev)))
+            tokens.data_ptr(), logprobs.data_ptr(), _status_ptr(dev), _raw_stream(dev)))
     return tokens, logprobs
