@@ -101,12 +101,13 @@ struct RowList {
 };
 
 // The next rows (at most kChunkRows) of block slots [s0, s0 + bs) at or after row `pos`, in order;
-// stops early once `want` rows have been found.  Called by the whole CTA.
-__device__ void next_rows(const AppendFp8Args& a, int64_t s0, int pos, int want, RowList& list,
-                          int32_t* warp_n) {
+// stops once `want` rows have been found.  want < 0: all rows from `pos` on are looked at, and the
+// number found is returned (the first kChunkRows of them are listed).  Called by the whole CTA.
+__device__ int next_rows(const AppendFp8Args& a, int64_t s0, int pos, int want, RowList& list,
+                         int32_t* warp_n) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int found = 0;
-  while (pos < a.num_tokens && found < want && found < kChunkRows) {
+  while (pos < a.num_tokens && (want < 0 || (found < want && found < kChunkRows))) {
     const int r = pos + tid;
     const int64_t slot = r < a.num_tokens ? a.slots[r] : -1;
     const bool in = slot >= s0 && slot < s0 + a.bs;
@@ -132,6 +133,7 @@ __device__ void next_rows(const AppendFp8Args& a, int64_t s0, int pos, int want,
   }
   if (tid == 0) list.n = min(found, kChunkRows);
   __syncthreads();
+  return found;
 }
 
 template <typename T, bool ROPE>
@@ -187,16 +189,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_fp8_kernel(AppendFp8Arg
     const int64_t blk = slot / a.bs, s0 = blk * a.bs;
     int want;
     if (scan) {
-      bool earlier = false;
-      want = 0;
-      for (int r0 = 0; r0 < a.num_tokens; r0 += kAppendThreads) {
-        const int r = r0 + tid;
-        const int64_t o = r < a.num_tokens ? a.slots[r] : -1;
-        const bool in = o >= s0 && o < s0 + a.bs;
-        earlier |= in && r < t;
-        want += __syncthreads_count(in);
-      }
-      if (__syncthreads_or(earlier)) continue;  // the block's first row owns it
+      want = next_rows(a, s0, 0, -1, list, warp_n);
+      if (list.row[0] != t) continue;  // the block's first row owns it
     } else {
       if (a.num_tokens - a.first[blk] != t) continue;
       want = a.count[blk];
@@ -319,6 +313,305 @@ __global__ void __launch_bounds__(kAppendThreads) append_fp8_kernel(AppendFp8Arg
   }
 }
 
+// ---- head dims 64 and 128, 16-byte aligned rows ---------------------------------------------------
+
+// Eight adjacent elements as fp32.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(e[i]);
+}
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+  const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
+  x[0] = u.x;
+  x[1] = u.y;
+  x[2] = u.z;
+  x[3] = u.w;
+  x[4] = v.x;
+  x[5] = v.y;
+  x[6] = v.z;
+  x[7] = v.w;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  uint4 u;
+  T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
+  *reinterpret_cast<uint4*>(p) = u;
+}
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+
+// Two values' codes; what is not finite becomes NaN.
+__device__ __forceinline__ uint32_t codes2(float x, float y) {
+  x = fabsf(x) < INFINITY ? x : NAN;
+  y = fabsf(y) < INFINITY ? y : NAN;
+  return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+}
+
+// Four held codes rescaled.
+__device__ __forceinline__ uint32_t rescale4(uint32_t c, float ratio) {
+  const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(c & 0xffffu, __NV_E4M3)));
+  const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(c >> 16, __NV_E4M3)));
+  return codes2(a.x * ratio, a.y * ratio) | (codes2(b.x * ratio, b.y * ratio) << 16);
+}
+
+// A warp takes one head's keys (or values) of up to 16 rows into registers: LPR lanes a row, each
+// with 8 elements of the row's first half and the 8 that they rotate with.  They are read once,
+// and the maximum, the scale and the codes follow without touching memory again.
+template <typename T, bool ROPE, int D>
+__global__ void __launch_bounds__(kAppendThreads, 2)
+    append_vec_kernel(AppendFp8Args a, int kv_ctas, int q_rows) {
+  constexpr int kHalf = D / 2, LPR = kHalf / 8, RPP = 32 / LPR, P = kChunkRows / RPP;
+  extern __shared__ __align__(16) float sm[];
+  __shared__ RowList list;
+  __shared__ int32_t warp_n[kAppendWarps];
+  __shared__ uint32_t written[kMaxBlockSize / 32];
+  __shared__ int32_t fresh_s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  // ---- queries: every thread keeps the angles of its 8 pairs for all its heads --------------------
+  if (ROPE && static_cast<int>(blockIdx.x) >= kv_ctas) {
+    const int r0 = (blockIdx.x - kv_ctas) * q_rows, rows = min(a.num_tokens - r0, q_rows);
+    float2* cs = reinterpret_cast<float2*>(sm);  // [q_rows][kHalf]
+    for (int w = tid; w < rows * kHalf; w += kAppendThreads) {
+      const Turn t = turn_of(a.positions[r0 + w / kHalf], a.inv_freq[w % kHalf]);
+      cs[w] = make_float2(t.ch, t.sh);
+    }
+    __syncthreads();
+    const int c = tid % LPR, row = (tid / LPR) % q_rows, groups = kAppendThreads / (LPR * q_rows);
+    if (row >= rows) return;
+    float cv[8], sv[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = cs[row * kHalf + c * 8 + i];
+      cv[i] = v.x;
+      sv[i] = v.y;
+    }
+    const T* src = static_cast<const T*>(a.q_in) + (r0 + row) * a.q_stok + c * 8;
+    T* dst = static_cast<T*>(a.q_out) + (r0 + row) * a.qo_stok + c * 8;
+#pragma unroll 4
+    for (int h = tid / (LPR * q_rows); h < a.hq; h += groups) {
+      float x[8], y[8];
+      load8<T>(src + h * D, x);
+      load8<T>(src + h * D + kHalf, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float u = x[i] * cv[i] - y[i] * sv[i];
+        y[i] = y[i] * cv[i] + x[i] * sv[i];
+        x[i] = u;
+      }
+      store8<T>(dst + h * D, x);
+      store8<T>(dst + h * D + kHalf, y);
+    }
+    return;
+  }
+
+  // ---- keys and values, block by block -------------------------------------------------------
+  const int64_t total_slots = static_cast<int64_t>(a.nb) * a.bs;
+  Turn* cs = reinterpret_cast<Turn*>(sm);                  // [kChunkRows][kHalf]
+  float* amax = sm + (ROPE ? kChunkRows * 2 * D : 0);      // [2 * hkv], calls with longer lists only
+  const int c = lane % LPR, rs = lane / LPR;
+  const bool scan = a.runs == nullptr;
+  const int units = scan ? a.num_tokens : *a.num_runs;
+  for (int unit = blockIdx.x; unit < units; unit += kv_ctas) {
+    const int t = scan ? unit : a.runs[unit];
+    const int64_t slot = a.slots[t];
+    if (slot < 0 || slot >= total_slots) {
+      if (slot >= total_slots && tid == 0) flag_status(a.status, B200_DEVICE_BAD_SLOT);
+      continue;
+    }
+    // 32-bit division where it does: 64-bit division takes some hundred cycles
+    const int64_t blk = (slot >> 32) == 0 ? static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.bs) : slot / a.bs;
+    const int64_t s0 = blk * a.bs;
+    __syncthreads();  // the list of the unit before is no longer read
+    int want;
+    if (scan) {
+      want = next_rows(a, s0, 0, -1, list, warp_n);
+      if (list.row[0] != t) continue;  // the block's first row owns it
+    } else {
+      if (a.num_tokens - a.first[blk] != t) continue;
+      want = a.count[blk];
+      next_rows(a, s0, t, want, list, warp_n);
+    }
+    if (tid == 0) fresh_s = 0;
+    for (int i = tid; i < (a.bs + 31) / 32; i += kAppendThreads) written[i] = 0u;
+    __syncthreads();
+
+    const auto turns = [&]() {  // of the list's rows; what the list says goes into written, fresh_s
+      if (tid < list.n) {
+        atomicOr(&written[list.off[tid] >> 5], 1u << (list.off[tid] & 31));
+        if (list.off[tid] == 0) fresh_s = 1;
+      }
+      if (ROPE) {
+        for (int w = tid; w < list.n * kHalf; w += kAppendThreads)
+          cs[w] = turn_of(a.positions[list.row[w / kHalf]], a.inv_freq[w % kHalf]);
+      }
+      __syncthreads();
+    };
+    const auto load = [&](int task, float (&x)[P][2][8]) {
+      const bool is_v = task & 1;
+      const T* base = static_cast<const T*>(is_v ? a.value : a.key) + (task >> 1) * (is_v ? a.v_shead : a.k_shead) + c * 8;
+      const int64_t stok = is_v ? a.v_stok : a.k_stok;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const int r = p * RPP + rs;
+        if (r < list.n) {
+          load8<T>(base + list.row[r] * stok, x[p][0]);
+          load8<T>(base + list.row[r] * stok + kHalf, x[p][1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[p][0][i] = x[p][1][i] = 0.f;
+        }
+      }
+      if (ROPE && !is_v) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const int r = p * RPP + rs;
+          if (r < list.n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const Turn w = cs[r * kHalf + c * 8 + i];
+              const float u = x[p][0][i], v = x[p][1][i];
+              x[p][0][i] = mul_add2(u, w.ch, w.cl, -v, w.sh, w.sl);
+              x[p][1][i] = mul_add2(v, w.ch, w.cl, u, w.sh, w.sl);
+            }
+          }
+        }
+      }
+    };
+    const auto largest = [&](const float (&x)[P][2][8]) {
+      float m = 0.f;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float u = fabsf(x[p][0][i]), v = fabsf(x[p][1][i]);
+          if (u < INFINITY) m = fmaxf(m, u);  // false for NaN too
+          if (v < INFINITY) m = fmaxf(m, v);
+        }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      return m;
+    };
+    const int64_t cache_blk = static_cast<int64_t>(a.layer) * a.nb + blk;
+    const int64_t row_bytes = static_cast<int64_t>(a.hkv) * D;
+    const auto codes_of = [&](int task) {
+      return ((task & 1) ? a.vc : a.kc) + (cache_blk * a.bs * a.hkv + (task >> 1)) * D;
+    };
+    // the block's new scale for this head; rescales what it holds where the scale grows
+    const auto settle = [&](int task, float old, float m) {
+      if (!(old > 0.f) || isinf(old)) old = 0.f;  // never written
+      float s = scale_for(m);
+      if (!fresh_s) {
+        s = fmaxf(s, old);
+        if (s != old) {
+          const float ratio = old / s;
+          uint8_t* codes = codes_of(task);
+          constexpr int kRowLanes = D / 16;
+          for (int o = lane / kRowLanes; o < a.bs; o += 32 / kRowLanes) {
+            if ((written[o >> 5] >> (o & 31)) & 1u) continue;
+            uint4* q = reinterpret_cast<uint4*>(codes + o * row_bytes) + lane % kRowLanes;
+            uint4 v = *q;
+            v.x = rescale4(v.x, ratio);
+            v.y = rescale4(v.y, ratio);
+            v.z = rescale4(v.z, ratio);
+            v.w = rescale4(v.w, ratio);
+            *q = v;
+          }
+        }
+      }
+      if (lane == 0) ((task & 1) ? a.vs : a.ks)[cache_blk * a.hkv + (task >> 1)] = s;
+      return s;
+    };
+    const auto store = [&](int task, float s, float (&x)[P][2][8]) {
+      uint8_t* codes = codes_of(task) + c * 8;
+      const bool pow2 = is_pow2(s);
+      const float inv = 1.f / s;
+      if (!pow2) {  // a scale that a caller wrote
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[p][0][i] /= s;
+            x[p][1][i] /= s;
+          }
+      }
+      const float f = pow2 ? inv : 1.f;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const int r = p * RPP + rs;
+        bool live = r < list.n;
+        // of rows with one slot only the last is stored
+        if (live)
+          for (int k = r + 1; k < list.n; ++k) live &= list.off[k] != list.off[r];
+        if (!live) continue;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const float(&y)[8] = x[p][hf];
+          uint2 v;
+          v.x = codes2(y[0] * f, y[1] * f) | (codes2(y[2] * f, y[3] * f) << 16);
+          v.y = codes2(y[4] * f, y[5] * f) | (codes2(y[6] * f, y[7] * f) << 16);
+          *reinterpret_cast<uint2*>(codes + list.off[r] * row_bytes + hf * kHalf) = v;
+        }
+      }
+    };
+
+    turns();
+    if (want <= kChunkRows) {
+      for (int task = warp; task < 2 * a.hkv; task += kAppendWarps) {
+        const float old = ((task & 1) ? a.vs : a.ks)[cache_blk * a.hkv + (task >> 1)];
+        float x[P][2][8];
+        load(task, x);
+        const float s = settle(task, old, largest(x));
+        store(task, s, x);
+      }
+      continue;
+    }
+    // more rows than the registers hold: the maxima over all chunks of rows first, then the codes
+    for (int i = tid; i < 2 * a.hkv; i += kAppendThreads) amax[i] = 0.f;
+    for (int pass = 0; pass < 2; ++pass) {
+      if (pass == 1) {
+        __syncthreads();
+        for (int task = warp; task < 2 * a.hkv; task += kAppendWarps) {
+          const float old = ((task & 1) ? a.vs : a.ks)[cache_blk * a.hkv + (task >> 1)];
+          __syncwarp();
+          const float s = settle(task, old, amax[task]);
+          __syncwarp();
+          if (lane == 0) amax[task] = s;
+        }
+      }
+      int pos = t, seen = 0;
+      while (seen < want) {
+        __syncthreads();
+        next_rows(a, s0, pos, want - seen, list, warp_n);
+        turns();
+        for (int task = warp; task < 2 * a.hkv; task += kAppendWarps) {
+          float x[P][2][8];
+          load(task, x);
+          if (pass == 0) {
+            const float m = largest(x);
+            if (lane == 0) amax[task] = fmaxf(amax[task], m);
+          } else {
+            store(task, amax[task], x);
+          }
+        }
+        __syncthreads();
+        seen += list.n;
+        pos = list.next;
+        if (list.n == 0) break;
+      }
+    }
+  }
+}
+
 // Rows per block, the first row of each block and the starts of runs of rows of one block.
 __global__ void __launch_bounds__(256) append_mark_kernel(AppendFp8Args a) {
   const int64_t total_slots = static_cast<int64_t>(a.nb) * a.bs;
@@ -374,9 +667,79 @@ __global__ void __launch_bounds__(256) gather_fp8_kernel(GatherFp8Args a) {
   }
 }
 
+// Rows of 16-byte multiples: 16 codes per thread and step.
+template <typename T>
+__global__ void __launch_bounds__(256) gather_vec_kernel(GatherFp8Args a) {
+  const uint32_t per_row = a.hkv * a.head_dim / 16, per_head = a.head_dim / 16;
+  const int64_t slots = static_cast<int64_t>(a.nb) * a.bs;
+  const uint32_t rows = 256 / per_row > 0 ? 256 / per_row : 1;  // of a CTA, side by side
+  const uint32_t r_in = threadIdx.x / per_row;
+  if (r_in >= rows) return;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * rows + r_in; r < a.n; r += static_cast<int64_t>(gridDim.x) * rows) {
+    const int64_t slot = a.slots[r];
+    const bool in = slot >= 0 && slot < slots;
+    if (slot >= slots && threadIdx.x % per_row == 0) flag_status(a.status, B200_DEVICE_BAD_SLOT);
+    const int64_t s = in ? slot : 0;
+    const int64_t blk = static_cast<int64_t>(a.layer) * a.nb +
+                        ((s >> 32) == 0 ? static_cast<uint32_t>(s) / static_cast<uint32_t>(a.bs) : s / a.bs);
+    const int64_t row = (static_cast<int64_t>(a.layer) * slots + s) * per_row;
+    for (uint32_t e = threadIdx.x - r_in * per_row; e < per_row; e += 256) {
+      const int64_t sc = blk * a.hkv + e / per_head;
+      uint4 kc = reinterpret_cast<const uint4*>(a.kc)[row + e], vc = reinterpret_cast<const uint4*>(a.vc)[row + e];
+      float ks = a.ks[sc], vs = a.vs[sc];
+      if (!in) {
+        kc = vc = make_uint4(0u, 0u, 0u, 0u);
+        ks = vs = 0.f;
+      }
+      const auto put = [&](uint4 code, float scale, void* out) {
+        const uint8_t* b = reinterpret_cast<const uint8_t*>(&code);
+        alignas(16) T v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = value_of<T>(b[i], scale);
+        uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(out) + (r * per_row + e) * 16);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) o[i] = reinterpret_cast<const uint4*>(v)[i];
+      };
+      put(kc, ks, a.k_out);
+      put(vc, vs, a.v_out);
+    }
+  }
+}
+
+template <typename T, bool ROPE, int D>
+cudaError_t launch_append_vec(const AppendFp8Args& a, int num_sms, cudaStream_t stream) {
+  // Query rows per CTA: with few rows one each, so that every SM has some (256 rows: 256 CTAs);
+  // with many, four, whose threads then reuse their angles for several heads.
+  const int q_rows = a.num_tokens > 2048 ? 4 : 1;
+  const int q_ctas = ROPE ? (a.num_tokens + q_rows - 1) / q_rows : 0;
+  int kv_ctas = a.num_tokens;
+  if (a.runs != nullptr && kv_ctas > num_sms * 4) kv_ctas = num_sms * 4;
+  const size_t smem = ((ROPE ? kChunkRows * 2 * D : 0) + 2 * a.hkv) * sizeof(float);
+  append_vec_kernel<T, ROPE, D><<<kv_ctas + q_ctas, kAppendThreads, smem, stream>>>(a, kv_ctas, q_rows);
+  return cudaGetLastError();
+}
+
+// Every row, head and page starts on a 16-byte boundary.
+template <typename T>
+bool aligned_rows(const AppendFp8Args& a) {
+  const int64_t es = sizeof(T);
+  uint64_t all = reinterpret_cast<uintptr_t>(a.key) | reinterpret_cast<uintptr_t>(a.value) |
+                 reinterpret_cast<uintptr_t>(a.kc) | reinterpret_cast<uintptr_t>(a.vc);
+  all |= static_cast<uint64_t>((a.k_stok | a.k_shead | a.v_stok | a.v_shead) * es);
+  if (a.positions != nullptr)
+    all |= reinterpret_cast<uintptr_t>(a.q_in) | reinterpret_cast<uintptr_t>(a.q_out) |
+           static_cast<uint64_t>((a.q_stok | a.qo_stok) * es);
+  return all % 16 == 0;
+}
+
 template <typename T>
 cudaError_t launch_append_t(const AppendFp8Args& a, int num_sms, cudaStream_t stream) {
   const bool rope = a.positions != nullptr;
+  if ((a.head_dim == 128 || a.head_dim == 64) && aligned_rows<T>(a)) {
+    if (a.head_dim == 128)
+      return rope ? launch_append_vec<T, true, 128>(a, num_sms, stream) : launch_append_vec<T, false, 128>(a, num_sms, stream);
+    return rope ? launch_append_vec<T, true, 64>(a, num_sms, stream) : launch_append_vec<T, false, 64>(a, num_sms, stream);
+  }
   const int q_rows = a.num_tokens > 2048 ? 8 : 1;
   const int q_ctas = rope ? (a.num_tokens + q_rows - 1) / q_rows : 0;
   int kv_ctas = a.num_tokens;
@@ -418,6 +781,20 @@ cudaError_t launch_append_fp8(const AppendFp8Args& a, int dtype, int num_sms,
 cudaError_t launch_gather_fp8(const GatherFp8Args& a, int dtype, int num_sms,
                               cudaStream_t stream) {
   if (a.n <= 0) return cudaSuccess;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(a.kc) | reinterpret_cast<uintptr_t>(a.vc) |
+                        reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out);
+  if (a.head_dim % 16 == 0 && all % 16 == 0) {
+    const int per_row = a.hkv * a.head_dim / 16, rows = 256 / per_row > 0 ? 256 / per_row : 1;
+    const int64_t need = (a.n + rows - 1) / rows, most = static_cast<int64_t>(num_sms) * 16;
+    const int grid = static_cast<int>(need < most ? need : most);
+    switch (dtype) {
+      case B200_DTYPE_BF16: gather_vec_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a); break;
+      case B200_DTYPE_F16: gather_vec_kernel<__half><<<grid, 256, 0, stream>>>(a); break;
+      case B200_DTYPE_F32: gather_vec_kernel<float><<<grid, 256, 0, stream>>>(a); break;
+      default: return cudaErrorInvalidValue;
+    }
+    return cudaGetLastError();
+  }
   const int64_t total = a.n * a.hkv * a.head_dim;
   int64_t blocks = (total + 255) / 256;
   const int64_t cap = static_cast<int64_t>(num_sms) * 8;
