@@ -363,19 +363,24 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t c, float ratio) {
   return codes2(a.x * ratio, a.y * ratio) | (codes2(b.x * ratio, b.y * ratio) << 16);
 }
 
-// A warp takes one head's keys (or values) of up to 16 rows into registers: LPR lanes a row, each
+// A warp takes one head's keys (or values) of up to 8 rows into registers: LPR lanes a row, each
 // with 8 elements of the row's first half and the 8 that they rotate with.  They are read once,
-// and the maximum, the scale and the codes follow without touching memory again.
+// and the maximum, the scale and the codes follow without touching memory again.  Of more than 8
+// rows two warps take half each and exchange their maxima.
 template <typename T, bool ROPE, int D>
-__global__ void __launch_bounds__(kAppendThreads, 2)
+__global__ void __launch_bounds__(kAppendThreads, 4)
     append_vec_kernel(AppendFp8Args a, int kv_ctas, int q_rows) {
-  constexpr int kHalf = D / 2, LPR = kHalf / 8, RPP = 32 / LPR, P = kChunkRows / RPP;
+  constexpr int kHalf = D / 2, LPR = kHalf / 8, RPP = 32 / LPR, P = kChunkRows / 2 / RPP;
   extern __shared__ __align__(16) float sm[];
   __shared__ RowList list;
   __shared__ int32_t warp_n[kAppendWarps];
   __shared__ uint32_t written[kMaxBlockSize / 32];
   __shared__ int32_t fresh_s;
+  __shared__ float half_max[kAppendWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // pair i of a row (elements i and i + D/2) in shared memory: the pairs that the LPR lanes of a row
+  // read together lie side by side
+  const auto place = [](int i) { return (i % 8) * LPR + i / 8; };
 
   // ---- queries: every thread keeps the angles of its 8 pairs for all its heads --------------------
   if (ROPE && static_cast<int>(blockIdx.x) >= kv_ctas) {
@@ -383,7 +388,7 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
     float2* cs = reinterpret_cast<float2*>(sm);  // [q_rows][kHalf]
     for (int w = tid; w < rows * kHalf; w += kAppendThreads) {
       const Turn t = turn_of(a.positions[r0 + w / kHalf], a.inv_freq[w % kHalf]);
-      cs[w] = make_float2(t.ch, t.sh);
+      cs[w / kHalf * kHalf + place(w % kHalf)] = make_float2(t.ch, t.sh);
     }
     __syncthreads();
     const int c = tid % LPR, row = (tid / LPR) % q_rows, groups = kAppendThreads / (LPR * q_rows);
@@ -391,7 +396,7 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
     float cv[8], sv[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 v = cs[row * kHalf + c * 8 + i];
+      const float2 v = cs[row * kHalf + i * LPR + c];
       cv[i] = v.x;
       sv[i] = v.y;
     }
@@ -452,17 +457,18 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
       }
       if (ROPE) {
         for (int w = tid; w < list.n * kHalf; w += kAppendThreads)
-          cs[w] = turn_of(a.positions[list.row[w / kHalf]], a.inv_freq[w % kHalf]);
+          cs[w / kHalf * kHalf + place(w % kHalf)] = turn_of(a.positions[list.row[w / kHalf]], a.inv_freq[w % kHalf]);
       }
       __syncthreads();
     };
-    const auto load = [&](int task, float (&x)[P][2][8]) {
+    // rows [r0, r0 + 8) of the list
+    const auto load = [&](int task, int r0, float (&x)[P][2][8]) {
       const bool is_v = task & 1;
       const T* base = static_cast<const T*>(is_v ? a.value : a.key) + (task >> 1) * (is_v ? a.v_shead : a.k_shead) + c * 8;
       const int64_t stok = is_v ? a.v_stok : a.k_stok;
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        const int r = p * RPP + rs;
+        const int r = r0 + p * RPP + rs;
         if (r < list.n) {
           load8<T>(base + list.row[r] * stok, x[p][0]);
           load8<T>(base + list.row[r] * stok + kHalf, x[p][1]);
@@ -474,11 +480,11 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
       if (ROPE && !is_v) {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          const int r = p * RPP + rs;
+          const int r = r0 + p * RPP + rs;
           if (r < list.n) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const Turn w = cs[r * kHalf + c * 8 + i];
+              const Turn w = cs[r * kHalf + i * LPR + c];
               const float u = x[p][0][i], v = x[p][1][i];
               x[p][0][i] = mul_add2(u, w.ch, w.cl, -v, w.sh, w.sl);
               x[p][1][i] = mul_add2(v, w.ch, w.cl, u, w.sh, w.sl);
@@ -507,7 +513,8 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
       return ((task & 1) ? a.vc : a.kc) + (cache_blk * a.bs * a.hkv + (task >> 1)) * D;
     };
     // the block's new scale for this head; rescales what it holds where the scale grows
-    const auto settle = [&](int task, float old, float m) {
+    // (part `part` of `parts` of its rows; part 0 writes the scale)
+    const auto settle = [&](int task, float old, float m, int part, int parts) {
       if (!(old > 0.f) || isinf(old)) old = 0.f;  // never written
       float s = scale_for(m);
       if (!fresh_s) {
@@ -516,7 +523,7 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
           const float ratio = old / s;
           uint8_t* codes = codes_of(task);
           constexpr int kRowLanes = D / 16;
-          for (int o = lane / kRowLanes; o < a.bs; o += 32 / kRowLanes) {
+          for (int o = part * (32 / kRowLanes) + lane / kRowLanes; o < a.bs; o += parts * (32 / kRowLanes)) {
             if ((written[o >> 5] >> (o & 31)) & 1u) continue;
             uint4* q = reinterpret_cast<uint4*>(codes + o * row_bytes) + lane % kRowLanes;
             uint4 v = *q;
@@ -528,10 +535,10 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
           }
         }
       }
-      if (lane == 0) ((task & 1) ? a.vs : a.ks)[cache_blk * a.hkv + (task >> 1)] = s;
+      if (lane == 0 && part == 0) ((task & 1) ? a.vs : a.ks)[cache_blk * a.hkv + (task >> 1)] = s;
       return s;
     };
-    const auto store = [&](int task, float s, float (&x)[P][2][8]) {
+    const auto store = [&](int task, int r0, float s, float (&x)[P][2][8]) {
       uint8_t* codes = codes_of(task) + c * 8;
       const bool pow2 = is_pow2(s);
       const float inv = 1.f / s;
@@ -547,7 +554,7 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
       const float f = pow2 ? inv : 1.f;
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        const int r = p * RPP + rs;
+        const int r = r0 + p * RPP + rs;
         bool live = r < list.n;
         // of rows with one slot only the last is stored
         if (live)
@@ -565,13 +572,30 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
     };
 
     turns();
-    if (want <= kChunkRows) {
+    const auto scale_at = [&](int task) { return ((task & 1) ? a.vs : a.ks) + cache_blk * a.hkv + (task >> 1); };
+    if (want <= kChunkRows / 2) {
       for (int task = warp; task < 2 * a.hkv; task += kAppendWarps) {
-        const float old = ((task & 1) ? a.vs : a.ks)[cache_blk * a.hkv + (task >> 1)];
+        const float old = *scale_at(task);
         float x[P][2][8];
-        load(task, x);
-        const float s = settle(task, old, largest(x));
-        store(task, s, x);
+        load(task, 0, x);
+        const float s = settle(task, old, largest(x), 0, 1);
+        store(task, 0, s, x);
+      }
+      continue;
+    }
+    const int part = warp & 1, r0 = part * (kChunkRows / 2);
+    if (want <= kChunkRows) {
+      for (int task = warp >> 1; task < 2 * a.hkv; task += kAppendWarps / 2) {
+        const float old = *scale_at(task);
+        float x[P][2][8];
+        load(task, r0, x);
+        const float m = largest(x);
+        if (lane == 0) half_max[warp] = m;
+        // the two warps of the task: both maxima written and both old scales read
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp >> 1)) : "memory");
+        const float s = settle(task, old, fmaxf(m, half_max[warp ^ 1]), part, 2);
+        store(task, r0, s, x);
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp >> 1)) : "memory");
       }
       continue;
     }
@@ -581,9 +605,9 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
       if (pass == 1) {
         __syncthreads();
         for (int task = warp; task < 2 * a.hkv; task += kAppendWarps) {
-          const float old = ((task & 1) ? a.vs : a.ks)[cache_blk * a.hkv + (task >> 1)];
+          const float old = *scale_at(task);
           __syncwarp();
-          const float s = settle(task, old, amax[task]);
+          const float s = settle(task, old, amax[task], 0, 1);
           __syncwarp();
           if (lane == 0) amax[task] = s;
         }
@@ -594,13 +618,15 @@ __global__ void __launch_bounds__(kAppendThreads, 2)
         next_rows(a, s0, pos, want - seen, list, warp_n);
         turns();
         for (int task = warp; task < 2 * a.hkv; task += kAppendWarps) {
-          float x[P][2][8];
-          load(task, x);
-          if (pass == 0) {
-            const float m = largest(x);
-            if (lane == 0) amax[task] = fmaxf(amax[task], m);
-          } else {
-            store(task, amax[task], x);
+          for (int h0 = 0; h0 < kChunkRows; h0 += kChunkRows / 2) {
+            float x[P][2][8];
+            load(task, h0, x);
+            if (pass == 0) {
+              const float m = largest(x);
+              if (lane == 0) amax[task] = fmaxf(amax[task], m);
+            } else {
+              store(task, h0, amax[task], x);
+            }
           }
         }
         __syncthreads();
@@ -713,7 +739,7 @@ cudaError_t launch_append_vec(const AppendFp8Args& a, int num_sms, cudaStream_t 
   const int q_rows = a.num_tokens > 2048 ? 4 : 1;
   const int q_ctas = ROPE ? (a.num_tokens + q_rows - 1) / q_rows : 0;
   int kv_ctas = a.num_tokens;
-  if (a.runs != nullptr && kv_ctas > num_sms * 4) kv_ctas = num_sms * 4;
+  if (a.runs != nullptr && kv_ctas > num_sms * 8) kv_ctas = num_sms * 8;
   const size_t smem = ((ROPE ? kChunkRows * 2 * D : 0) + 2 * a.hkv) * sizeof(float);
   append_vec_kernel<T, ROPE, D><<<kv_ctas + q_ctas, kAppendThreads, smem, stream>>>(a, kv_ctas, q_rows);
   return cudaGetLastError();
