@@ -8,6 +8,8 @@
 //   cumulative w exceeds u times the kept sum.
 // What a draw and a top-p border are decided by are sums of up to 10^5 weights, so w is computed
 // in 64 bits and summed in fixed point (64-bit integers): exact sums, in any order.
+#include <cooperative_groups.h>
+
 #include "api_common.cuh"
 #include "cache_ops.cuh"
 #include "nvtx.cuh"
@@ -71,16 +73,52 @@ __device__ __forceinline__ float float_of(uint32_t key) {
   return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// w of a logit x in a row with maximum mx; it = 1 / temperature is applied by division to stay
-// within a rounding of the definition.
-__device__ __forceinline__ double weight(float x, float mx, double t) {
-  if (x == mx) return 1.0;
-  return exp((static_cast<double>(x) - static_cast<double>(mx)) / t);
+// w of a logit in a row with maximum mx, from a table of 2^(j/64) and four terms of the exponential
+// series: with y = 64 (x - mx) log2(e) / t = n + r, w = 2^(n/64) e^(r ln2 / 64), |r ln2 / 64| <=
+// 0.0055, remainder below 5e-14.
+struct Weights {
+  const double* table;  // 2^(j/64), j < 64, in shared memory
+  double mx, c;         // maximum; 64 log2(e) / t
+  float mxf;
+  double bias;          // 2^(52 - shift): adding it leaves round(w 2^shift) in the mantissa's low bits
+
+  __device__ __forceinline__ void set(const double* tab, float m, double t, int shift) {
+    table = tab;
+    mxf = m;
+    mx = static_cast<double>(m);
+    c = 64.0 * 1.4426950408889634 / t;
+    bias = static_cast<double>(1ull << (52 - shift));
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    if (x == mxf) return 1.0;
+    const double y = (static_cast<double>(x) - mx) * c;
+    if (!(y > -3968.0)) return 0.0;  // below 2^-62
+    const double v = y + 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are round(y)
+    const int n = __double2loint(v);
+    const double f = (y - (v - 6755399441055744.0)) * (0.6931471805599453 / 64.0);
+    double p = fma(f, 1.0 / 24.0, 1.0 / 6.0);
+    p = fma(p, f, 0.5);
+    p = fma(p, f, 1.0);
+    p = fma(p, f, 1.0);
+    const double w = table[n & 63] * p;
+    return __hiloint2double(__double2hiint(w) + ((n >> 6) << 20), __double2loint(w));
+  }
+  __device__ __forceinline__ unsigned long long fixed(double w) const {
+    return static_cast<unsigned long long>(__double_as_longlong(w + bias)) & 0xfffffffffffffull;
+  }
+};
+
+__device__ __forceinline__ void fill_table(double* table) {
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / 64.0);
 }
 
-// One CTA per row; the row is read from memory once per pass.
+// One CTA per row; the row is read from memory once per pass.  Takes the rows that the cluster
+// kernel below has left (their token is kTodo), or every row of a vocabulary that is too large for it.
+constexpr int64_t kTodo = -2;
+
 template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a, bool todo_only) {
+  __shared__ double table[64];
   __shared__ unsigned long long hist[256];
   __shared__ uint32_t count[256];
   __shared__ int64_t warp_buf[32];
@@ -93,6 +131,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
   __shared__ int32_t found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x, V = a.vocab;
+  if (todo_only) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (a.tokens[row] != kTodo) return;
+  }
+  fill_table(table);
   const T* x = static_cast<const T*>(a.logits) + row * a.stride;
   const RowParams rp = row_params(a, row);
   const double one = static_cast<double>(1ull << a.shift);
@@ -131,11 +174,13 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
     return;
   }
   const double t = rp.greedy ? 1.0 : static_cast<double>(rp.t);
-  const auto fixed = [&](double w) { return static_cast<unsigned long long>(__double2ll_rn(w * one)); };
+  Weights weight;
+  weight.set(table, mx, t, a.shift);
+  const auto fixed = [&](double w) { return weight.fixed(w); };
 
   // the whole vocabulary's sum, for the log probability
   unsigned long long mine = 0;
-  for (int i = tid; i < V; i += kSampleThreads) mine += fixed(weight(logit<T>(x[i]), mx, t));
+  for (int i = tid; i < V; i += kSampleThreads) mine += fixed(weight(logit<T>(x[i])));
   block_exclusive_scan_1024(static_cast<int64_t>(mine), warp_buf, &block_total);
   const unsigned long long sum_all = block_total;
   __syncthreads();
@@ -171,12 +216,12 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
   }
   // ---- top-p: where the sum from the top reaches p times the sum ----------------------------
   if (rp.p < 1.f && rp.k > 1) {
-    const unsigned long long w_thr = fixed(weight(float_of(thr), mx, t));
+    const unsigned long long w_thr = fixed(weight(float_of(thr)));
     const bool limited = rp.k < V;
     mine = 0;
     for (int i = tid; i < V; i += kSampleThreads) {
       const float v = logit<T>(x[i]);
-      if (!limited || key_of(v) > thr) mine += fixed(weight(v, mx, t));
+      if (!limited || key_of(v) > thr) mine += fixed(weight(v));
     }
     block_exclusive_scan_1024(static_cast<int64_t>(mine), warp_buf, &block_total);
     unsigned long long total = block_total;
@@ -196,7 +241,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
         const uint32_t key = key_of(v);
         if (limited && key <= thr) continue;
         if (bits == 24 || (key >> (bits + 8)) == prefix) {
-          atomicAdd(&hist[(key >> bits) & 255u], fixed(weight(v, mx, t)));
+          atomicAdd(&hist[(key >> bits) & 255u], fixed(weight(v)));
           atomicAdd(&count[(key >> bits) & 255u], 1u);
         }
       }
@@ -228,7 +273,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
       __syncthreads();
     }
     thr = prefix;
-    const double w = static_cast<double>(fixed(weight(float_of(thr), mx, t)));
+    const double w = static_cast<double>(fixed(weight(float_of(thr))));
     int64_t n = sel_count;
     if (w > 0) n = min(n, static_cast<int64_t>(ceil((target - static_cast<double>(above)) / w)));
     ties = max(n, static_cast<int64_t>(1));
@@ -256,7 +301,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
         __syncthreads();
         unsigned long long w = 0;
         if (i < V && (key > thr || (tie && rank < ties))) {
-          const double wd = weight(v, mx, t);
+          const double wd = weight(v);
           if (wd >= mp) w = fixed(wd);
         }
         const unsigned long long before =
@@ -282,6 +327,620 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
   }
 }
 
+// ---- a cluster of CTAs per row ----------------------------------------------------------------------
+//
+// The CTAs of a cluster hold a row in their shared memory, each a slice, so it is read from memory
+// once; what follows are passes over shared memory, joined through the cluster's.
+//   1. the maximum, while the slice is loaded
+//   2. top-k and top-p: counts of tokens by (max - x) in 2048 steps of 1/64 (of 1/64 t for top-p).
+//      Steps that narrow make the probability of a step known to 0.8 % from its count alone.
+//   3. top-p: the exact sum over all tokens and above the few steps that can hold the border, and of
+//      each of these steps
+//   4. the tokens of the border's step, sorted: the border itself, a token
+//   5. exact sums of the kept tokens in index order, by warp; the warp that holds the draw finds it
+// Where at most kList tokens can be kept after step 2 (top-k), these alone are sorted and 3 to 5
+// done on them.  Rows whose border step holds more than kList tokens (many equal logits) are left
+// to sample_row_kernel.
+constexpr int kClThreads = 512;
+constexpr int kClWarps = kClThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kList = 1024;
+constexpr int kBracket = 64;
+constexpr float kBinScale = 64.f;
+
+struct ClusterShared {
+  uint32_t hist[kBins];
+  unsigned long long bins[kBracket];  // exact sums of the border's steps
+  unsigned long long list[kList];     // key << 32 | ~index (descending: larger logit, lower index first)
+  unsigned long long sums[kList];
+  unsigned long long red[3][kClWarps];
+  double table[64];
+  float warp_x[kClWarps];
+  double warp_d[kClWarps];
+  int32_t warp_i[kClWarps];
+  // of this CTA, for its peers
+  float mx;
+  int32_t mi;
+  unsigned long long total, kept;
+  // rank 0's: sums over the cluster
+  unsigned long long all_total, all_above, sum32;
+  // what rank 0 decides
+  int32_t bin, lo, hi, list_n, state, token;
+  unsigned long long above_bin;
+  uint32_t cut_key;
+  uint32_t cut_idx;
+};
+
+// Sum of a 64-bit integer over the CTA, known to all threads.  `slot`: which of the scratch rows.
+__device__ __forceinline__ unsigned long long cta_sum(unsigned long long v, unsigned long long* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < kClWarps; ++w) v += red[w];
+  return v;
+}
+
+// Descending bitonic sort of n <= kList entries, padded with zeros to a power of two.
+__device__ void sort_list(unsigned long long* v, int n) {
+  int size = 2;
+  while (size < n) size <<= 1;
+  for (int i = n + threadIdx.x; i < size; i += kClThreads) v[i] = 0;
+  __syncthreads();
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int p = threadIdx.x; p < size / 2; p += kClThreads) {
+        const int lo = 2 * p - (p & (j - 1)), hi = lo + j;
+        const bool down = (lo & k) == 0;
+        const unsigned long long a = v[lo], b = v[hi];
+        if ((a < b) == down) {
+          v[lo] = b;
+          v[hi] = a;
+        }
+      }
+      __syncthreads();
+    }
+}
+
+// Exclusive prefix sums of n <= kList entries in place; returns their sum.  Whole CTA.
+__device__ unsigned long long scan_list(unsigned long long* v, int n, unsigned long long* red) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const unsigned long long a = 2 * tid < n ? v[2 * tid] : 0, b = 2 * tid + 1 < n ? v[2 * tid + 1] : 0;
+  unsigned long long x = a + b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long t = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += t;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = x;
+  __syncthreads();
+  unsigned long long before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kClWarps; ++w) {
+    if (w < warp) before += red[w];
+    all += red[w];
+  }
+  const unsigned long long excl = before + x - a - b;
+  if (2 * tid < n) v[2 * tid] = excl;
+  if (2 * tid + 1 < n) v[2 * tid + 1] = excl + a;
+  __syncthreads();
+  return all;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArgs a) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ __align__(16) uint8_t dyn[];
+  ClusterShared& sh = *reinterpret_cast<ClusterShared*>(dyn);
+  uint8_t* buf = dyn + (sizeof(ClusterShared) + 15) / 16 * 16;
+  const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = blockIdx.x / C, V = a.vocab;
+  const int per = (V + C - 1) / C;
+  const int begin = min(V, rank * per), n = min(V, begin + per) - begin;
+  ClusterShared* head = cluster.map_shared_rank(&sh, 0);
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  // ---- 1. load: whole 16-byte pieces where they lie inside the row, single elements at its ends -----
+  const T* x0 = static_cast<const T*>(a.logits) + row * a.stride;
+  const T* src = x0 + begin;
+  const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src) & 15u);
+  const T* s = reinterpret_cast<const T*>(buf + shift);  // s[i]: token begin + i
+  fill_table(sh.table);
+  for (int i = tid; i < kBins; i += kClThreads) sh.hist[i] = 0;
+  if (tid < kBracket) sh.bins[tid] = 0;
+  if (tid == 0) {
+    sh.list_n = 0;
+    sh.state = 0;
+    sh.token = 0x7fffffff;
+    sh.all_total = sh.all_above = sh.sum32 = 0;
+  }
+  float mx = -INFINITY;
+  int mi = V;
+  const auto better = [&](float v, int i) {
+    if (v > mx || (v == mx && i < mi)) {
+      mx = v;
+      mi = i;
+    }
+  };
+  {
+    constexpr int E = 16 / sizeof(T);
+    const uint8_t* aligned = reinterpret_cast<const uint8_t*>(src) - shift;
+    const int pieces = n > 0 ? static_cast<int>((shift + n * sizeof(T) + 15) / 16) : 0;
+    const int first = -static_cast<int>(shift / sizeof(T));  // token (from begin) of the first piece's first
+#pragma unroll 4
+    for (int p = tid; p < pieces; p += kClThreads) {
+      const int i0 = first + p * E;
+      if (begin + i0 >= 0 && begin + i0 + E <= V) {
+        const uint4 u = *reinterpret_cast<const uint4*>(aligned + 16 * p);
+        *reinterpret_cast<uint4*>(buf + 16 * p) = u;
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (i0 + j >= 0 && i0 + j < n) better(logit<T>(e[j]), begin + i0 + j);
+      } else {
+        for (int j = 0; j < E; ++j)
+          if (i0 + j >= 0 && i0 + j < n) {
+            const T v = src[i0 + j];
+            reinterpret_cast<T*>(buf + shift)[i0 + j] = v;
+            better(logit<T>(v), begin + i0 + j);
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    better(__shfl_xor_sync(0xffffffffu, mx, o), __shfl_xor_sync(0xffffffffu, mi, o));
+  if (lane == 0) {
+    sh.warp_x[warp] = mx;
+    sh.warp_i[warp] = mi;
+  }
+  __syncthreads();
+  for (int w = 0; w < kClWarps; ++w) better(sh.warp_x[w], sh.warp_i[w]);
+  if (tid == 0) {
+    sh.mx = mx;
+    sh.mi = mi;
+  }
+  cluster.sync();
+  if (lane < C) {
+    const ClusterShared* o = cluster.map_shared_rank(&sh, lane);
+    better(o->mx, o->mi);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1)
+    better(__shfl_xor_sync(0xffffffffu, mx, o), __shfl_xor_sync(0xffffffffu, mi, o));
+  mx = __shfl_sync(0xffffffffu, mx, 0);
+  mi = __shfl_sync(0xffffffffu, mi, 0);
+
+  const RowParams rp = row_params(a, row);
+  if (!rp.ok || mx == -INFINITY) {
+    if (rank == 0 && tid == 0) {
+      a.tokens[row] = -1;
+      if (a.logprobs) a.logprobs[row] = nanf("");
+      flag_status(a.status, B200_DEVICE_BAD_SAMPLE);
+    }
+    cluster.sync();  // no CTA leaves while its peers read from it
+    return;
+  }
+  const double t = rp.greedy ? 1.0 : static_cast<double>(rp.t);
+  Weights weight;
+  weight.set(sh.table, mx, t, a.shift);
+  const double one = static_cast<double>(1ull << a.shift);
+  const bool top_k = rp.k < V && rp.k > 1, top_p = rp.p < 1.f && rp.k > 1;
+  // each warp's tokens of the slice: [w0, w1), in index order over warps and ranks
+  const int wper = ((n + kClWarps - 1) / kClWarps + 31) & ~31;
+  const int w0 = min(n, warp * wper), w1 = min(n, w0 + wper);
+
+  uint32_t cut_key = 0, cut_idx = 0xffffffffu;  // kept: larger keys, and this key up to this index
+  const auto kept = [&](uint32_t key, uint32_t idx) { return key > cut_key || (key == cut_key && idx <= cut_idx); };
+  const auto bin_of = [&](float v, float scale) {
+    return v == mx ? 0 : static_cast<int>(fminf((mx - v) * scale, static_cast<float>(kBins - 1)));
+  };
+  // w where only the log probability asks for it: exact for the terms above 2^-10, in fp32 (4e-7
+  // off at most, either way) for the many small ones behind them
+  const float c32 = static_cast<float>(1.4426950408889634 / t);
+  const auto sum32 = [&](float v) {
+    const float y = v == mx ? 0.f : (v - mx) * c32;
+    return y > -10.f ? weight(v) : static_cast<double>(fast_exp2(y));
+  };
+  const auto finish = [&](int token, double sum_all) {
+    a.tokens[row] = token;
+    if (a.logprobs) {
+      const float v = logit<T>(x0[token]);
+      const double z = v == mx ? 0.0 : (static_cast<double>(v) - static_cast<double>(mx)) / t;
+      a.logprobs[row] = static_cast<float>(z - log(sum_all));
+    }
+  };
+  // the warps' parts of that sum into rank 0's, in fixed point (so their order does not matter)
+  const auto add_sum32 = [&]() {
+    double all = 0.0;
+    for (int w = 0; w < kClWarps; ++w) all += sh.warp_d[w];
+    atomicAdd(&head->sum32, static_cast<unsigned long long>(all * 0x1p+38));
+  };
+  const auto sum32_all = [&]() { return static_cast<double>(head->sum32) * 0x1p-38; };
+  // counts by step of the kept tokens, summed over the cluster into rank 0's
+  const auto histogram = [&](float scale, bool with_sum) {
+    double part = 0.0;
+    for (int i = w0 + lane; i < w1; i += 32) {
+      const float v = logit<T>(s[i]);
+      if (with_sum) part += sum32(v);
+      if (kept(key_of(v), begin + i)) atomicAdd(&sh.hist[bin_of(v, scale)], 1u);
+    }
+    if (with_sum) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+      if (lane == 0) sh.warp_d[warp] = part;
+    }
+    __syncthreads();
+    if (with_sum && tid == 0) add_sum32();
+    if (rank != 0)
+      for (int i = tid; i < kBins; i += kClThreads)
+        if (sh.hist[i]) atomicAdd(&head->hist[i], sh.hist[i]);
+    cluster.sync();
+  };
+  // tokens of steps [lo, hi] that are kept, into rank 0's list
+  const auto gather = [&](float scale, int lo, int hi) {
+    for (int i = w0 + lane; i < w1; i += 32) {
+      const float v = logit<T>(s[i]);
+      const int b = bin_of(v, scale);
+      const uint32_t key = key_of(v), idx = begin + i;
+      if (b >= lo && b <= hi && kept(key, idx)) {
+        const int at = atomicAdd(&head->list_n, 1);
+        if (at < kList) head->list[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - idx);
+      }
+    }
+    cluster.sync();
+  };
+
+  if (rp.greedy || rp.k == 1) {
+    double part = 0.0;
+    for (int i = w0 + lane; i < w1; i += 32) part += sum32(logit<T>(s[i]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    if (lane == 0) sh.warp_d[warp] = part;
+    __syncthreads();
+    if (tid == 0) add_sum32();
+    cluster.sync();
+    if (rank == 0 && tid == 0) finish(mi, sum32_all());
+    cluster.sync();
+    return;
+  }
+
+  if (top_k) {
+    histogram(kBinScale, true);
+    if (rank == 0) {
+      // the step that holds the k-th token, and how many tokens lie up to it
+      const int per_t = kBins / kClThreads;
+      unsigned long long mine = 0;
+      for (int j = 0; j < per_t; ++j) mine += sh.hist[tid * per_t + j];
+      unsigned long long x = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
+      }
+      if (lane == 31) sh.red[0][warp] = x;
+      __syncthreads();
+      unsigned long long before = x - mine;
+      for (int w = 0; w < warp; ++w) before += sh.red[0][w];
+      const unsigned long long k = static_cast<unsigned long long>(rp.k);
+      for (int j = 0; j < per_t; ++j) {
+        const unsigned long long h = sh.hist[tid * per_t + j];
+        if (before < k && before + h >= k) {
+          sh.bin = tid * per_t + j;
+          sh.above_bin = before;
+          // 1: all tokens up to the step fit in the list; 2: the step's tokens do; 3: neither
+          sh.state = before + h <= kList ? 1 : h <= kList ? 2 : 3;
+        }
+        before += h;
+      }
+    }
+    cluster.sync();
+    const int state = head->state, bin = head->bin;
+    if (state == 3) {
+      if (rank == 0 && tid == 0) a.tokens[row] = kTodo;
+      cluster.sync();
+      return;
+    }
+    gather(kBinScale, state == 1 ? 0 : bin, bin);
+    if (rank == 0) {
+      const int m = sh.list_n;
+      sort_list(sh.list, m);
+      if (state == 1) {
+        // everything else on the list: its first k tokens, their sums in order, in index order
+        const int keep_k = min(m, rp.k);
+        for (int i = tid; i < kList; i += kClThreads)
+          sh.sums[i] = i < keep_k ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32)))) : 0;
+        __syncthreads();
+        const unsigned long long total = scan_list(sh.sums, keep_k, sh.red[0]);
+        const double target = static_cast<double>(rp.p) * static_cast<double>(total);
+        const double mp = static_cast<double>(rp.mp);
+        for (int i = tid; i < m; i += kClThreads) {
+          const unsigned long long e = sh.list[i];
+          const double w = weight(float_of(static_cast<uint32_t>(e >> 32)));
+          const bool in = i < keep_k && (!top_p || i == 0 || static_cast<double>(sh.sums[i]) < target) && w >= mp;
+          // by index; a token that is not kept sorts behind as 0
+          sh.list[i] = in ? (e << 32) | (e >> 32) : 0;
+        }
+        __syncthreads();
+        sort_list(sh.list, m);
+        for (int i = tid; i < kList; i += kClThreads)
+          sh.sums[i] = i < m && sh.list[i] != 0 ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i])))) : 0;
+        __syncthreads();
+        const unsigned long long sum = scan_list(sh.sums, m, sh.red[0]);
+        const unsigned long long goal =
+            static_cast<unsigned long long>(static_cast<double>(rp.u) * static_cast<double>(sum));
+        for (int i = tid; i < m; i += kClThreads) {
+          const unsigned long long after = i + 1 < m ? sh.sums[i + 1] : sum;
+          if (sh.sums[i] <= goal && goal < after) sh.token = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(sh.list[i] >> 32));
+        }
+        __syncthreads();
+        if (tid == 0) finish(sh.token < V ? sh.token : mi, sum32_all());
+      } else if (tid == 0) {
+        const unsigned long long e = sh.list[rp.k - static_cast<int>(sh.above_bin) - 1];
+        sh.cut_key = static_cast<uint32_t>(e >> 32);
+        sh.cut_idx = 0xffffffffu - static_cast<uint32_t>(e);
+      }
+    }
+    cluster.sync();
+    if (state == 1) return;
+    cut_key = head->cut_key;
+    cut_idx = head->cut_idx;
+    cluster.sync();
+  }
+
+  if (top_p) {
+    const float scale = kBinScale / static_cast<float>(t);
+    if (top_k) {  // a second set of counts
+      for (int i = tid; i < kBins; i += kClThreads) sh.hist[i] = 0;
+      if (tid == 0) {
+        sh.list_n = 0;
+        sh.state = 0;
+      }
+      cluster.sync();
+    }
+    histogram(scale, false);
+    if (rank == 0) {
+      // the border's steps: where p times the sum can lie, with a step's sum known to e^(1/64)
+      const int per_t = kBins / kClThreads;
+      double mine[per_t], sum = 0.0;
+      for (int j = 0; j < per_t; ++j) {
+        const int b = tid * per_t + j;
+        mine[j] = sh.hist[b] * exp(-static_cast<double>(b) / 64.0);  // at most this
+        sum += mine[j];
+      }
+      double x = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
+      }
+      if (lane == 31) sh.red[0][warp] = static_cast<unsigned long long>(__double_as_longlong(x));
+      if (tid == 0) {
+        sh.lo = kBins - 1;
+        sh.hi = kBins - 1;
+      }
+      __syncthreads();
+      double before = x - sum, all = 0.0;
+      for (int w = 0; w < kClWarps; ++w) {
+        const double v = __longlong_as_double(static_cast<long long>(sh.red[0][w]));
+        if (w < warp) before += v;
+        all += v;
+      }
+      // A step's true sum lies between e^(-1/64) and 1 times what is counted, but for the last step,
+      // which is open; kLow and kUp leave 1e-5 for bin_of's rounding.  The border is the first step
+      // where the sum from the top reaches p times the whole, and where the sum behind it is at most
+      // 1 - p times the whole: for p near 1 the latter says far more.
+      constexpr double kLow = 0.98447, kUp = 1.00001;
+      const double last = sh.hist[kBins - 1] * exp(-static_cast<double>(kBins - 1) / 64.0);
+      const double p = static_cast<double>(rp.p), most = all * kUp, least = (all - last) * kLow;
+      for (int j = 0; j < per_t; ++j) {
+        const int b = tid * per_t + j;
+        const double after = before + mine[j], tail = fmax(all - after, 0.0);
+        const bool may = after * kUp >= p * least && (tail - last) * kLow <= (1.0 - p) * most;
+        const bool must = (b == kBins - 1 ? 0.0 : after * kLow) >= p * most || tail * kUp + 1e-12 * all <= (1.0 - p) * least;
+        if (may) atomicMin(&sh.lo, b);
+        if (must) atomicMin(&sh.hi, b);
+        before = after;
+      }
+    }
+    cluster.sync();
+    const int lo = head->lo, hi = head->hi;
+    // exact sums: all kept tokens, those above the border's steps, each of these steps
+    unsigned long long total = 0, above = 0;
+    const bool few = hi - lo < kBracket;
+    if (few) {
+      for (int i = w0 + lane; i < w1; i += 32) {
+        const float v = logit<T>(s[i]);
+        if (!kept(key_of(v), begin + i)) continue;
+        const unsigned long long w = weight.fixed(weight(v));
+        const int b = bin_of(v, scale);
+        total += w;
+        if (b < lo) above += w;
+        else if (b <= hi) atomicAdd(&sh.bins[b - lo], w);
+      }
+    }
+    total = cta_sum(total, sh.red[1]);
+    above = cta_sum(above, sh.red[2]);  // its barriers order the steps' sums too
+    if (tid == 0) {
+      atomicAdd(&head->all_total, total);
+      atomicAdd(&head->all_above, above);
+    }
+    if (rank != 0 && few && tid <= hi - lo && sh.bins[tid]) atomicAdd(&head->bins[tid], sh.bins[tid]);
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      unsigned long long up = sh.all_above;
+      const double target = static_cast<double>(rp.p) * static_cast<double>(sh.all_total);
+      int found = -1;
+      if (few && (static_cast<double>(up) < target || up == 0))
+        for (int b = lo; b <= hi; ++b) {
+          const unsigned long long h = sh.bins[b - lo];
+          if (static_cast<double>(up + h) >= target) {
+            found = b;
+            break;
+          }
+          up += h;
+        }
+      sh.bin = found;
+      sh.above_bin = up;
+      sh.state = found >= 0 && sh.hist[found] <= kList ? 2 : 3;
+    }
+    cluster.sync();
+    const int state = head->state, bin = head->bin;
+    if (state == 3) {
+      if (rank == 0 && tid == 0) a.tokens[row] = kTodo;
+      cluster.sync();
+      return;
+    }
+    gather(scale, bin, bin);
+    if (rank == 0) {
+      const int m = sh.list_n;
+      sort_list(sh.list, m);
+      for (int i = tid; i < kList; i += kClThreads)
+        sh.sums[i] = i < m ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32)))) : 0;
+      __syncthreads();
+      scan_list(sh.sums, m, sh.red[0]);
+      const double target = static_cast<double>(rp.p) * static_cast<double>(sh.all_total);
+      for (int i = tid; i < m; i += kClThreads) {
+        const bool in = static_cast<double>(sh.above_bin + sh.sums[i]) < target;
+        const bool next = i + 1 < m && static_cast<double>(sh.above_bin + sh.sums[i + 1]) < target;
+        if (in && !next) {  // the last token that is kept
+          sh.cut_key = static_cast<uint32_t>(sh.list[i] >> 32);
+          sh.cut_idx = 0xffffffffu - static_cast<uint32_t>(sh.list[i]);
+        }
+      }
+    }
+    cluster.sync();
+    cut_key = head->cut_key;
+    cut_idx = head->cut_idx;
+  }
+
+  // ---- 5. draw -----------------------------------------------------------------------------------
+  const double mp = static_cast<double>(rp.mp);
+  const bool filtered = top_k || top_p;
+  unsigned long long mine = 0, all = 0;
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const float v = logit<T>(s[i]);
+    if (filtered && !kept(key_of(v), begin + i)) continue;
+    const double w = weight(v);
+    const unsigned long long f = weight.fixed(w);
+    all += f;
+    if (w >= mp) mine += f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  __syncthreads();
+  if (lane == 0) sh.red[0][warp] = mine;
+  all = cta_sum(all, sh.red[1]);
+  if (tid == 0) {
+    unsigned long long sum = 0;
+    for (int w = 0; w < kClWarps; ++w) sum += sh.red[0][w];
+    sh.kept = sum;
+    sh.total = all;
+  }
+  cluster.sync();
+  unsigned long long before = 0, sum = 0, sum_all = 0;
+  if (lane < C) {
+    const ClusterShared* o = cluster.map_shared_rank(&sh, lane);
+    sum = o->kept;
+    sum_all = o->total;
+    before = lane < rank ? sum : 0;
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    sum_all += __shfl_xor_sync(0xffffffffu, sum_all, o);
+  }
+  before = __shfl_sync(0xffffffffu, before, 0);
+  sum = __shfl_sync(0xffffffffu, sum, 0);
+  sum_all = __shfl_sync(0xffffffffu, sum_all, 0);
+  const unsigned long long goal = static_cast<unsigned long long>(static_cast<double>(rp.u) * static_cast<double>(sum));
+  for (int w = 0; w < warp; ++w) before += sh.red[0][w];
+  if (before <= goal && goal < before + mine) {  // this warp's
+    int token = mi;
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+      const int i = i0 + lane;
+      unsigned long long f = 0;
+      if (i < w1) {
+        const float v = logit<T>(s[i]);
+        if (!filtered || kept(key_of(v), begin + i)) {
+          const double w = weight(v);
+          if (w >= mp) f = weight.fixed(w);
+        }
+      }
+      unsigned long long x = f;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, before + x > goal);
+      if (hit) {
+        token = begin + i0 + __ffs(hit) - 1;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) {
+      // the whole vocabulary's sum: of this pass, or of the top-p's, or (top-k) in fp32
+      const double z = top_k ? sum32_all() : static_cast<double>(top_p ? head->all_total : sum_all) / one;
+      finish(token, z);
+    }
+  }
+  cluster.sync();
+}
+
+// CTAs a row: as many as it takes to make a slice at most 64 KB (two CTAs then fit an SM, and one
+// loads while the other computes: 256 x 128256 fp32 in 8 slices of 64 KB), or 192 KB with 8; more
+// where the rows would leave SMs idle.  0: the vocabulary does not fit.
+int cluster_size(int rows, int vocab, int es, int num_sms) {
+  const int64_t bytes = static_cast<int64_t>(vocab) * es;
+  if ((bytes + 7) / 8 > 192 * 1024) return 0;
+  int c = 1;
+  while (c < 8 && (bytes / c > 64 * 1024 || (rows * c * 2 <= num_sms && bytes / c > 4096))) c *= 2;
+  return c;
+}
+
+template <typename T>
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream) {
+  const int C = cluster_size(a.rows, a.vocab, sizeof(T), num_sms());
+  if (C == 0) {
+    sample_row_kernel<T><<<a.rows, kSampleThreads, 0, stream>>>(a, false);
+    return cudaGetLastError();
+  }
+  const int slice = (a.vocab + C - 1) / C;
+  const size_t smem = (sizeof(ClusterShared) + 15) / 16 * 16 + (static_cast<size_t>(slice) * sizeof(T) + 47) / 16 * 16;
+  cudaError_t e = allow_smem<sample_cluster_kernel<T>>(227 * 1024);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.rows * C);
+  cfg.blockDim = dim3(kClThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, sample_cluster_kernel<T>, a);
+  if (e != cudaSuccess) return e;
+  // the rows that are left; its launch overlaps the cluster kernel's end
+  attr[0] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(a.rows);
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, sample_row_kernel<T>, a, true);
+}
+
 }  // namespace
 
 }  // namespace b200
@@ -303,12 +962,9 @@ extern "C" int b200_sample(const void* logits, int32_t dtype, int64_t stride_row
   while ((1 << bits) < vocab) ++bits;
   a.shift = 62 - bits < 46 ? 62 - bits : 46;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case B200_DTYPE_F32: sample_row_kernel<float><<<rows, kSampleThreads, 0, st>>>(a); break;
-    case B200_DTYPE_BF16: sample_row_kernel<__nv_bfloat16><<<rows, kSampleThreads, 0, st>>>(a); break;
-    default: sample_row_kernel<__half><<<rows, kSampleThreads, 0, st>>>(a); break;
-  }
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = dtype == B200_DTYPE_F32    ? launch_sample<float>(a, st)
+                        : dtype == B200_DTYPE_BF16 ? launch_sample<__nv_bfloat16>(a, st)
+                                                   : launch_sample<__half>(a, st);
   if (e != cudaSuccess) return cuda_fail(e, "sample");
   return B200_OK;
 }
