@@ -78,28 +78,28 @@ __device__ __forceinline__ float float_of(uint32_t key) {
 // 0.0055, remainder below 5e-14.
 struct Weights {
   const double* table;  // 2^(j/64), j < 64, in shared memory
-  double mx, c;         // maximum; 64 log2(e) / t
-  float mxf;
+  double mx, c;         // maximum (an infinite one counts as the largest number); 64 log2(e) / t
   double bias;          // 2^(52 - shift): adding it leaves round(w 2^shift) in the mantissa's low bits
 
   __device__ __forceinline__ void set(const double* tab, float m, double t, int shift) {
     table = tab;
-    mxf = m;
-    mx = static_cast<double>(m);
+    mx = static_cast<double>(fminf(m, 3.402823466e38f));
     c = 64.0 * 1.4426950408889634 / t;
     bias = static_cast<double>(1ull << (52 - shift));
   }
+  // No branches, so that several run in flight.  y is clamped at -3968 (w = 2^-62, which rounds to
+  // 0) by its high word: among negative numbers the larger word is the lower number.
   __device__ __forceinline__ double operator()(float x) const {
-    if (x == mxf) return 1.0;
-    const double y = (static_cast<double>(x) - mx) * c;
-    if (!(y > -3968.0)) return 0.0;  // below 2^-62
+    double y = (static_cast<double>(fminf(x, 3.402823466e38f)) - mx) * c;
+    y = __hiloint2double(static_cast<int>(umin(static_cast<uint32_t>(__double2hiint(y)), 0xC0AF0000u)), __double2loint(y));
     const double v = y + 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are round(y)
     const int n = __double2loint(v);
-    const double f = (y - (v - 6755399441055744.0)) * (0.6931471805599453 / 64.0);
-    double p = fma(f, 1.0 / 24.0, 1.0 / 6.0);
-    p = fma(p, f, 0.5);
-    p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
+    const double r = y - (v - 6755399441055744.0);
+    constexpr double k = 0.6931471805599453 / 64.0;
+    double p = fma(r, k * k * k * k / 24.0, k * k * k / 6.0);
+    p = fma(p, r, k * k / 2.0);
+    p = fma(p, r, k);
+    p = fma(p, r, 1.0);
     const double w = table[n & 63] * p;
     return __hiloint2double(__double2hiint(w) + ((n >> 6) << 20), __double2loint(w));
   }
@@ -345,7 +345,7 @@ constexpr int kClThreads = 512;
 constexpr int kClWarps = kClThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;
-constexpr int kBracket = 64;
+constexpr int kBracket = kClThreads;  // steps that can hold a top-p border: 512, one a thread
 constexpr float kBinScale = 64.f;
 
 struct ClusterShared {
@@ -357,10 +357,8 @@ struct ClusterShared {
   double table[64];
   float warp_x[kClWarps];
   double warp_d[kClWarps];
-  int32_t warp_i[kClWarps];
   // of this CTA, for its peers
   float mx;
-  int32_t mi;
   unsigned long long total, kept;
   // rank 0's: sums over the cluster
   unsigned long long all_total, all_above, sum32;
@@ -431,6 +429,27 @@ __device__ unsigned long long scan_list(unsigned long long* v, int n, unsigned l
   return all;
 }
 
+// The largest logit of 16 bytes, NaN apart (-inf where there is none).
+template <typename T>
+__device__ __forceinline__ float largest_of(uint4 u);
+template <>
+__device__ __forceinline__ float largest_of<float>(uint4 u) {
+  return fmaxf(fmaxf(logit<float>(__uint_as_float(u.x)), logit<float>(__uint_as_float(u.y))),
+               fmaxf(logit<float>(__uint_as_float(u.z)), logit<float>(__uint_as_float(u.w))));
+}
+template <>
+__device__ __forceinline__ float largest_of<__nv_bfloat16>(uint4 u) {
+  const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&u);
+  const __nv_bfloat162 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+  return fmaxf(logit<__nv_bfloat16>(m.x), logit<__nv_bfloat16>(m.y));
+}
+template <>
+__device__ __forceinline__ float largest_of<__half>(uint4 u) {
+  const __half2* v = reinterpret_cast<const __half2*>(&u);
+  const __half2 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+  return fmaxf(logit<__half>(m.x), logit<__half>(m.y));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArgs a) {
   namespace cg = cooperative_groups;
@@ -453,7 +472,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
   const T* s = reinterpret_cast<const T*>(buf + shift);  // s[i]: token begin + i
   fill_table(sh.table);
   for (int i = tid; i < kBins; i += kClThreads) sh.hist[i] = 0;
-  if (tid < kBracket) sh.bins[tid] = 0;
+  sh.bins[tid] = 0;
   if (tid == 0) {
     sh.list_n = 0;
     sh.state = 0;
@@ -461,61 +480,39 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
     sh.all_total = sh.all_above = sh.sum32 = 0;
   }
   float mx = -INFINITY;
-  int mi = V;
-  const auto better = [&](float v, int i) {
-    if (v > mx || (v == mx && i < mi)) {
-      mx = v;
-      mi = i;
-    }
-  };
   {
     constexpr int E = 16 / sizeof(T);
     const uint8_t* aligned = reinterpret_cast<const uint8_t*>(src) - shift;
     const int pieces = n > 0 ? static_cast<int>((shift + n * sizeof(T) + 15) / 16) : 0;
-    const int first = -static_cast<int>(shift / sizeof(T));  // token (from begin) of the first piece's first
+    const int first = begin - static_cast<int>(shift / sizeof(T));  // token of the first piece's first
 #pragma unroll 4
     for (int p = tid; p < pieces; p += kClThreads) {
       const int i0 = first + p * E;
-      if (begin + i0 >= 0 && begin + i0 + E <= V) {
+      if (i0 >= 0 && i0 + E <= V) {  // (a piece at the slice's end may hold tokens of the next one's)
         const uint4 u = *reinterpret_cast<const uint4*>(aligned + 16 * p);
         *reinterpret_cast<uint4*>(buf + 16 * p) = u;
-        const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (i0 + j >= 0 && i0 + j < n) better(logit<T>(e[j]), begin + i0 + j);
+        mx = fmaxf(mx, largest_of<T>(u));
       } else {
         for (int j = 0; j < E; ++j)
-          if (i0 + j >= 0 && i0 + j < n) {
-            const T v = src[i0 + j];
-            reinterpret_cast<T*>(buf + shift)[i0 + j] = v;
-            better(logit<T>(v), begin + i0 + j);
+          if (i0 + j >= begin && i0 + j < begin + n) {
+            const T v = x0[i0 + j];
+            reinterpret_cast<T*>(buf)[p * E + j] = v;
+            mx = fmaxf(mx, logit<T>(v));
           }
       }
     }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    better(__shfl_xor_sync(0xffffffffu, mx, o), __shfl_xor_sync(0xffffffffu, mi, o));
-  if (lane == 0) {
-    sh.warp_x[warp] = mx;
-    sh.warp_i[warp] = mi;
-  }
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) sh.warp_x[warp] = mx;
   __syncthreads();
-  for (int w = 0; w < kClWarps; ++w) better(sh.warp_x[w], sh.warp_i[w]);
-  if (tid == 0) {
-    sh.mx = mx;
-    sh.mi = mi;
-  }
+  for (int w = 0; w < kClWarps; ++w) mx = fmaxf(mx, sh.warp_x[w]);
+  if (tid == 0) sh.mx = mx;
   cluster.sync();
-  if (lane < C) {
-    const ClusterShared* o = cluster.map_shared_rank(&sh, lane);
-    better(o->mx, o->mi);
-  }
+  if (lane < C) mx = cluster.map_shared_rank(&sh, lane)->mx;
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1)
-    better(__shfl_xor_sync(0xffffffffu, mx, o), __shfl_xor_sync(0xffffffffu, mi, o));
+  for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   mx = __shfl_sync(0xffffffffu, mx, 0);
-  mi = __shfl_sync(0xffffffffu, mi, 0);
 
   const RowParams rp = row_params(a, row);
   if (!rp.ok || mx == -INFINITY) {
@@ -599,14 +596,20 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
 
   if (rp.greedy || rp.k == 1) {
     double part = 0.0;
-    for (int i = w0 + lane; i < w1; i += 32) part += sum32(logit<T>(s[i]));
+    int best = V;
+    for (int i = w0 + lane; i < w1; i += 32) {
+      const float v = logit<T>(s[i]);
+      part += sum32(v);
+      if (v == mx) best = min(best, begin + i);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
     if (lane == 0) sh.warp_d[warp] = part;
+    if (best < V) atomicMin(&head->token, best);
     __syncthreads();
     if (tid == 0) add_sum32();
     cluster.sync();
-    if (rank == 0 && tid == 0) finish(mi, sum32_all());
+    if (rank == 0 && tid == 0) finish(sh.token, sum32_all());
     cluster.sync();
     return;
   }
@@ -641,7 +644,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
       }
     }
     cluster.sync();
-    const int state = head->state, bin = head->bin;
+    const int state = head->state, bin = head->bin;  // 3: left to sample_row_kernel
     if (state == 3) {
       if (rank == 0 && tid == 0) a.tokens[row] = kTodo;
       cluster.sync();
@@ -680,7 +683,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
           if (sh.sums[i] <= goal && goal < after) sh.token = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(sh.list[i] >> 32));
         }
         __syncthreads();
-        if (tid == 0) finish(sh.token < V ? sh.token : mi, sum32_all());
+        if (tid == 0) finish(sh.token, sum32_all());
       } else if (tid == 0) {
         const unsigned long long e = sh.list[rp.k - static_cast<int>(sh.above_bin) - 1];
         sh.cut_key = static_cast<uint32_t>(e >> 32);
@@ -773,22 +776,22 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
     }
     if (rank != 0 && few && tid <= hi - lo && sh.bins[tid]) atomicAdd(&head->bins[tid], sh.bins[tid]);
     cluster.sync();
-    if (rank == 0 && tid == 0) {
-      unsigned long long up = sh.all_above;
+    if (rank == 0) {
+      const int steps = few ? hi - lo + 1 : 0;
+      const unsigned long long h = tid < steps ? sh.bins[tid] : 0;
+      sh.sums[tid] = h;
+      if (tid == 0) sh.state = 3;
+      __syncthreads();
+      scan_list(sh.sums, kClThreads, sh.red[0]);
       const double target = static_cast<double>(rp.p) * static_cast<double>(sh.all_total);
-      int found = -1;
-      if (few && (static_cast<double>(up) < target || up == 0))
-        for (int b = lo; b <= hi; ++b) {
-          const unsigned long long h = sh.bins[b - lo];
-          if (static_cast<double>(up + h) >= target) {
-            found = b;
-            break;
-          }
-          up += h;
-        }
-      sh.bin = found;
-      sh.above_bin = up;
-      sh.state = found >= 0 && sh.hist[found] <= kList ? 2 : 3;
+      const unsigned long long up = sh.all_above + sh.sums[tid];
+      // the border's step: the first one that reaches the target (step lo where rounding left it just
+      // behind)
+      if (tid < steps && (static_cast<double>(up) < target || tid == 0) && static_cast<double>(up + h) >= target) {
+        sh.bin = lo + tid;
+        sh.above_bin = up;
+        sh.state = sh.hist[lo + tid] <= kList ? 2 : 3;
+      }
     }
     cluster.sync();
     const int state = head->state, bin = head->bin;
@@ -824,13 +827,20 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
   const double mp = static_cast<double>(rp.mp);
   const bool filtered = top_k || top_p;
   unsigned long long mine = 0, all = 0;
-  for (int i = w0 + lane; i < w1; i += 32) {
-    const float v = logit<T>(s[i]);
-    if (filtered && !kept(key_of(v), begin + i)) continue;
-    const double w = weight(v);
-    const unsigned long long f = weight.fixed(w);
-    all += f;
-    if (w >= mp) mine += f;
+  if (!filtered && mp <= 0.0) {
+#pragma unroll 4
+    for (int i = w0 + lane; i < w1; i += 32) mine += weight.fixed(weight(logit<T>(s[i])));
+    all = mine;
+  } else {
+#pragma unroll 2
+    for (int i = w0 + lane; i < w1; i += 32) {
+      const float v = logit<T>(s[i]);
+      if (filtered && !kept(key_of(v), begin + i)) continue;
+      const double w = weight(v);
+      const unsigned long long f = weight.fixed(w);
+      all += f;
+      if (w >= mp) mine += f;
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -861,33 +871,46 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
   sum = __shfl_sync(0xffffffffu, sum, 0);
   sum_all = __shfl_sync(0xffffffffu, sum_all, 0);
   const unsigned long long goal = static_cast<unsigned long long>(static_cast<double>(rp.u) * static_cast<double>(sum));
-  for (int w = 0; w < warp; ++w) before += sh.red[0][w];
-  if (before <= goal && goal < before + mine) {  // this warp's
-    int token = mi;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-      const int i = i0 + lane;
-      unsigned long long f = 0;
-      if (i < w1) {
-        const float v = logit<T>(s[i]);
-        if (!filtered || kept(key_of(v), begin + i)) {
-          const double w = weight(v);
-          if (w >= mp) f = weight.fixed(w);
+  // the warp's part that holds the draw, if it is one of this CTA's: all threads look through it
+  int part = -1;
+  for (int w = 0; w < kClWarps; ++w) {
+    const unsigned long long m = sh.red[0][w];
+    if (part < 0) {
+      if (before <= goal && goal < before + m) part = w;
+      else before += m;
+    }
+  }
+  if (part >= 0) {
+    const int p0 = min(n, part * wper), p1 = min(n, p0 + wper);
+    const int each = (p1 - p0 + kClThreads - 1) / kClThreads;
+    const int i0 = min(p1, p0 + tid * each), i1 = min(p1, i0 + each);
+    const auto counts = [&](int i) -> unsigned long long {
+      const float v = logit<T>(s[i]);
+      if (filtered && !kept(key_of(v), begin + i)) return 0;
+      const double w = weight(v);
+      return w >= mp ? weight.fixed(w) : 0;
+    };
+    unsigned long long own = 0;
+    for (int i = i0; i < i1; ++i) own += counts(i);
+    unsigned long long x = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long u = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += u;
+    }
+    if (lane == 31) sh.red[1][warp] = x;
+    __syncthreads();
+    before += x - own;
+    for (int w = 0; w < warp; ++w) before += sh.red[1][w];
+    if (before <= goal && goal < before + own) {
+      int token = V;
+      for (int i = i0; i < i1; ++i) {
+        before += counts(i);
+        if (before > goal) {
+          token = begin + i;
+          break;
         }
       }
-      unsigned long long x = f;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long u = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += u;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, before + x > goal);
-      if (hit) {
-        token = begin + i0 + __ffs(hit) - 1;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, x, 31);
-    }
-    if (lane == 0) {
       // the whole vocabulary's sum: of this pass, or of the top-p's, or (top-k) in fp32
       const double z = top_k ? sum32_all() : static_cast<double>(top_p ? head->all_total : sum_all) / one;
       finish(token, z);
@@ -896,14 +919,14 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
   cluster.sync();
 }
 
-// CTAs a row: as many as it takes to make a slice at most 64 KB (two CTAs then fit an SM, and one
-// loads while the other computes: 256 x 128256 fp32 in 8 slices of 64 KB), or 192 KB with 8; more
-// where the rows would leave SMs idle.  0: the vocabulary does not fit.
+// CTAs a row: enough to make a slice at most 16384 tokens and 64 KB (two CTAs fit an SM, and one
+// loads while the other computes), but 8 at most (192 KB of tokens each); more where the rows would
+// leave SMs idle.  0: the vocabulary does not fit.
 int cluster_size(int rows, int vocab, int es, int num_sms) {
   const int64_t bytes = static_cast<int64_t>(vocab) * es;
   if ((bytes + 7) / 8 > 192 * 1024) return 0;
   int c = 1;
-  while (c < 8 && (bytes / c > 64 * 1024 || (rows * c * 2 <= num_sms && bytes / c > 4096))) c *= 2;
+  while (c < 8 && (vocab / c > 16384 || bytes / c > 64 * 1024 || (rows * c * 2 <= num_sms && vocab / c > 1024))) c *= 2;
   return c;
 }
 
