@@ -608,9 +608,8 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
     if (best < V) atomicMin(&head->token, best);
     __syncthreads();
     if (tid == 0) add_sum32();
-    cluster.sync();
+    cluster.sync();  // rank 0 goes on with what it holds; its peers are done
     if (rank == 0 && tid == 0) finish(sh.token, sum32_all());
-    cluster.sync();
     return;
   }
 
@@ -651,6 +650,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
       return;
     }
     gather(kBinScale, state == 1 ? 0 : bin, bin);
+    if (state == 1 && rank != 0) return;  // rank 0 has all that is left
     if (rank == 0) {
       const int m = sh.list_n;
       sort_list(sh.list, m);
@@ -690,8 +690,8 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
         sh.cut_idx = 0xffffffffu - static_cast<uint32_t>(e);
       }
     }
-    cluster.sync();
     if (state == 1) return;
+    cluster.sync();
     cut_key = head->cut_key;
     cut_idx = head->cut_idx;
     cluster.sync();
@@ -871,6 +871,9 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
   sum = __shfl_sync(0xffffffffu, sum, 0);
   sum_all = __shfl_sync(0xffffffffu, sum_all, 0);
   const unsigned long long goal = static_cast<unsigned long long>(static_cast<double>(rp.u) * static_cast<double>(sum));
+  // the whole vocabulary's sum: of this pass, or of the top-p's, or (top-k) of the first
+  const double z = top_k ? sum32_all() : static_cast<double>(top_p ? head->all_total : sum_all) / one;
+  cluster.sync();  // from here on each CTA reads its own memory only, and may end
   // the warp's part that holds the draw, if it is one of this CTA's: all threads look through it
   int part = -1;
   for (int w = 0; w < kClWarps; ++w) {
@@ -911,12 +914,9 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
           break;
         }
       }
-      // the whole vocabulary's sum: of this pass, or of the top-p's, or (top-k) in fp32
-      const double z = top_k ? sum32_all() : static_cast<double>(top_p ? head->all_total : sum_all) / one;
       finish(token, z);
     }
   }
-  cluster.sync();
 }
 
 // CTAs a row: enough to make a slice at most 16384 tokens and 64 KB (two CTAs fit an SM, and one
