@@ -5,7 +5,9 @@ The package directory name is not a Python identifier, so it is imported under t
 
 Submodules:
   _native            ctypes binding of the C-ABI library libb200paged.so (include/b200_paged.h)
-  paged_ops          torch-tensor front end of the C ABI (decode, prefill, cache writes, copies)
+  paged_ops          torch-tensor front end of the C ABI (decode, prefill, cache writes, copies; the
+                     same over an 8-bit cache)
+  sampling           temperature, top-k, top-p and min-p sampling by given random numbers
   llm_allocator_cpp  drop-in for the reference's pybind module of the same name
   block_manager      device-resident FIFO block pool and per-sequence block tables
   kv_cache           paged KV store on the device (reshape_and_cache, slot mapping, block tables,

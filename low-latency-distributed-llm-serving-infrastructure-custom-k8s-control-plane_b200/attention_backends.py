@@ -61,7 +61,20 @@ class NativePagedBackend(AttentionBackend):
         q = query[0].transpose(0, 1)  # (Nq, Hq, D) view
         if q.stride(-1) != 1:
             q = q.contiguous()
-        if context.is_decode:
+        if getattr(store, "is_fp8", False):
+            if context.is_decode:
+                out = paged_ops.paged_decode_fp8(q, *store.arrays, layer_idx, context.block_tables,
+                                                 context.context_lens_device, scaling,
+                                                 context.max_context_len)
+            else:
+                blocks = sum(-(-c // store.block_size) for c, n in
+                             zip(context.context_lens, context.new_token_counts) if n > 1)
+                out = paged_ops.paged_prefill_fp8(q, *store.arrays, layer_idx, context.block_tables,
+                                                  context.cu_seqlens_device,
+                                                  context.context_lens_device, scaling,
+                                                  context.max_query_len, context.max_context_len,
+                                                  prefill_blocks=blocks)
+        elif context.is_decode:
             out = paged_ops.paged_decode(q, store.key_cache, store.value_cache, layer_idx,
                                          context.block_tables, context.context_lens_device,
                                          scaling, context.max_context_len)

@@ -10,8 +10,12 @@ Scheduling policy and engine API follow the reference:
     has_unfinished_requests).
 Differences that are the point of the rebuild: block allocation goes to the device block pool
 (K5), the step's metadata is built on the device (K4), the prefill and decode groups run as one
-mixed forward, and sampling is a greedy argmax on the device with one host read per step
-(instead of one ``int(argmax)`` per sequence, llm_engine.py:200-204).
+mixed forward, and sampling runs on the device with one host read per step (instead of one
+``int(argmax)`` per sequence, llm_engine.py:200-204): a greedy argmax, or, in steps with a request
+that asks for it (``SamplingParams``), temperature, top-k, top-p and min-p for every row by its own
+parameters.  A request's random numbers come from its seed and the index of the output token, so
+they do not depend on the batch it runs in, on preemption or on the tensor-parallel size.
+The KV cache may be 8 bits wide (``build_engine(kv_dtype=torch.float8_e4m3fn)``).
 
 Pure decode steps replay a CUDA graph captured per batch-size bucket (step metadata, the whole
 model forward with the fused rotary/cache-write and decode kernels, greedy sampling): the host
@@ -32,11 +36,13 @@ from dataclasses import dataclass
 from enum import Enum
 from typing import Dict, List, Optional
 
+import numpy as np
 import torch
 
 from . import _native as N
-from . import paged_ops
+from . import paged_ops, sampling
 from .kv_cache import PagedKVCacheManager
+from .sampling import SamplingParams
 
 
 class SequenceStatus(Enum):
@@ -47,7 +53,8 @@ class SequenceStatus(Enum):
 
 class Sequence:
     def __init__(self, seq_id: int, prompt_token_ids: List[int], max_tokens: int = 128,
-                 eos_token_id: Optional[int] = None) -> None:
+                 eos_token_id: Optional[int] = None,
+                 sampling: Optional[SamplingParams] = None) -> None:
         if not prompt_token_ids:
             raise ValueError(f"Sequence {seq_id}: Prompt and prompt_token_ids cannot be both empty.")
         self.seq_id = seq_id
@@ -55,6 +62,7 @@ class Sequence:
         self.output_token_ids: List[int] = []
         self.max_tokens = max_tokens
         self.eos_token_id = eos_token_id
+        self.sampling = sampling  # None: greedy
         self.status = SequenceStatus.WAITING
         self.block_table = None
         self.arrival = 0.0
@@ -205,11 +213,59 @@ def graph_decode_workspace_bytes(num_query_heads: int, key_cache: torch.Tensor,
     return need
 
 
-class _DecodeGraph:
-    """Static buffers and the captured graph of one decode bucket (``rows`` sequences)."""
+def graph_decode_fp8_workspace_bytes(num_query_heads: int, arrays, max_blocks_per_seq: int,
+                                     ctx_bound: int, max_rows: int, scale: float,
+                                     dtype: torch.dtype) -> int:
+    """``graph_decode_workspace_bytes`` for an 8-bit cache (``arrays``: caches and scales) and
+    queries of ``dtype``."""
+    L = N.lib()
+    dev = arrays[0].device
+    q = torch.empty((max_rows, num_query_heads, arrays[0].shape[-1]), dtype=dtype, device=dev)
+    bt = torch.empty((max_rows, max_blocks_per_seq), dtype=torch.int32, device=dev)
+    ctx = torch.empty(max_rows, dtype=torch.int32, device=dev)
+    need = 256
+    for rows in _GRAPH_BUCKETS:
+        if rows > max_rows:
+            break
+        p = paged_ops.attention_fp8_params(q[:rows], *arrays, 0, bt[:rows], ctx[:rows], scale,
+                                           q[:rows], ctx_bound)
+        need = max(need, int(L.b200_paged_decode_fp8_workspace_bytes(ctypes.byref(p))))
+    return need
 
-    def __init__(self, rows: int, device: torch.device) -> None:
+
+def uniforms(seeds, indices) -> np.ndarray:
+    """One uniform number in [0, 1) per (seed, index): 24 bits of a 64-bit mix of the two (the
+    splitmix64 finaliser, Steele et al. 2014), so any number of a request's sequence can be had
+    by itself."""
+    with np.errstate(over="ignore"):
+        z = (np.asarray(seeds, dtype=np.uint64) * np.uint64(0xD1342543DE82EF95)
+             + np.asarray(indices, dtype=np.uint64) + np.uint64(1)) * np.uint64(0x9E3779B97F4A7C15)
+        z = (z ^ (z >> np.uint64(30))) * np.uint64(0xBF58476D1CE4E5B9)
+        z = (z ^ (z >> np.uint64(27))) * np.uint64(0x94D049BB133111EB)
+        z = z ^ (z >> np.uint64(31))
+    return ((z >> np.uint64(40)).astype(np.float64) * 2.0 ** -24).astype(np.float32)
+
+
+def sampling_rows(seqs: List[Sequence], floats: np.ndarray, top_k: np.ndarray) -> None:
+    """Fills the sampling inputs of a step: ``floats`` (4, rows) with uniform, temperature, top-p
+    and min-p, ``top_k`` (rows,).  Greedy requests have temperature 0."""
+    n = len(seqs)
+    params = [s.sampling for s in seqs]
+    floats[0, :n] = uniforms([p.seed & 0xFFFFFFFFFFFFFFFF if p else 0 for p in params],
+                             [len(s.output_token_ids) for s in seqs])
+    floats[1, :n] = [p.temperature if p else 0.0 for p in params]
+    floats[2, :n] = [p.top_p if p else 1.0 for p in params]
+    floats[3, :n] = [p.min_p if p else 0.0 for p in params]
+    top_k[:n] = [min(p.top_k, 0x7FFFFFFF) if p else 0 for p in params]
+
+
+class _DecodeGraph:
+    """Static buffers and the captured graph of one decode bucket (``rows`` sequences);
+    ``sampled``: its tokens are drawn, not the greedy ones."""
+
+    def __init__(self, rows: int, device: torch.device, sampled: bool = False) -> None:
         self.rows = rows
+        self.sampled = sampled
         # rows of (sequence slot, start position, new-token count) and the input token ids
         self.h_meta = torch.zeros((3, rows), dtype=torch.int32).pin_memory()
         self.h_ids = torch.zeros(rows, dtype=torch.int64).pin_memory()
@@ -217,6 +273,13 @@ class _DecodeGraph:
         self.h_ids_np = self.h_ids.numpy()
         self.d_meta = torch.zeros((3, rows), dtype=torch.int32, device=device)
         self.d_ids = torch.zeros(rows, dtype=torch.int64, device=device)
+        if sampled:
+            # rows of (uniform, temperature, top-p, min-p), and top-k
+            self.h_samp = torch.zeros((4, rows)).pin_memory()
+            self.h_topk = torch.zeros(rows, dtype=torch.int32).pin_memory()
+            self.h_samp_np, self.h_topk_np = self.h_samp.numpy(), self.h_topk.numpy()
+            self.d_samp = torch.zeros((4, rows), device=device)
+            self.d_topk = torch.zeros(rows, dtype=torch.int32, device=device)
         self.graph = torch.cuda.CUDAGraph()
         self.out: Optional[torch.Tensor] = None
 
@@ -235,7 +298,7 @@ class Engine:
         self.prefill_tokens = 0
         self.graph_steps = 0
         self.cuda_graphs = cuda_graphs
-        self._graphs: Dict[int, _DecodeGraph] = {}
+        self._graphs: Dict[tuple, _DecodeGraph] = {}  # by (rows, sampled)
         self._graph_pool = None
         self._graph_ws: Optional[torch.Tensor] = None
         # decode graphs size their split plan and workspace for this context bound
@@ -244,9 +307,11 @@ class Engine:
                               _GRAPH_BUCKETS[-1])
 
     def add_request(self, prompt_token_ids: List[int], max_tokens: int = 128,
-                    eos_token_id: Optional[int] = None, arrival: float = 0.0) -> Sequence:
+                    eos_token_id: Optional[int] = None, arrival: float = 0.0,
+                    sampling: Optional[SamplingParams] = None) -> Sequence:
+        """``sampling``: how the request's tokens are drawn (None: greedy)."""
         self.seq_counter += 1
-        seq = Sequence(self.seq_counter, prompt_token_ids, max_tokens, eos_token_id)
+        seq = Sequence(self.seq_counter, prompt_token_ids, max_tokens, eos_token_id, sampling)
         seq.arrival = arrival
         self.scheduler.add_sequence(seq)
         return seq
@@ -297,6 +362,9 @@ class Engine:
             nvtx.range_pop()
         now = time.perf_counter()
         for s, t in zip(seqs, next_tokens):
+            if t < 0:
+                raise RuntimeError(f"Sequence {s.seq_id}: no token can be drawn (its logits are "
+                                   "all NaN or -inf)")
             if s.first_token_time is None:
                 s.first_token_time = now
             s.append_token(int(t))
@@ -330,6 +398,8 @@ class Engine:
         is_decode = not out.scheduled_prefills
         max_q = max(counts)
         max_ctx = max(s + c for s, c in zip(starts, counts))
+        bs = self.kv.block_size
+        prefill_blocks = sum((s + c + bs - 1) // bs for s, c in zip(starts, counts) if c > 1)
         kc, vc = self.kv.key_cache, self.kv.value_cache
         bt, ctx, cu = md["block_tables"], md["context_lens"], md["cu_seqlens"]
         slots = md["slot_mapping"]
@@ -337,6 +407,14 @@ class Engine:
         positions = md["position_ids"]
         inv_freq = self.model.inv_freq
         hq = self.model.hq
+
+        def attend_qkv_fp8(layer, qkv):
+            cache = (*self.kv.arrays, layer)
+            q = paged_ops.rope_reshape_and_cache_fp8(qkv, positions, inv_freq, hq, *cache, slots)
+            if is_decode:
+                return paged_ops.paged_decode_fp8(q, *cache, bt, ctx, scale, max_ctx)
+            return paged_ops.paged_prefill_fp8(q, *cache, bt, cu, ctx, scale, max_q, max_ctx,
+                                               prefill_blocks=prefill_blocks)
 
         def attend_qkv(layer, qkv):
             # rotary + cache write in one kernel, then attention over the paged cache
@@ -347,9 +425,16 @@ class Engine:
             return paged_ops.paged_prefill(q, kc, vc, layer, bt, cu, ctx, scale, max_q, max_ctx)
 
         with torch.inference_mode():
-            hidden = self.model.forward(input_ids, positions, attend_qkv=attend_qkv)
+            hidden = self.model.forward(input_ids, positions,
+                                        attend_qkv=attend_qkv_fp8 if self.kv.is_fp8 else attend_qkv)
             last = hidden.index_select(0, cu[1:] - 1)
-            return self.model.greedy(last).cpu().tolist()
+            if not any(s.sampling for s in seqs):
+                return self.model.greedy(last).cpu().tolist()
+            samp, top_k = torch.empty((4, len(seqs))), torch.empty(len(seqs), dtype=torch.int32)
+            sampling_rows(seqs, samp.numpy(), top_k.numpy())
+            u, t, p, m = samp.to(dev)
+            return sampling.sample(self.model.logits(last), u, t, top_k.to(dev), p,
+                                   m)[0].cpu().tolist()
 
     # ---- captured decode step --------------------------------------------------------------------
     def _decode_body(self, g: _DecodeGraph) -> torch.Tensor:
@@ -364,17 +449,32 @@ class Engine:
         inv_freq, hq, scale = self.model.inv_freq, self.model.hq, self.scale
         bound, ws = self._ctx_bound, self._graph_ws
 
+        def attend_qkv_fp8(layer, qkv):
+            cache = (*self.kv.arrays, layer)
+            q = paged_ops.rope_reshape_and_cache_fp8(qkv, positions, inv_freq, hq, *cache, slots)
+            return paged_ops.paged_decode_fp8(q, *cache, bt, ctx, scale, bound, workspace=ws)
+
         def attend_qkv(layer, qkv):
             q = paged_ops.rope_reshape_and_cache(qkv, positions, inv_freq, hq, kc, vc, slots,
                                                  layer)
             return paged_ops.paged_decode(q, kc, vc, layer, bt, ctx, scale, bound, workspace=ws)
 
-        hidden = self.model.forward(g.d_ids, positions, attend_qkv=attend_qkv)
-        return self.model.greedy(hidden)
+        hidden = self.model.forward(g.d_ids, positions,
+                                    attend_qkv=attend_qkv_fp8 if self.kv.is_fp8 else attend_qkv)
+        if not g.sampled:
+            return self.model.greedy(hidden)
+        u, t, p, m = g.d_samp
+        return sampling.sample(self.model.logits(hidden), u, t, g.d_topk, p, m)[0]
 
     def _graph_workspace(self) -> torch.Tensor:
         """Decode workspace shared by every captured graph (graphs never run concurrently), sized
         once for every bucket at the context bound so no capture ever reallocates it."""
+        if self._graph_ws is None and self.kv.is_fp8:
+            need = graph_decode_fp8_workspace_bytes(self.model.hq, self.kv.arrays,
+                                                    self.kv.pool.max_blocks_per_seq,
+                                                    self._ctx_bound, self._max_rows, self.scale,
+                                                    self.model.dtype)
+            self._graph_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         if self._graph_ws is None:
             need = graph_decode_workspace_bytes(self.model.hq, self.kv.key_cache,
                                                 self.kv.value_cache,
@@ -388,10 +488,11 @@ class Engine:
         rows = next((b for b in _GRAPH_BUCKETS if b >= B), None)
         if rows is None or rows > self._max_rows:
             return None
-        g = self._graphs.get(rows)
+        sampled = any(s.sampling for s in decodes)
+        g = self._graphs.get((rows, sampled))
         fresh = g is None
         if fresh:
-            g = _DecodeGraph(rows, self.device)
+            g = _DecodeGraph(rows, self.device, sampled)
         tokens = [s.block_table.get_tokens_count() for s in decodes]
         donor = min(range(B), key=lambda i: tokens[i])  # pad rows repeat the shortest sequence
         m, ids = g.h_meta_np, g.h_ids_np
@@ -403,6 +504,12 @@ class Engine:
         m[1, B:] = m[1, donor]
         m[2, :] = 1
         ids[B:] = ids[donor]
+        if sampled:
+            sampling_rows(decodes, g.h_samp_np, g.h_topk_np)
+            g.h_samp_np[:, B:] = g.h_samp_np[:, donor:donor + 1]
+            g.h_topk_np[B:] = g.h_topk_np[donor]
+            g.d_samp.copy_(g.h_samp, non_blocking=True)
+            g.d_topk.copy_(g.h_topk, non_blocking=True)
         self.kv.pool.flush()  # this step's slot allocations, before the metadata kernel reads them
         g.d_meta.copy_(g.h_meta, non_blocking=True)
         g.d_ids.copy_(g.h_ids, non_blocking=True)
@@ -429,19 +536,22 @@ class Engine:
             self._graph_pool = torch.cuda.graph_pool_handle()
         with torch.inference_mode(), torch.cuda.graph(g.graph, pool=self._graph_pool):
             g.out = self._decode_body(g)
-        self._graphs[g.rows] = g
+        self._graphs[(g.rows, g.sampled)] = g
 
 
 def build_engine(shape, total_blocks: int, block_size: int = 16, rank: int = 0, world: int = 1,
                  device=None, dtype=torch.bfloat16, seed: int = 0, max_batch_size: int = 256,
                  max_num_batched_tokens: int = 16384, max_model_len: int = 8192,
-                 full_init: bool = False, group=None, cuda_graphs: bool = True) -> Engine:
+                 full_init: bool = False, group=None, cuda_graphs: bool = True,
+                 kv_dtype: Optional[torch.dtype] = None) -> Engine:
+    """``kv_dtype``: the KV cache's type where it is not the model's; torch.float8_e4m3fn holds it
+    in 8 bits."""
     from .model import TPLlama
     device = torch.device(device or "cuda")
     model = TPLlama(shape, rank, world, device, dtype, seed, full_init=full_init, group=group)
     max_blocks = (max_model_len + block_size - 1) // block_size
     kv = PagedKVCacheManager(total_blocks, block_size, shape.num_kv_heads // world,
-                             shape.head_dim, dtype=dtype, num_layers=shape.num_layers,
+                             shape.head_dim, dtype=kv_dtype or dtype, num_layers=shape.num_layers,
                              device=device, max_seqs=max(16 * max_batch_size, 4096),
                              max_blocks_per_seq=max_blocks)
     sched = Scheduler(kv, max_batch_size, max_num_batched_tokens, max_model_len)

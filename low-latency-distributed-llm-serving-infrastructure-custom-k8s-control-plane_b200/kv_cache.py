@@ -5,6 +5,10 @@ Scheduler and engine drive it unchanged; underneath, block allocation goes to th
 pool (K5), slot mappings and block tables come from the metadata kernels (K4) and the KV write is
 reshape_and_cache (K2).  The caches are ``(L, NB, BS, Hkv, D)`` tensors on the GPU
 (app/memory/strategies.py:110-115).
+
+With ``dtype=torch.float8_e4m3fn`` the caches hold 8-bit codes and the manager has ``key_scale`` and
+``value_scale``, one fp32 power of two per (layer, block, head); writes, reads and block copies then
+go through the 8-bit forms.
 """
 from __future__ import annotations
 
@@ -77,7 +81,22 @@ class PagedKVCacheManager:
         shape = (num_layers, total_blocks, block_size, num_heads, head_dim)
         self.key_cache = torch.empty(shape, dtype=dtype, device=dev)
         self.value_cache = torch.empty(shape, dtype=dtype, device=dev)
+        self.key_scale = self.value_scale = None
+        if self.is_fp8:  # 0: never written
+            self.key_scale = torch.zeros((num_layers, total_blocks, num_heads), device=dev)
+            self.value_scale = torch.zeros((num_layers, total_blocks, num_heads), device=dev)
         self._free_slots = list(range(max_seqs - 1, -1, -1))
+
+    @property
+    def is_fp8(self) -> bool:
+        return self.dtype == torch.float8_e4m3fn
+
+    @property
+    def arrays(self):
+        """(key cache, value cache), and with an 8-bit cache its (key scale, value scale)."""
+        if self.is_fp8:
+            return self.key_cache, self.value_cache, self.key_scale, self.value_scale
+        return self.key_cache, self.value_cache
 
     @property
     def device(self) -> str:
@@ -197,23 +216,36 @@ class PagedKVCacheManager:
         if slot_mapping.numel() == 0:
             return
         dev = self._device
-        k = keys.to(device=dev, dtype=self.dtype)
-        v = values.to(device=dev, dtype=self.dtype)
+        dtype = keys.dtype if self.is_fp8 else self.dtype
+        k = keys.to(device=dev, dtype=dtype)
+        v = values.to(device=dev, dtype=dtype)
         if k.stride(-1) != 1:
             k = k.contiguous()
         if v.stride(-1) != 1:
             v = v.contiguous()
-        paged_ops.reshape_and_cache(k, v, self.key_cache, self.value_cache,
-                                    slot_mapping.to(device=dev, dtype=torch.int64), layer_idx)
+        slots = slot_mapping.to(device=dev, dtype=torch.int64)
+        if self.is_fp8:
+            paged_ops.reshape_and_cache_fp8(k, v, *self.arrays, layer_idx, slots.contiguous())
+        else:
+            paged_ops.reshape_and_cache(k, v, self.key_cache, self.value_cache, slots, layer_idx)
 
     # ---- compatibility reads (manager.py:170-234); not on the hot path --------------------
+    # An 8-bit cache reads back as bf16 values (exact: 4 significant bits times a power of two).
+    def _gather_fp8(self, layer_idx: int, slot_indices: torch.Tensor):
+        slots = slot_indices.to(device=self._device, dtype=torch.int64).contiguous()
+        return paged_ops.gather_cache_fp8(*self.arrays, layer_idx, slots, torch.bfloat16)
+
     def gather_layer_keys(self, layer_idx: int, slot_indices: torch.Tensor) -> torch.Tensor:
         self._validate_layer_idx(layer_idx)
+        if self.is_fp8:
+            return self._gather_fp8(layer_idx, slot_indices)[0]
         return self.key_cache[layer_idx].view(-1, self.num_heads, self.head_dim).index_select(
             0, slot_indices.to(self._device))
 
     def gather_layer_values(self, layer_idx: int, slot_indices: torch.Tensor) -> torch.Tensor:
         self._validate_layer_idx(layer_idx)
+        if self.is_fp8:
+            return self._gather_fp8(layer_idx, slot_indices)[1]
         return self.value_cache[layer_idx].view(-1, self.num_heads, self.head_dim).index_select(
             0, slot_indices.to(self._device))
 
@@ -230,6 +262,13 @@ class PagedKVCacheManager:
             return None
         ids = torch.tensor(blocks, dtype=torch.long, device=self._device)
         out = []
+        if self.is_fp8:
+            pos = torch.arange(read_len, device=self._device)
+            slots = ids[pos // self.block_size] * self.block_size + pos % self.block_size
+            for layer in range(self.num_layers):
+                k, v = self._gather_fp8(layer, slots)
+                out.append((k.unsqueeze(0).transpose(1, 2), v.unsqueeze(0).transpose(1, 2)))
+            return tuple(out)
         for layer in range(self.num_layers):
             k = self.key_cache[layer].index_select(0, ids).reshape(-1, self.num_heads,
                                                                     self.head_dim)[:read_len]
@@ -273,8 +312,7 @@ class PagedKVCacheManager:
         self.pool.flush()
         old, new = self.pool.cow_pairs()
         if old.numel():
-            paged_ops.copy_blocks(self.key_cache, self.value_cache, self.key_cache,
-                                  self.value_cache, old, new, device=self._device)
+            self.copy_blocks(old, new)
 
     # ---- block copies (strategies.py:117-122) -------------------------------------------------
     def copy_blocks(self, src_blocks, dst_blocks) -> None:
@@ -282,6 +320,10 @@ class PagedKVCacheManager:
         copy a caller makes before writing a block it shares with another sequence
         (PageAllocator::share_block / SequenceBlockTable::replace_block,
         csrc/include/page_allocator.hpp:142-149, :416-424).  Asynchronous on the current stream."""
+        if self.is_fp8:
+            paged_ops.copy_blocks_fp8(self.arrays, self.arrays, src_blocks, dst_blocks,
+                                      device=self._device)
+            return
         paged_ops.copy_blocks(self.key_cache, self.value_cache, self.key_cache, self.value_cache,
                               src_blocks, dst_blocks, device=self._device)
 
@@ -299,16 +341,28 @@ class HostSwapSpace:
         self.manager = manager
         self.key_cache = torch.empty(shape, dtype=manager.dtype, pin_memory=True)
         self.value_cache = torch.empty(shape, dtype=manager.dtype, pin_memory=True)
+        self.arrays = (self.key_cache, self.value_cache)
+        if manager.is_fp8:
+            self.arrays += tuple(torch.empty((L, int(num_blocks), H), pin_memory=True)
+                                 for _ in range(2))
 
     def swap_out(self, device_blocks, host_blocks) -> None:
         """Device block ``device_blocks[i]`` -> host block ``host_blocks[i]``."""
         m = self.manager
+        if m.is_fp8:
+            paged_ops.copy_blocks_fp8(m.arrays, self.arrays, device_blocks, host_blocks,
+                                      device=m.torch_device)
+            return
         paged_ops.copy_blocks(m.key_cache, m.value_cache, self.key_cache, self.value_cache,
                               device_blocks, host_blocks, device=m.torch_device)
 
     def swap_in(self, host_blocks, device_blocks) -> None:
         """Host block ``host_blocks[i]`` -> device block ``device_blocks[i]``."""
         m = self.manager
+        if m.is_fp8:
+            paged_ops.copy_blocks_fp8(self.arrays, m.arrays, host_blocks, device_blocks,
+                                      device=m.torch_device)
+            return
         paged_ops.copy_blocks(self.key_cache, self.value_cache, m.key_cache, m.value_cache,
                               host_blocks, device_blocks, device=m.torch_device)
 

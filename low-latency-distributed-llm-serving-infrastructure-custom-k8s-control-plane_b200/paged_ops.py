@@ -94,7 +94,9 @@ def status_word(device: torch.device) -> torch.Tensor:
     index = device.index if device.index is not None else torch.cuda.current_device()
     key = (device.type, index)
     if key not in _STATUS:
-        _STATUS[key] = torch.zeros(1, dtype=torch.int32, device=torch.device(device.type, index))
+        with torch.inference_mode(False):  # the first call may come from inside a model's forward
+            _STATUS[key] = torch.zeros(1, dtype=torch.int32,
+                                       device=torch.device(device.type, index))
     return _STATUS[key]
 
 
@@ -475,6 +477,24 @@ def gather_cache_fp8(key_cache: torch.Tensor, value_cache: torch.Tensor, key_sca
             ctypes.byref(c), _DTYPES[dtype], slots.data_ptr(), slots.shape[0], out[0].data_ptr(),
             out[1].data_ptr(), _status_ptr(dev), _raw_stream(dev)))
     return out[0], out[1]
+
+
+def copy_blocks_fp8(src, dst, src_blocks, dst_blocks,
+                    device: Optional[torch.device] = None) -> None:
+    """``copy_blocks`` between two 8-bit caches, each (key_cache, value_cache, key_scale,
+    value_scale) on the GPU or in page-locked host memory: codes and scales of every layer."""
+    s_ids, d_ids = src_blocks, dst_blocks
+    if device is not None:  # one upload of the ids for both copies
+        s_ids, d_ids = _block_ids(src_blocks, device), _block_ids(dst_blocks, device)
+    codes = lambda c: c.view(torch.float16)  # moved as bytes
+    rows = lambda t: t.view(t.shape[0], t.shape[1], 1, t.shape[2], 1)
+    for c in (src, dst):
+        if c[0].dtype != torch.float8_e4m3fn or c[0].shape[-1] % 2:
+            raise ValueError("8-bit caches must be float8_e4m3fn with an even head dim")
+        if c[2].dtype != torch.float32 or c[2].shape != (*c[0].shape[:2], c[0].shape[3]):
+            raise ValueError("scales must be float32 (layers, blocks, heads)")
+    copy_blocks(codes(src[0]), codes(src[1]), codes(dst[0]), codes(dst[1]), s_ids, d_ids, device)
+    copy_blocks(rows(src[2]), rows(src[3]), rows(dst[2]), rows(dst[3]), s_ids, d_ids, device)
 
 
 def attention_fp8_params(query, key_cache, value_cache, key_scale, value_scale, layer_idx,
