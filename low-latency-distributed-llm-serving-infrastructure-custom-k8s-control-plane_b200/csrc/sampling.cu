@@ -341,22 +341,25 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
 // Where at most kList tokens can be kept after step 2 (top-k), these alone are sorted and 3 to 5
 // done on them.  Rows whose border step holds more than kList tokens (many equal logits) are left
 // to sample_row_kernel.
-constexpr int kClThreads = 512;
-constexpr int kClWarps = kClThreads / 32;
+constexpr int kMaxClWarps = 16;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;
-constexpr int kBracket = kClThreads;  // steps that can hold a top-p border: 512, one a thread
+constexpr int kBracket = 512;       // steps that can hold a top-p border
 constexpr float kBinScale = 64.f;
 
 struct ClusterShared {
-  uint32_t hist[kBins];
-  unsigned long long bins[kBracket];  // exact sums of the border's steps
-  unsigned long long list[kList];     // key << 32 | ~index (descending: larger logit, lower index first)
-  unsigned long long sums[kList];
-  unsigned long long red[3][kClWarps];
+  union {  // the counts are read before the sums are written
+    uint32_t hist[kBins];
+    unsigned long long sums[kList];
+  };
+  union {  // and the exact sums of the border's steps before the list
+    unsigned long long bins[kBracket];
+    unsigned long long list[kList];  // key << 32 | ~index (descending: larger logit, lower index first)
+  };
+  unsigned long long red[3][kMaxClWarps];
   double table[64];
-  float warp_x[kClWarps];
-  double warp_d[kClWarps];
+  float warp_x[kMaxClWarps];
+  double warp_d[kMaxClWarps];
   // of this CTA, for its peers
   float mx;
   unsigned long long total, kept;
@@ -370,7 +373,9 @@ struct ClusterShared {
 };
 
 // Sum of a 64-bit integer over the CTA, known to all threads.  `slot`: which of the scratch rows.
+template <int kClThreads>
 __device__ __forceinline__ unsigned long long cta_sum(unsigned long long v, unsigned long long* red) {
+  constexpr int kClWarps = kClThreads / 32;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
@@ -383,6 +388,7 @@ __device__ __forceinline__ unsigned long long cta_sum(unsigned long long v, unsi
 }
 
 // Descending bitonic sort of n <= kList entries, padded with zeros to a power of two.
+template <int kClThreads>
 __device__ void sort_list(unsigned long long* v, int n) {
   int size = 2;
   while (size < n) size <<= 1;
@@ -404,10 +410,17 @@ __device__ void sort_list(unsigned long long* v, int n) {
 }
 
 // Exclusive prefix sums of n <= kList entries in place; returns their sum.  Whole CTA.
+template <int kClThreads>
 __device__ unsigned long long scan_list(unsigned long long* v, int n, unsigned long long* red) {
+  constexpr int kClWarps = kClThreads / 32, kPer = kList / kClThreads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const unsigned long long a = 2 * tid < n ? v[2 * tid] : 0, b = 2 * tid + 1 < n ? v[2 * tid + 1] : 0;
-  unsigned long long x = a + b;
+  unsigned long long a[kPer], own = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    a[j] = kPer * tid + j < n ? v[kPer * tid + j] : 0;
+    own += a[j];
+  }
+  unsigned long long x = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned long long t = __shfl_up_sync(0xffffffffu, x, o);
@@ -422,9 +435,12 @@ __device__ unsigned long long scan_list(unsigned long long* v, int n, unsigned l
     if (w < warp) before += red[w];
     all += red[w];
   }
-  const unsigned long long excl = before + x - a - b;
-  if (2 * tid < n) v[2 * tid] = excl;
-  if (2 * tid + 1 < n) v[2 * tid + 1] = excl + a;
+  before += x - own;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (kPer * tid + j < n) v[kPer * tid + j] = before;
+    before += a[j];
+  }
   __syncthreads();
   return all;
 }
@@ -450,8 +466,12 @@ __device__ __forceinline__ float largest_of<__half>(uint4 u) {
   return fmaxf(logit<__half>(m.x), logit<__half>(m.y));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArgs a) {
+// kClThreads: 256 for 16-bit logits (four CTAs an SM) and 512 for fp32 (two, as their slices are
+// twice the size): 256 x 128256 with every row's own parameters takes 170 us with 256 threads and
+// 205 with 512 in bf16, 255 (32 KB slices, 16 CTAs a row) and 234 in fp32.
+template <typename T, int kClThreads>
+__global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_kernel(SampleArgs a) {
+  constexpr int kClWarps = kClThreads / 32;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) uint8_t dyn[];
@@ -472,7 +492,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
   const T* s = reinterpret_cast<const T*>(buf + shift);  // s[i]: token begin + i
   fill_table(sh.table);
   for (int i = tid; i < kBins; i += kClThreads) sh.hist[i] = 0;
-  sh.bins[tid] = 0;
+  for (int i = tid; i < kBracket; i += kClThreads) sh.bins[i] = 0;
   if (tid == 0) {
     sh.list_n = 0;
     sh.state = 0;
@@ -653,14 +673,14 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
     if (state == 1 && rank != 0) return;  // rank 0 has all that is left
     if (rank == 0) {
       const int m = sh.list_n;
-      sort_list(sh.list, m);
+      sort_list<kClThreads>(sh.list, m);
       if (state == 1) {
         // everything else on the list: its first k tokens, their sums in order, in index order
         const int keep_k = min(m, rp.k);
         for (int i = tid; i < kList; i += kClThreads)
           sh.sums[i] = i < keep_k ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32)))) : 0;
         __syncthreads();
-        const unsigned long long total = scan_list(sh.sums, keep_k, sh.red[0]);
+        const unsigned long long total = scan_list<kClThreads>(sh.sums, keep_k, sh.red[0]);
         const double target = static_cast<double>(rp.p) * static_cast<double>(total);
         const double mp = static_cast<double>(rp.mp);
         for (int i = tid; i < m; i += kClThreads) {
@@ -671,11 +691,11 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
           sh.list[i] = in ? (e << 32) | (e >> 32) : 0;
         }
         __syncthreads();
-        sort_list(sh.list, m);
+        sort_list<kClThreads>(sh.list, m);
         for (int i = tid; i < kList; i += kClThreads)
           sh.sums[i] = i < m && sh.list[i] != 0 ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i])))) : 0;
         __syncthreads();
-        const unsigned long long sum = scan_list(sh.sums, m, sh.red[0]);
+        const unsigned long long sum = scan_list<kClThreads>(sh.sums, m, sh.red[0]);
         const unsigned long long goal =
             static_cast<unsigned long long>(static_cast<double>(rp.u) * static_cast<double>(sum));
         for (int i = tid; i < m; i += kClThreads) {
@@ -701,6 +721,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
     const float scale = kBinScale / static_cast<float>(t);
     if (top_k) {  // a second set of counts
       for (int i = tid; i < kBins; i += kClThreads) sh.hist[i] = 0;
+      for (int i = tid; i < kBracket; i += kClThreads) sh.bins[i] = 0;
       if (tid == 0) {
         sh.list_n = 0;
         sh.state = 0;
@@ -768,29 +789,49 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
         else if (b <= hi) atomicAdd(&sh.bins[b - lo], w);
       }
     }
-    total = cta_sum(total, sh.red[1]);
-    above = cta_sum(above, sh.red[2]);  // its barriers order the steps' sums too
+    total = cta_sum<kClThreads>(total, sh.red[1]);
+    above = cta_sum<kClThreads>(above, sh.red[2]);  // its barriers order the steps' sums too
     if (tid == 0) {
       atomicAdd(&head->all_total, total);
       atomicAdd(&head->all_above, above);
     }
-    if (rank != 0 && few && tid <= hi - lo && sh.bins[tid]) atomicAdd(&head->bins[tid], sh.bins[tid]);
+    if (rank != 0 && few)
+      for (int i = tid; i <= hi - lo; i += kClThreads)
+        if (sh.bins[i]) atomicAdd(&head->bins[i], sh.bins[i]);
     cluster.sync();
     if (rank == 0) {
+      // the border's step: the first one that reaches the target (step lo where rounding left it just
+      // behind); each thread looks at kPer steps in a row
+      constexpr int kPer = kBracket / kClThreads;
       const int steps = few ? hi - lo + 1 : 0;
-      const unsigned long long h = tid < steps ? sh.bins[tid] : 0;
-      sh.sums[tid] = h;
+      unsigned long long h[kPer], own = 0;
+      uint32_t held[kPer];
+      for (int j = 0; j < kPer; ++j) {
+        const int b = kPer * tid + j;
+        h[j] = b < steps ? sh.bins[b] : 0;
+        held[j] = b < steps ? sh.hist[lo + b] : 0;
+        own += h[j];
+      }
+      unsigned long long x = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
+      }
+      if (lane == 31) sh.red[0][warp] = x;
       if (tid == 0) sh.state = 3;
       __syncthreads();
-      scan_list(sh.sums, kClThreads, sh.red[0]);
       const double target = static_cast<double>(rp.p) * static_cast<double>(sh.all_total);
-      const unsigned long long up = sh.all_above + sh.sums[tid];
-      // the border's step: the first one that reaches the target (step lo where rounding left it just
-      // behind)
-      if (tid < steps && (static_cast<double>(up) < target || tid == 0) && static_cast<double>(up + h) >= target) {
-        sh.bin = lo + tid;
-        sh.above_bin = up;
-        sh.state = sh.hist[lo + tid] <= kList ? 2 : 3;
+      unsigned long long up = sh.all_above + x - own;
+      for (int w = 0; w < warp; ++w) up += sh.red[0][w];
+      for (int j = 0; j < kPer; ++j) {
+        const int b = kPer * tid + j;
+        if (b < steps && (static_cast<double>(up) < target || b == 0) && static_cast<double>(up + h[j]) >= target) {
+          sh.bin = lo + b;
+          sh.above_bin = up;
+          sh.state = held[j] <= kList ? 2 : 3;
+        }
+        up += h[j];
       }
     }
     cluster.sync();
@@ -803,11 +844,11 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
     gather(scale, bin, bin);
     if (rank == 0) {
       const int m = sh.list_n;
-      sort_list(sh.list, m);
+      sort_list<kClThreads>(sh.list, m);
       for (int i = tid; i < kList; i += kClThreads)
         sh.sums[i] = i < m ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32)))) : 0;
       __syncthreads();
-      scan_list(sh.sums, m, sh.red[0]);
+      scan_list<kClThreads>(sh.sums, m, sh.red[0]);
       const double target = static_cast<double>(rp.p) * static_cast<double>(sh.all_total);
       for (int i = tid; i < m; i += kClThreads) {
         const bool in = static_cast<double>(sh.above_bin + sh.sums[i]) < target;
@@ -846,7 +887,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   __syncthreads();
   if (lane == 0) sh.red[0][warp] = mine;
-  all = cta_sum(all, sh.red[1]);
+  all = cta_sum<kClThreads>(all, sh.red[1]);
   if (tid == 0) {
     unsigned long long sum = 0;
     for (int w = 0; w < kClWarps; ++w) sum += sh.red[0][w];
@@ -919,19 +960,19 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(SampleArg
   }
 }
 
-// CTAs a row: enough to make a slice at most 16384 tokens and 64 KB (two CTAs fit an SM, and one
-// loads while the other computes), but 8 at most (192 KB of tokens each); more where the rows would
-// leave SMs idle.  0: the vocabulary does not fit.
+// CTAs a row: enough to make a slice at most 16384 tokens, but 8 at most (192 KB of tokens each);
+// more where the rows would leave SMs idle.  0: the vocabulary does not fit.
 int cluster_size(int rows, int vocab, int es, int num_sms) {
   const int64_t bytes = static_cast<int64_t>(vocab) * es;
   if ((bytes + 7) / 8 > 192 * 1024) return 0;
   int c = 1;
-  while (c < 8 && (vocab / c > 16384 || bytes / c > 64 * 1024 || (rows * c * 2 <= num_sms && vocab / c > 1024))) c *= 2;
+  while (c < 8 && (vocab / c > 16384 || bytes / c > 192 * 1024 || (rows * c * 2 <= num_sms && vocab / c > 1024))) c *= 2;
   return c;
 }
 
 template <typename T>
 cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream) {
+  constexpr int kClThreads = sizeof(T) == 2 ? 256 : 512;
   const int C = cluster_size(a.rows, a.vocab, sizeof(T), num_sms());
   if (C == 0) {
     sample_row_kernel<T><<<a.rows, kSampleThreads, 0, stream>>>(a, false);
@@ -939,7 +980,7 @@ cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream) {
   }
   const int slice = (a.vocab + C - 1) / C;
   const size_t smem = (sizeof(ClusterShared) + 15) / 16 * 16 + (static_cast<size_t>(slice) * sizeof(T) + 47) / 16 * 16;
-  cudaError_t e = allow_smem<sample_cluster_kernel<T>>(227 * 1024);
+  cudaError_t e = allow_smem<sample_cluster_kernel<T, kClThreads>>(227 * 1024);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -952,7 +993,7 @@ cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, sample_cluster_kernel<T>, a);
+  e = cudaLaunchKernelEx(&cfg, sample_cluster_kernel<T, kClThreads>, a);
   if (e != cudaSuccess) return e;
   // the rows that are left; its launch overlaps the cluster kernel's end
   attr[0] = {};
