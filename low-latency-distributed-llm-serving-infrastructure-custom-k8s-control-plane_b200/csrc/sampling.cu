@@ -359,7 +359,6 @@ struct ClusterShared {
   unsigned long long red[3][kMaxClWarps];
   double table[64];
   float warp_x[kMaxClWarps];
-  double warp_d[kMaxClWarps];
   // of this CTA, for its peers
   float mx;
   unsigned long long total, kept;
@@ -555,16 +554,37 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
 
   uint32_t cut_key = 0, cut_idx = 0xffffffffu;  // kept: larger keys, and this key up to this index
   const auto kept = [&](uint32_t key, uint32_t idx) { return key > cut_key || (key == cut_key && idx <= cut_idx); };
-  const auto bin_of = [&](float v, float scale) {
-    return v == mx ? 0 : static_cast<int>(fminf((mx - v) * scale, static_cast<float>(kBins - 1)));
+  // f(logit, token of the slice) for the warp's tokens; four are read before the first is worked on
+  const auto each = [&](auto f) {
+    constexpr int U = 4;
+    int i = w0 + lane;
+    for (; i + 32 * (U - 1) < w1; i += 32 * U) {
+      float v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = logit<T>(s[i + 32 * u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) f(v[u], i + 32 * u);
+    }
+    for (; i < w1; i += 32) f(logit<T>(s[i]), i);
   };
-  // w where only the log probability asks for it: exact for the terms above 2^-10, in fp32 (4e-7
-  // off at most, either way) for the many small ones behind them
+  // Sum of w where only the log probability asks for it: exact for the terms above 2^-10, in fp32
+  // (4e-7 off at most, either way) for the many small ones behind them.
   const float c32 = static_cast<float>(1.4426950408889634 / t);
+  double sum_large = 0.0;
+  float sum_small = 0.f;
   const auto sum32 = [&](float v) {
     const float y = v == mx ? 0.f : (v - mx) * c32;
-    return y > -10.f ? weight(v) : static_cast<double>(fast_exp2(y));
+    if (y > -10.f) sum_large += weight(v);
+    else sum_small += fast_exp2(y);
   };
+  // the warps' sums into rank 0's, in fixed point (so their order does not matter); whole CTA
+  const auto add_sum32 = [&]() {
+    double part = sum_large + static_cast<double>(sum_small);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    if (lane == 0) atomicAdd(&head->sum32, static_cast<unsigned long long>(part * 0x1p+38));
+  };
+  const auto sum32_all = [&]() { return static_cast<double>(head->sum32) * 0x1p-38; };
   const auto finish = [&](int token, double sum_all) {
     a.tokens[row] = token;
     if (a.logprobs) {
@@ -573,68 +593,56 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       a.logprobs[row] = static_cast<float>(z - log(sum_all));
     }
   };
-  // the warps' parts of that sum into rank 0's, in fixed point (so their order does not matter)
-  const auto add_sum32 = [&]() {
-    double all = 0.0;
-    for (int w = 0; w < kClWarps; ++w) all += sh.warp_d[w];
-    atomicAdd(&head->sum32, static_cast<unsigned long long>(all * 0x1p+38));
+  // the place of a logit below the maximum, in steps; its step is the place's whole part, the last
+  // one being open
+  const auto place_of = [&](float v, float scale) { return v == mx ? 0.f : (mx - v) * scale; };
+  const auto bin_of = [&](float v, float scale) {
+    return static_cast<int>(fminf(place_of(v, scale), static_cast<float>(kBins - 1)));
   };
-  const auto sum32_all = [&]() { return static_cast<double>(head->sum32) * 0x1p-38; };
-  // counts by step of the kept tokens, summed over the cluster into rank 0's
-  const auto histogram = [&](float scale, bool with_sum) {
-    double part = 0.0;
-    for (int i = w0 + lane; i < w1; i += 32) {
-      const float v = logit<T>(s[i]);
-      if (with_sum) part += sum32(v);
-      if (kept(key_of(v), begin + i)) atomicAdd(&sh.hist[bin_of(v, scale)], 1u);
-    }
-    if (with_sum) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      if (lane == 0) sh.warp_d[warp] = part;
-    }
+  // counts by step, summed over the cluster into rank 0's; `f` is given every logit
+  const auto histogram = [&](float scale, bool all, auto f) {
+    each([&](float v, int i) {
+      f(v);
+      if (all || kept(key_of(v), begin + i)) atomicAdd(&sh.hist[bin_of(v, scale)], 1u);
+    });
     __syncthreads();
-    if (with_sum && tid == 0) add_sum32();
     if (rank != 0)
       for (int i = tid; i < kBins; i += kClThreads)
         if (sh.hist[i]) atomicAdd(&head->hist[i], sh.hist[i]);
-    cluster.sync();
   };
   // tokens of steps [lo, hi] that are kept, into rank 0's list
   const auto gather = [&](float scale, int lo, int hi) {
-    for (int i = w0 + lane; i < w1; i += 32) {
-      const float v = logit<T>(s[i]);
-      const int b = bin_of(v, scale);
-      const uint32_t key = key_of(v), idx = begin + i;
-      if (b >= lo && b <= hi && kept(key, idx)) {
-        const int at = atomicAdd(&head->list_n, 1);
-        if (at < kList) head->list[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - idx);
+    const float from = static_cast<float>(lo), to = hi >= kBins - 1 ? INFINITY : static_cast<float>(hi + 1);
+    each([&](float v, int i) {
+      const float at_step = place_of(v, scale);
+      if (at_step >= from && (at_step < to || to == INFINITY)) {
+        const uint32_t key = key_of(v), idx = begin + i;
+        if (kept(key, idx)) {
+          const int at = atomicAdd(&head->list_n, 1);
+          if (at < kList) head->list[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - idx);
+        }
       }
-    }
+    });
     cluster.sync();
   };
 
   if (rp.greedy || rp.k == 1) {
-    double part = 0.0;
     int best = V;
-    for (int i = w0 + lane; i < w1; i += 32) {
-      const float v = logit<T>(s[i]);
-      part += sum32(v);
+    each([&](float v, int i) {
+      sum32(v);
       if (v == mx) best = min(best, begin + i);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-    if (lane == 0) sh.warp_d[warp] = part;
+    });
     if (best < V) atomicMin(&head->token, best);
-    __syncthreads();
-    if (tid == 0) add_sum32();
+    add_sum32();
     cluster.sync();  // rank 0 goes on with what it holds; its peers are done
     if (rank == 0 && tid == 0) finish(sh.token, sum32_all());
     return;
   }
 
   if (top_k) {
-    histogram(kBinScale, true);
+    histogram(kBinScale, true, sum32);
+    add_sum32();
+    cluster.sync();
     if (rank == 0) {
       // the step that holds the k-th token, and how many tokens lie up to it
       const int per_t = kBins / kClThreads;
@@ -728,7 +736,8 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       }
       cluster.sync();
     }
-    histogram(scale, false);
+    histogram(scale, !top_k, [](float) {});
+    cluster.sync();
     if (rank == 0) {
       // the border's steps: where p times the sum can lie, with a step's sum known to e^(1/64)
       const int per_t = kBins / kClThreads;
@@ -779,15 +788,19 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
     unsigned long long total = 0, above = 0;
     const bool few = hi - lo < kBracket;
     if (few) {
-      for (int i = w0 + lane; i < w1; i += 32) {
-        const float v = logit<T>(s[i]);
-        if (!kept(key_of(v), begin + i)) continue;
+      const float from = static_cast<float>(lo);
+      each([&](float v, int i) {
+        if (top_k && !kept(key_of(v), begin + i)) return;
         const unsigned long long w = weight.fixed(weight(v));
-        const int b = bin_of(v, scale);
         total += w;
-        if (b < lo) above += w;
-        else if (b <= hi) atomicAdd(&sh.bins[b - lo], w);
-      }
+        const float at_step = place_of(v, scale);
+        if (at_step < from) {
+          above += w;
+        } else {
+          const int b = static_cast<int>(fminf(at_step, static_cast<float>(kBins - 1)));
+          if (b <= hi) atomicAdd(&sh.bins[b - lo], w);
+        }
+      });
     }
     total = cta_sum<kClThreads>(total, sh.red[1]);
     above = cta_sum<kClThreads>(above, sh.red[2]);  // its barriers order the steps' sums too
@@ -869,19 +882,16 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
   const bool filtered = top_k || top_p;
   unsigned long long mine = 0, all = 0;
   if (!filtered && mp <= 0.0) {
-#pragma unroll 4
-    for (int i = w0 + lane; i < w1; i += 32) mine += weight.fixed(weight(logit<T>(s[i])));
+    each([&](float v, int) { mine += weight.fixed(weight(v)); });
     all = mine;
   } else {
-#pragma unroll 2
-    for (int i = w0 + lane; i < w1; i += 32) {
-      const float v = logit<T>(s[i]);
-      if (filtered && !kept(key_of(v), begin + i)) continue;
+    each([&](float v, int i) {
+      if (filtered && !kept(key_of(v), begin + i)) return;
       const double w = weight(v);
       const unsigned long long f = weight.fixed(w);
       all += f;
       if (w >= mp) mine += f;
-    }
+    });
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
