@@ -57,16 +57,16 @@ __device__ __forceinline__ RowParams row_params(const SampleArgs& a, int row) {
   return r;
 }
 
-// A logit; NaN counts as masked, -0 as 0.
+// A logit; NaN counts as masked, an infinite one as the largest number.
 template <typename T>
 __device__ __forceinline__ float logit(T v) {
-  const float x = to_f32<T>(v) + 0.f;
-  return x == x ? x : -INFINITY;
+  const float x = to_f32<T>(v);
+  return x == x ? fminf(x, 3.402823466e38f) : -INFINITY;
 }
 
-// Unsigned key with the order of the floats.
+// Unsigned key with the order of the floats; -0 and 0 are one number.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f);
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float float_of(uint32_t key) {
@@ -78,19 +78,19 @@ __device__ __forceinline__ float float_of(uint32_t key) {
 // 0.0055, remainder below 5e-14.
 struct Weights {
   const double* table;  // 2^(j/64), j < 64, in shared memory
-  double mx, c;         // maximum (an infinite one counts as the largest number); 64 log2(e) / t
+  double mx, c;         // maximum; 64 log2(e) / t
   double bias;          // 2^(52 - shift): adding it leaves round(w 2^shift) in the mantissa's low bits
 
   __device__ __forceinline__ void set(const double* tab, float m, double t, int shift) {
     table = tab;
-    mx = static_cast<double>(fminf(m, 3.402823466e38f));
+    mx = static_cast<double>(m);
     c = 64.0 * 1.4426950408889634 / t;
     bias = static_cast<double>(1ull << (52 - shift));
   }
   // No branches, so that several run in flight.  y is clamped at -3968 (w = 2^-62, which rounds to
   // 0) by its high word: among negative numbers the larger word is the lower number.
   __device__ __forceinline__ double operator()(float x) const {
-    double y = (static_cast<double>(fminf(x, 3.402823466e38f)) - mx) * c;
+    double y = (static_cast<double>(x) - mx) * c;
     y = __hiloint2double(static_cast<int>(umin(static_cast<uint32_t>(__double2hiint(y)), 0xC0AF0000u)), __double2loint(y));
     const double v = y + 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are round(y)
     const int n = __double2loint(v);
@@ -344,6 +344,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
 constexpr int kMaxClWarps = 16;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;
+constexpr int kCounted = 384;  // entries up to which a list's order is counted out instead of sorted
 constexpr int kBracket = 512;       // steps that can hold a top-p border
 constexpr float kBinScale = 64.f;
 
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
     const uint8_t* aligned = reinterpret_cast<const uint8_t*>(src) - shift;
     const int pieces = n > 0 ? static_cast<int>((shift + n * sizeof(T) + 15) / 16) : 0;
     const int first = begin - static_cast<int>(shift / sizeof(T));  // token of the first piece's first
-#pragma unroll 4
+#pragma unroll 8
     for (int p = tid; p < pieces; p += kClThreads) {
       const int i0 = first + p * E;
       if (i0 >= 0 && i0 + E <= V) {  // (a piece at the slice's end may hold tokens of the next one's)
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
   double sum_large = 0.0;
   float sum_small = 0.f;
   const auto sum32 = [&](float v) {
-    const float y = v == mx ? 0.f : (v - mx) * c32;
+    const float y = (v - mx) * c32;
     if (y > -10.f) sum_large += weight(v);
     else sum_small += fast_exp2(y);
   };
@@ -595,7 +596,7 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
   };
   // the place of a logit below the maximum, in steps; its step is the place's whole part, the last
   // one being open
-  const auto place_of = [&](float v, float scale) { return v == mx ? 0.f : (mx - v) * scale; };
+  const auto place_of = [&](float v, float scale) { return (mx - v) * scale; };
   const auto bin_of = [&](float v, float scale) {
     return static_cast<int>(fminf(place_of(v, scale), static_cast<float>(kBins - 1)));
   };
@@ -639,6 +640,30 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
     return;
   }
 
+  // Of up to kCounted entries of the list, by comparing all with all: how many are ahead of this
+  // thread's, and their weights' sum; every entry's weight into sums.  Whole CTA.
+  int place[(kCounted + kClThreads - 1) / kClThreads];
+  unsigned long long ahead[(kCounted + kClThreads - 1) / kClThreads];
+  const auto order_list = [&](int m) {
+    for (int i = tid; i < m; i += kClThreads)
+      sh.sums[i] = weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32))));
+    __syncthreads();
+    for (int j = 0; j < static_cast<int>(sizeof(place) / sizeof(place[0])); ++j) {
+      const int i = tid + j * kClThreads;
+      place[j] = 0;
+      ahead[j] = 0;
+      if (i >= m) continue;
+      const unsigned long long own = sh.list[i];
+#pragma unroll 4
+      for (int o = 0; o < m; ++o)
+        if (sh.list[o] > own) {
+          ++place[j];
+          ahead[j] += sh.sums[o];
+        }
+    }
+    __syncthreads();
+  };
+
   if (top_k) {
     histogram(kBinScale, true, sum32);
     add_sum32();
@@ -681,41 +706,80 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
     if (state == 1 && rank != 0) return;  // rank 0 has all that is left
     if (rank == 0) {
       const int m = sh.list_n;
-      sort_list<kClThreads>(sh.list, m);
       if (state == 1) {
-        // everything else on the list: its first k tokens, their sums in order, in index order
-        const int keep_k = min(m, rp.k);
-        for (int i = tid; i < kList; i += kClThreads)
-          sh.sums[i] = i < keep_k ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32)))) : 0;
-        __syncthreads();
-        const unsigned long long total = scan_list<kClThreads>(sh.sums, keep_k, sh.red[0]);
-        const double target = static_cast<double>(rp.p) * static_cast<double>(total);
+        // everything else on the list: its first k tokens, of these top-p's, and the draw
         const double mp = static_cast<double>(rp.mp);
-        for (int i = tid; i < m; i += kClThreads) {
-          const unsigned long long e = sh.list[i];
-          const double w = weight(float_of(static_cast<uint32_t>(e >> 32)));
-          const bool in = i < keep_k && (!top_p || i == 0 || static_cast<double>(sh.sums[i]) < target) && w >= mp;
-          // by index; a token that is not kept sorts behind as 0
-          sh.list[i] = in ? (e << 32) | (e >> 32) : 0;
-        }
-        __syncthreads();
-        sort_list<kClThreads>(sh.list, m);
-        for (int i = tid; i < kList; i += kClThreads)
-          sh.sums[i] = i < m && sh.list[i] != 0 ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i])))) : 0;
-        __syncthreads();
-        const unsigned long long sum = scan_list<kClThreads>(sh.sums, m, sh.red[0]);
-        const unsigned long long goal =
-            static_cast<unsigned long long>(static_cast<double>(rp.u) * static_cast<double>(sum));
-        for (int i = tid; i < m; i += kClThreads) {
-          const unsigned long long after = i + 1 < m ? sh.sums[i + 1] : sum;
-          if (sh.sums[i] <= goal && goal < after) sh.token = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(sh.list[i] >> 32));
+        if (m <= kCounted) {
+          constexpr int kPer = (kCounted + kClThreads - 1) / kClThreads;
+          order_list(m);
+          unsigned long long w[kPer], total = 0, sum = 0;
+          for (int j = 0; j < kPer; ++j) {
+            const int i = tid + j * kClThreads;
+            w[j] = i < m ? sh.sums[i] : 0;
+            if (i < m && place[j] < rp.k) total += w[j];
+          }
+          total = cta_sum<kClThreads>(total, sh.red[0]);
+          const double target = static_cast<double>(rp.p) * static_cast<double>(total);
+          for (int j = 0; j < kPer; ++j) {
+            const int i = tid + j * kClThreads;
+            if (i >= m) continue;
+            const bool in = place[j] < rp.k &&
+                            (!top_p || place[j] == 0 || static_cast<double>(ahead[j]) < target) &&
+                            weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32))) >= mp;
+            if (!in) w[j] = 0;
+            sh.sums[i] = w[j];
+            sum += w[j];
+          }
+          sum = cta_sum<kClThreads>(sum, sh.red[0]);
+          const unsigned long long goal =
+              static_cast<unsigned long long>(static_cast<double>(rp.u) * static_cast<double>(sum));
+          for (int j = 0; j < kPer; ++j) {
+            const int i = tid + j * kClThreads;
+            if (i >= m || w[j] == 0) continue;
+            const uint32_t own = static_cast<uint32_t>(sh.list[i]);  // ~index: larger for lower ones
+            unsigned long long before = 0;
+            for (int o = 0; o < m; ++o)
+              if (static_cast<uint32_t>(sh.list[o]) > own) before += sh.sums[o];
+            if (before <= goal && goal < before + w[j]) sh.token = static_cast<int32_t>(0xffffffffu - own);
+          }
+        } else {
+          sort_list<kClThreads>(sh.list, m);
+          const int keep_k = min(m, rp.k);
+          for (int i = tid; i < kList; i += kClThreads)
+            sh.sums[i] = i < keep_k ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32)))) : 0;
+          __syncthreads();
+          const unsigned long long total = scan_list<kClThreads>(sh.sums, keep_k, sh.red[0]);
+          const double target = static_cast<double>(rp.p) * static_cast<double>(total);
+          for (int i = tid; i < m; i += kClThreads) {
+            const unsigned long long e = sh.list[i];
+            const double w = weight(float_of(static_cast<uint32_t>(e >> 32)));
+            const bool in = i < keep_k && (!top_p || i == 0 || static_cast<double>(sh.sums[i]) < target) && w >= mp;
+            // by index; a token that is not kept sorts behind as 0
+            sh.list[i] = in ? (e << 32) | (e >> 32) : 0;
+          }
+          __syncthreads();
+          sort_list<kClThreads>(sh.list, m);
+          for (int i = tid; i < kList; i += kClThreads)
+            sh.sums[i] = i < m && sh.list[i] != 0 ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i])))) : 0;
+          __syncthreads();
+          const unsigned long long sum = scan_list<kClThreads>(sh.sums, m, sh.red[0]);
+          const unsigned long long goal =
+              static_cast<unsigned long long>(static_cast<double>(rp.u) * static_cast<double>(sum));
+          for (int i = tid; i < m; i += kClThreads) {
+            const unsigned long long after = i + 1 < m ? sh.sums[i + 1] : sum;
+            if (sh.sums[i] <= goal && goal < after)
+              sh.token = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(sh.list[i] >> 32));
+          }
         }
         __syncthreads();
         if (tid == 0) finish(sh.token, sum32_all());
-      } else if (tid == 0) {
-        const unsigned long long e = sh.list[rp.k - static_cast<int>(sh.above_bin) - 1];
-        sh.cut_key = static_cast<uint32_t>(e >> 32);
-        sh.cut_idx = 0xffffffffu - static_cast<uint32_t>(e);
+      } else {
+        sort_list<kClThreads>(sh.list, m);
+        if (tid == 0) {
+          const unsigned long long e = sh.list[rp.k - static_cast<int>(sh.above_bin) - 1];
+          sh.cut_key = static_cast<uint32_t>(e >> 32);
+          sh.cut_idx = 0xffffffffu - static_cast<uint32_t>(e);
+        }
       }
     }
     if (state == 1) return;
@@ -857,18 +921,32 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
     gather(scale, bin, bin);
     if (rank == 0) {
       const int m = sh.list_n;
-      sort_list<kClThreads>(sh.list, m);
-      for (int i = tid; i < kList; i += kClThreads)
-        sh.sums[i] = i < m ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32)))) : 0;
-      __syncthreads();
-      scan_list<kClThreads>(sh.sums, m, sh.red[0]);
       const double target = static_cast<double>(rp.p) * static_cast<double>(sh.all_total);
-      for (int i = tid; i < m; i += kClThreads) {
-        const bool in = static_cast<double>(sh.above_bin + sh.sums[i]) < target;
-        const bool next = i + 1 < m && static_cast<double>(sh.above_bin + sh.sums[i + 1]) < target;
-        if (in && !next) {  // the last token that is kept
-          sh.cut_key = static_cast<uint32_t>(sh.list[i] >> 32);
-          sh.cut_idx = 0xffffffffu - static_cast<uint32_t>(sh.list[i]);
+      if (m <= kCounted) {
+        order_list(m);
+        for (int j = 0; j < static_cast<int>(sizeof(place) / sizeof(place[0])); ++j) {
+          const int i = tid + j * kClThreads;
+          if (i >= m) continue;
+          // the last token that is kept: the sum ahead of it is short of the target, with it it is not
+          const unsigned long long up = sh.above_bin + ahead[j];
+          if (static_cast<double>(up) < target && (static_cast<double>(up + sh.sums[i]) >= target || place[j] == m - 1)) {
+            sh.cut_key = static_cast<uint32_t>(sh.list[i] >> 32);
+            sh.cut_idx = 0xffffffffu - static_cast<uint32_t>(sh.list[i]);
+          }
+        }
+      } else {
+        sort_list<kClThreads>(sh.list, m);
+        for (int i = tid; i < kList; i += kClThreads)
+          sh.sums[i] = i < m ? weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32)))) : 0;
+        __syncthreads();
+        scan_list<kClThreads>(sh.sums, m, sh.red[0]);
+        for (int i = tid; i < m; i += kClThreads) {
+          const bool in = static_cast<double>(sh.above_bin + sh.sums[i]) < target;
+          const bool next = i + 1 < m && static_cast<double>(sh.above_bin + sh.sums[i + 1]) < target;
+          if (in && !next) {
+            sh.cut_key = static_cast<uint32_t>(sh.list[i] >> 32);
+            sh.cut_idx = 0xffffffffu - static_cast<uint32_t>(sh.list[i]);
+          }
         }
       }
     }
