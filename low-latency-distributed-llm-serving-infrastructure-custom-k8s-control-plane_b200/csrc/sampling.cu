@@ -358,6 +358,7 @@ struct ClusterShared {
     unsigned long long list[kList];  // key << 32 | ~index (descending: larger logit, lower index first)
   };
   unsigned long long red[3][kMaxClWarps];
+  uint64_t loaded[4];  // barriers of the slice's quarters
   double table[64];
   float warp_x[kMaxClWarps];
   // of this CTA, for its peers
@@ -501,25 +502,48 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
   }
   float mx = -INFINITY;
   {
+    // the pieces that lie inside the row come by bulk copy, a quarter at a time (a piece at the
+    // slice's end may hold tokens of the next one's)
     constexpr int E = 16 / sizeof(T);
     const uint8_t* aligned = reinterpret_cast<const uint8_t*>(src) - shift;
     const int pieces = n > 0 ? static_cast<int>((shift + n * sizeof(T) + 15) / 16) : 0;
     const int first = begin - static_cast<int>(shift / sizeof(T));  // token of the first piece's first
-#pragma unroll 8
-    for (int p = tid; p < pieces; p += kClThreads) {
-      const int i0 = first + p * E;
-      if (i0 >= 0 && i0 + E <= V) {  // (a piece at the slice's end may hold tokens of the next one's)
-        const uint4 u = *reinterpret_cast<const uint4*>(aligned + 16 * p);
-        *reinterpret_cast<uint4*>(buf + 16 * p) = u;
-        mx = fmaxf(mx, largest_of<T>(u));
-      } else {
-        for (int j = 0; j < E; ++j)
-          if (i0 + j >= begin && i0 + j < begin + n) {
-            const T v = x0[i0 + j];
-            reinterpret_cast<T*>(buf)[p * E + j] = v;
-            mx = fmaxf(mx, logit<T>(v));
-          }
+    const int p0 = pieces > 0 && first < 0 ? 1 : 0;
+    const int p1 = pieces > p0 && first + pieces * E > V ? pieces - 1 : pieces;
+    const int quarter = (p1 - p0 + 3) / 4;
+    if (tid == 0) {
+      for (int q = 0; q < 4; ++q) mbar_init(&sh.loaded[q], 1);
+      fence_proxy_async_smem();
+      for (int q = 0; q < 4; ++q) {
+        const int b = p0 + q * quarter, e = min(p1, b + quarter);
+        if (e <= b) continue;
+        mbar_arrive_expect_tx(&sh.loaded[q], (e - b) * 16);
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                smem_u32(buf + 16 * b)),
+            "l"(aligned + 16 * static_cast<int64_t>(b)), "r"((e - b) * 16), "r"(smem_u32(&sh.loaded[q]))
+            : "memory");
       }
+    }
+    // the pieces at the row's ends, by element
+    const auto edge = [&](int p) {
+      const int i = first + p * E + tid;
+      if (tid < E && i >= begin && i < begin + n) {
+        const T v = x0[i];
+        reinterpret_cast<T*>(buf)[p * E + tid] = v;
+        mx = fmaxf(mx, logit<T>(v));
+      }
+    };
+    if (p0 == 1) edge(0);
+    if (p1 < pieces) edge(p1);
+    __syncthreads();
+    for (int q = 0; q < 4; ++q) {
+      const int b = p0 + q * quarter, e = min(p1, b + quarter);
+      if (e <= b) break;
+      if (!mbar_wait_bounded(&sh.loaded[q], 0) && lane == 0) flag_status(a.status, B200_DEVICE_TIMEOUT);
+#pragma unroll 2
+      for (int p = b + tid; p < e; p += kClThreads)
+        mx = fmaxf(mx, largest_of<T>(*reinterpret_cast<const uint4*>(buf + 16 * p)));
     }
   }
 #pragma unroll
