@@ -129,7 +129,7 @@ DecodePlan decode_plan(const B200AttentionFp8Params& p) {
   if (pl.max_ctx < 0) pl.max_ctx = 0;
   pl.grid = b200::decode_fp8_grid(S, pl.max_ctx, c.num_kv_heads * pl.nchunks, num_sms());
   const size_t parts = b200::decode_fp8_parts(pl.grid);
-  pl.off_ml = align256((S + 1) * sizeof(int32_t));
+  pl.off_ml = align256(parts / 2 * sizeof(b200::MergeItem));
   pl.off_o = pl.off_ml + align256(parts * 8 * sizeof(float2));
   pl.total = pl.off_o + align256(parts * 8 * c.head_dim * sizeof(float));
   return pl;
@@ -181,7 +181,7 @@ int run_decode(const B200AttentionFp8Params& p, const DecodePlan& pl, const int6
   a.o_srow = p.o_stride_row;
   a.o_shead = p.o_stride_head;
   a.status = p.status_word;
-  a.cu_units = reinterpret_cast<int32_t*>(ws);
+  a.merge = reinterpret_cast<b200::MergeItem*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + pl.off_ml);
   a.part_o = reinterpret_cast<float*>(ws + pl.off_o);
   for (int s0 = 0; s0 < p.num_seqs; s0 += b200::kDecodeFp8MaxSeqs) {

@@ -253,9 +253,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     prefetch_tensormap(&vmap);
   }
   prefix_units(a, cu, warp_sums);  // its barriers publish the mbarriers too
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= a.S; i += kThreads) a.cu_units[i] = cu[i];
   __syncthreads();
+  // decoded sequences without context: zeros
+  for (int s = blockIdx.x; s < a.S; s += gridDim.x) {
+    if (tid == 0 && a.ctx_lens[s] > a.max_ctx) flag_status(a.status, B200_DEVICE_BAD_OP);
+    if (cu[s + 1] != cu[s] || (a.cu_q != nullptr && a.cu_q[s + 1] - a.cu_q[s] != 1)) continue;
+    const int64_t row = a.cu_q ? a.cu_q[s] : (a.query_rows ? a.query_rows[s] : s);
+    const int hq = a.hkv * a.group;
+    for (int i = tid; i < hq * D; i += kThreads)
+      static_cast<T*>(a.out)[row * a.o_srow + static_cast<int64_t>(i / D) * a.o_shead + i % D] = from_f32<T>(0.f);
+  }
 
   asm volatile("griddepcontrol.launch_dependents;");
   // teams of ts warps walk the line side by side, each warp with an item of its own
@@ -409,6 +416,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   uint64_t* my_empty = empty + warp * NS;
   int stage = 0;
   uint32_t phase = 0;
+  MergeItem joined{};  // what the merge is to do for this warp
   // ldmatrix: lane's row of 16 tokens and 16-byte chunk 0 or 1, swizzled; chunk k is at ^ (k << 4)
   const int krow = (lane & 7) + 8 * ((lane >> 3) & 1);
   const uint32_t lane_at = tile_at<D>(krow, lane >> 4);
@@ -416,7 +424,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   for (;;) {
     int seq, hct, u0;
     const int n = next_piece(walk, cu, ips, 0x7fffffff, seq, hct, u0);
-    if (n == 0) break;
+    if (n == 0) {
+      if (lane == 0) a.merge[gw] = joined;
+      break;
+    }
     const int hc = hct * ts + warp % ts;
     const int h = hc / a.nchunks, cch = hc - h * a.nchunks;
     const int units = cu[seq + 1] - cu[seq] - kItemCost;
@@ -472,6 +483,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (!mbar_wait_bounded(&my_full[stage], phase)) {
         if (lane == 0) flag_status(a.status, B200_DEVICE_TIMEOUT);
         *abort_s = 1;  // the producer sees to what is in flight
+        if (lane == 0) a.merge[gw] = MergeItem{};
         return;
       }
       const uint32_t kb = ring_u32 + stage * R::kStage + lane_at;
@@ -683,6 +695,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       }
     } else {
       // a part of an item: sums relative to 2^m, the output sum as the values' (without F)
+      if (done) {
+        const int64_t w0 = quotient(item0, share);
+        joined.n = gw / ts - static_cast<int>(w0) + 1;
+        joined.hc = hc;
+        joined.qrow = qrow;
+        joined.slot = 2 * (w0 * ts + warp % ts);
+        joined.slot_step = 2 * ts;
+        joined.first_slot = joined.slot + (item0 > w0 * share ? 1 : 0);
+      }
       const int64_t slot = 2 * static_cast<int64_t>(gw) + (item0 <= begin ? 0 : 1);
       float* po = a.part_o + slot * 8 * D;
       float2* ml = a.part_ml + slot * 8;
@@ -703,183 +724,69 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   }
 }
 
-// The merge: joins the parts of items that several warps shared, in the order of the warps, and
-// writes zeros for decoded sequences without context.  Launched while the decode still runs; its
-// first statement waits for the decode's results.
-
-// An item as the merge sees it.
-struct MergeItem {
-  int64_t qrow, w0, share, first;  // output row; first warp team, the share, the place of the first unit
-  int n, h0, nh, sub, ts;          // parts (1: the warp wrote the output), query heads, warp in the team
-};
-
-// Item `hc` of sequence s; false where nothing is left to do but zeros (n = 0) or nothing (n = 1).
-__device__ __forceinline__ MergeItem merge_item(const DecodeFp8Args& a, int s, int hc, int warps) {
-  MergeItem it;
-  const int items = a.hkv * a.nchunks;
-  const int begin = a.cu_units[s], length = a.cu_units[s + 1] - begin, all = a.cu_units[a.S];
-  const bool decoded = a.cu_q == nullptr || a.cu_q[s + 1] - a.cu_q[s] == 1;
-  it.qrow = a.cu_q ? a.cu_q[s] : (a.query_rows ? a.query_rows[s] : s);
-  const int h = hc / a.nchunks, cch = hc - h * a.nchunks;
-  it.nh = min(8, a.group - cch * 8);
-  it.h0 = h * a.group + cch * 8;
-  it.ts = team_of(items);
-  it.sub = hc % it.ts;
-  it.n = decoded ? 0 : 1;
-  if (length == 0) return it;
-  const int ips = items / it.ts;
-  it.share = share_of(static_cast<int64_t>(all) * ips, warps / it.ts);
-  const int64_t end = static_cast<int64_t>(begin) * ips + static_cast<int64_t>(hc / it.ts + 1) * length;
-  it.first = end - length + kItemCost;
-  it.w0 = quotient(it.first, it.share);
-  it.n = static_cast<int>(quotient(end - 1, it.share) - it.w0) + 1;
-  return it;
-}
-
-__device__ __forceinline__ int64_t merge_slot(const MergeItem& it, int i) {
-  return 2 * ((it.w0 + i) * it.ts + it.sub) + (i == 0 && it.first > it.w0 * it.share ? 1 : 0);
-}
-
-// Few parts an item: one warp per item.
-constexpr int kMergeWarps = 4;
+// The merge: joins the parts of an item that several warps shared, in the order of the warps.  One
+// CTA per warp of the decode, for the item that ended in that warp's share after beginning in an
+// earlier one; the warp has left what there is to know about it.  Launched while the decode still
+// runs: its first statement waits for the decode's results.
+constexpr int kMergeWarps = 8;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kMergeWarps) merge_few_kernel(DecodeFp8Args a, int warps) {
+__global__ void __launch_bounds__(32 * kMergeWarps) merge_fp8_kernel(DecodeFp8Args a) {
+  __shared__ float4 o_s[kMergeWarps][D / 4];
+  __shared__ float2 ml_s[kMergeWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int items = a.hkv * a.nchunks;
-  const int idx = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
-  if (idx >= a.S * items) return;
-  const int s = idx / items, hc = idx - s * items;
-  if (hc == 0 && lane == 0 && a.ctx_lens[s] > a.max_ctx) flag_status(a.status, B200_DEVICE_BAD_OP);
-  const MergeItem it = merge_item(a, s, hc, warps);
-  if (it.n == 1) return;
-  T* out = static_cast<T*>(a.out) + it.qrow * a.o_srow + static_cast<int64_t>(it.h0) * a.o_shead;
-  constexpr int kVec = D / 4, kPer = 32 / kVec;  // float4s of a head, heads at a time
+  const MergeItem it = a.merge[blockIdx.x];
+  if (it.n == 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int h = it.hc / a.nchunks, cch = it.hc - h * a.nchunks;
+  const int nh = min(8, a.group - cch * 8), hq0 = h * a.group + cch * 8;
+  // warps: heads first, then groups that take every groups-th part; with D = 64 a warp's halves
+  // are groups of their own
+  constexpr int kVec = D / 4, kPer = 32 / kVec;
+  const int hh = warp % nh, grp = warp / nh, groups = kMergeWarps / nh;
   const int e = lane % kVec;
-#pragma unroll 4
-  for (int hb = 0; hb < it.nh; hb += kPer) {
-    const int hh = hb + lane / kVec;
-    const bool live = hh < it.nh;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float M = -INFINITY, L = 0.f;
-    for (int i = 0; i < it.n; ++i) {
-      const int64_t sl = merge_slot(it, i);
-      const float2 ml = live ? a.part_ml[sl * 8 + hh] : make_float2(-INFINITY, 0.f);
-      const float4 v = live ? *reinterpret_cast<const float4*>(a.part_o + (sl * 8 + hh) * D + e * 4) : o;
-      const float N = fmaxf(M, ml.x);
-      const float Nu = N == -INFINITY ? 0.f : N;
-      const float wa = fast_exp2(M - Nu), wb = fast_exp2(ml.x - Nu);
-      o.x = o.x * wa + v.x * wb;
-      o.y = o.y * wa + v.y * wb;
-      o.z = o.z * wa + v.z * wb;
-      o.w = o.w * wa + v.w * wb;
-      L = L * wa + ml.y * wb;
-      M = N;
-    }
-    if (!live) continue;
-    const float inv = L != 0.f ? 1.f / L : 0.f;
-    T* d = out + static_cast<int64_t>(hh) * a.o_shead + e * 4;
-    d[0] = from_f32<T>(o.x * inv);
-    d[1] = from_f32<T>(o.y * inv);
-    d[2] = from_f32<T>(o.z * inv);
-    d[3] = from_f32<T>(o.w * inv);
-  }
-}
-
-// Many parts an item: one CTA per item.
-constexpr int kMergeThreads = 512;
-constexpr int kMergeParts = 128;  // parts joined per pass
-
-template <typename T, int D>
-__global__ void __launch_bounds__(kMergeThreads) merge_many_kernel(DecodeFp8Args a, int warps) {
-  __shared__ float4 sum_s[kMergeThreads];
-  __shared__ float wt[8][kMergeParts];
-  __shared__ float m_s[8], l_s[8], al_s[8];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int items = a.hkv * a.nchunks;
-  const int s = blockIdx.x / items, hc = blockIdx.x - s * items;
-  if (hc == 0 && tid == 0 && a.ctx_lens[s] > a.max_ctx) flag_status(a.status, B200_DEVICE_BAD_OP);
-  const MergeItem it = merge_item(a, s, hc, warps);
-  const int n = it.n, nh = it.nh;
-  if (n == 1) return;
-  T* out = static_cast<T*>(a.out) + it.qrow * a.o_srow + static_cast<int64_t>(it.h0) * a.o_shead;
-  if (n == 0) {
-    for (int i = tid; i < nh * D; i += kMergeThreads) out[(i / D) * a.o_shead + i % D] = from_f32<T>(0.f);
-    return;
-  }
-  constexpr int kVec = D / 4;       // float4s of a head
-  const int lanes = nh * kVec;
-  const int groups = kMergeThreads / lanes;
-  const int grp = tid / lanes, e = tid - grp * lanes;
-  const int hh = e / kVec;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < n; p0 += kMergeParts) {
-    const int np = min(kMergeParts, n - p0);
-    for (int w8 = warp; w8 < nh; w8 += kMergeThreads / 32) {
-      // head w8's reference, the parts' weights, the sum of p
-      float mine[kMergeParts / 32], l[kMergeParts / 32];
-      float M = p0 == 0 ? -INFINITY : m_s[w8];
-      const float M_old = M;
+  float M = -INFINITY, L = 0.f;
+  const auto add = [&](float2 ml, float4 v) {
+    const float N = fmaxf(M, ml.x);
+    const float Nu = N == -INFINITY ? 0.f : N;
+    const float wa = fast_exp2(M - Nu), wb = fast_exp2(ml.x - Nu);
+    o.x = o.x * wa + v.x * wb;
+    o.y = o.y * wa + v.y * wb;
+    o.z = o.z * wa + v.z * wb;
+    o.w = o.w * wa + v.w * wb;
+    L = L * wa + ml.y * wb;
+    M = N;
+  };
+  if (grp < groups) {
+    constexpr int U = 4;
+    const int step = groups * kPer;
+    for (int i0 = grp * kPer + lane / kVec; i0 < it.n; i0 += U * step) {
+      float2 ml[U];
+      float4 v[U];
 #pragma unroll
-      for (int j = 0; j < kMergeParts / 32; ++j) {
-        const int i = lane + 32 * j;
-        const float2 ml = i < np ? a.part_ml[merge_slot(it, p0 + i) * 8 + w8] : make_float2(-INFINITY, 0.f);
-        mine[j] = ml.x;
-        l[j] = ml.y;
-        M = fmaxf(M, ml.x);
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * step;
+        const int64_t sl = i == 0 ? it.first_slot : it.slot + static_cast<int64_t>(i) * it.slot_step;
+        ml[u] = i < it.n ? a.part_ml[sl * 8 + hh] : make_float2(-INFINITY, 0.f);
+        v[u] = i < it.n ? *reinterpret_cast<const float4*>(a.part_o + (sl * 8 + hh) * D + e * 4)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-      const float Mu = M == -INFINITY ? 0.f : M;
-      float L = 0.f;
-#pragma unroll
-      for (int j = 0; j < kMergeParts / 32; ++j) {
-        const float w = fast_exp2(mine[j] - Mu);
-        wt[w8][lane + 32 * j] = w;
-        L += w * l[j];
-      }
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-      if (lane == 0) {
-        const float al = fast_exp2(M_old - Mu);
-        m_s[w8] = M;
-        al_s[w8] = al;
-        l_s[w8] = (p0 == 0 ? 0.f : l_s[w8] * al) + L;
-      }
+      for (int u = 0; u < U; ++u) add(ml[u], v[u]);
     }
-    __syncthreads();
-    if (grp < groups) {
-      const float al = p0 == 0 ? 0.f : al_s[hh];
-      o.x *= al;
-      o.y *= al;
-      o.z *= al;
-      o.w *= al;
-#pragma unroll 4
-      for (int i = grp; i < np; i += groups) {
-        const float4 v = *reinterpret_cast<const float4*>(a.part_o + (merge_slot(it, p0 + i) * 8 + hh) * D + (e % kVec) * 4);
-        const float w = wt[hh][i];
-        o.x = fmaf(v.x, w, o.x);
-        o.y = fmaf(v.y, w, o.y);
-        o.z = fmaf(v.z, w, o.z);
-        o.w = fmaf(v.w, w, o.w);
-      }
-    }
-    __syncthreads();
+    if (kPer == 2)
+      add(make_float2(__shfl_xor_sync(0xffffffffu, M, 16), __shfl_xor_sync(0xffffffffu, L, 16)),
+          make_float4(__shfl_xor_sync(0xffffffffu, o.x, 16), __shfl_xor_sync(0xffffffffu, o.y, 16),
+                      __shfl_xor_sync(0xffffffffu, o.z, 16), __shfl_xor_sync(0xffffffffu, o.w, 16)));
+    if (lane < kVec) o_s[warp][lane] = o;
+    if (lane == 0) ml_s[warp] = make_float2(M, L);
   }
-  sum_s[tid] = o;
   __syncthreads();
-  if (grp == 0) {
-    for (int g = 1; g < groups; ++g) {
-      const float4 v = sum_s[g * lanes + e];
-      o.x += v.x;
-      o.y += v.y;
-      o.z += v.z;
-      o.w += v.w;
-    }
-    const float inv = l_s[hh] != 0.f ? 1.f / l_s[hh] : 0.f;
-    T* d = out + static_cast<int64_t>(hh) * a.o_shead + (e % kVec) * 4;
+  if (grp == 0 && lane < kVec) {
+    for (int g = 1; g < groups; ++g) add(ml_s[g * nh + hh], o_s[g * nh + hh][lane]);
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+    T* d = static_cast<T*>(a.out) + it.qrow * a.o_srow + static_cast<int64_t>(hq0 + hh) * a.o_shead + e * 4;
     d[0] = from_f32<T>(o.x * inv);
     d[1] = from_f32<T>(o.y * inv);
     d[2] = from_f32<T>(o.z * inv);
@@ -908,21 +815,13 @@ cudaError_t launch_t(const CUtensorMap& km, const CUtensorMap& vm, const DecodeF
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  const int items = a.hkv * a.nchunks;
-  // the parts of an item, on average: a warp joins few of them while a CTA would still start up
-  const int64_t parts = static_cast<int64_t>(grid) * kWarps / (static_cast<int64_t>(a.S) * items) + 1;
   cudaLaunchConfig_t cfg{};
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (parts > 6) {
-    cfg.gridDim = dim3(a.S * items);
-    cfg.blockDim = dim3(kMergeThreads);
-    return cudaLaunchKernelEx(&cfg, merge_many_kernel<T, D>, a, grid * kWarps);
-  }
-  cfg.gridDim = dim3((a.S * items + kMergeWarps - 1) / kMergeWarps);
+  cfg.gridDim = dim3(grid * kWarps);
   cfg.blockDim = dim3(32 * kMergeWarps);
-  return cudaLaunchKernelEx(&cfg, merge_few_kernel<T, D>, a, grid * kWarps);
+  return cudaLaunchKernelEx(&cfg, merge_fp8_kernel<T, D>, a);
 }
 
 template <typename T, bool SPLIT>

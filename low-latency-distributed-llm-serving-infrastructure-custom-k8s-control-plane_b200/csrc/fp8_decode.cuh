@@ -7,6 +7,12 @@ namespace b200 {
 
 constexpr int kDecodeFp8MaxSeqs = 1024;  // sequences of one launch (their unit sums sit in shared memory)
 
+// An item that the merge joins: its parts lie at first_slot and at slot + i * slot_step.
+struct MergeItem {
+  int64_t qrow, slot, first_slot;
+  int32_t n, hc, slot_step, pad;
+};
+
 struct DecodeFp8Args {
   const void* q;
   int64_t q_srow, q_shead;
@@ -24,8 +30,8 @@ struct DecodeFp8Args {
   void* out;
   int64_t o_srow, o_shead;
   int32_t* status;
-  // workspace: prefix sums of units, and two parts per warp: 8 heads of (m, l) and of D sums
-  int32_t* cu_units;
+  // workspace: an item to join per warp, and two parts per warp: 8 heads of (m, l) and of D sums
+  MergeItem* merge;
   float2* part_ml;
   float* part_o;
 };
