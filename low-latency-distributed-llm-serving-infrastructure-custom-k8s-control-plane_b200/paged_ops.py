@@ -350,7 +350,7 @@ def fp8_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scale: tor
         raise ValueError("value_cache must have the key cache's shape and dtype")
     L, NB, BS, H, D = key_cache.shape
     want = (L, NB, H)
-    if key_scale.shape != want or value_scale.shape != want:
+    if key_scale.shape != want or value_scale.shape != want:  # (equal to a plain tuple)
         raise ValueError(f"scales must be (layers, blocks, heads) = {want}")
     if key_scale.dtype != torch.float32 or value_scale.dtype != torch.float32:
         raise ValueError("scales must be float32")
@@ -501,49 +501,44 @@ def attention_fp8_params(query, key_cache, value_cache, key_scale, value_scale, 
                          block_tables, context_lens, scale, out, max_context_len, query_rows=None,
                          cu_seqlens=None, max_query_len=0, prefill_blocks=-1):
     """The C struct of an attention call over an 8-bit cache; checks what the struct cannot say."""
-    p = N.AttentionFp8Params()
-    p.cache = fp8_cache(key_cache, value_cache, key_scale, value_scale, layer_idx)
-    if query.dim() != 3 or query.stride(-1) != 1:
+    cache = fp8_cache(key_cache, value_cache, key_scale, value_scale, layer_idx)
+    q_shape, q_stride = query.shape, query.stride()
+    if len(q_shape) != 3 or q_stride[2] != 1:
         raise ValueError("query must be (rows, Hq, D) with the head dim contiguous")
-    if query.shape[2] != p.cache.head_dim:
-        raise ValueError(f"query head dim {query.shape[2]} != cache head dim {p.cache.head_dim}")
-    p.dtype = _dtype_code(query, "query")
-    if out.dtype != query.dtype or out.shape != query.shape or out.stride(-1) != 1:
+    if q_shape[2] != key_cache.shape[4]:
+        raise ValueError(f"query head dim {q_shape[2]} != cache head dim {key_cache.shape[4]}")
+    code = _dtype_code(query, "query")
+    o_stride = out.stride()
+    if out.dtype != query.dtype or out.shape != q_shape or o_stride[2] != 1:
         raise ValueError("out must have the query's shape and dtype, the head dim contiguous")
     if block_tables.dtype != torch.int32 or context_lens.dtype != torch.int32:
         raise ValueError("block_tables and context_lens must be int32")
-    if block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+    bt_shape, bt_stride = block_tables.shape, block_tables.stride()
+    if len(bt_shape) != 2 or (bt_shape[1] > 1 and bt_stride[1] != 1):
         raise ValueError("block_tables must be (S, max_blocks) with unit stride along a row")
     if context_lens.dim() != 1 or not context_lens.is_contiguous():
         raise ValueError("context_lens must be a contiguous (S,) tensor")
     S = context_lens.shape[0]
-    if block_tables.shape[0] < S:
+    if bt_shape[0] < S:
         raise ValueError("block_tables has fewer rows than context_lens has sequences")
-    if S > 1 and block_tables.stride(0) < block_tables.shape[1]:
+    if S > 1 and bt_stride[0] < bt_shape[1]:
         raise ValueError("block_tables rows must not overlap")
     if query_rows is not None and (query_rows.dtype != torch.int32 or query_rows.shape != (S,) or
                                    not query_rows.is_contiguous()):
         raise ValueError("query_rows must be int32 with one entry per sequence")
     if cu_seqlens is None:
-        if query_rows is None and query.shape[0] < S:
-            raise ValueError(f"query has {query.shape[0]} rows, the batch needs {S}")
+        if query_rows is None and q_shape[0] < S:
+            raise ValueError(f"query has {q_shape[0]} rows, the batch needs {S}")
     elif (cu_seqlens.dtype != torch.int64 or cu_seqlens.shape != (S + 1,) or
           not cu_seqlens.is_contiguous()):
         raise ValueError("cu_seqlens must be a contiguous int64 (S+1,) tensor")
-    p.query, p.q_stride_row, p.q_stride_head = query.data_ptr(), query.stride(0), query.stride(1)
-    p.out, p.o_stride_row, p.o_stride_head = out.data_ptr(), out.stride(0), out.stride(1)
-    p.num_query_heads = query.shape[1]
-    p.block_tables, p.block_table_stride = block_tables.data_ptr(), block_tables.shape[1]
-    if S > 1:
-        p.block_table_stride = block_tables.stride(0)
-    p.context_lens, p.num_seqs = context_lens.data_ptr(), S
     # no sequence reaches past its row of the table
-    p.max_context_len = min(int(max_context_len), block_tables.shape[1] * p.cache.block_size)
-    p.scale = float(scale)
-    p.query_rows, p.cu_seqlens = _ptr(query_rows), _ptr(cu_seqlens)
-    p.num_tokens, p.max_query_len = query.shape[0], int(max_query_len)
-    p.prefill_blocks = int(prefill_blocks)
-    return p
+    most = min(int(max_context_len), bt_shape[1] * key_cache.shape[2])
+    return N.AttentionFp8Params(
+        cache, query.data_ptr(), q_stride[0], q_stride[1], out.data_ptr(), o_stride[0],
+        o_stride[1], code, q_shape[1], block_tables.data_ptr(),
+        bt_stride[0] if S > 1 else bt_shape[1], context_lens.data_ptr(), S, most, float(scale),
+        _ptr(query_rows), _ptr(cu_seqlens), q_shape[0], int(max_query_len), int(prefill_blocks))
 
 
 def paged_decode_fp8(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
