@@ -25,11 +25,13 @@ constexpr int kAppendWarps = kAppendThreads / 32;
 constexpr int kChunkRows = 16;    // rows of a block handled per pass
 constexpr int kMaxBlockSize = 1024;
 
-// cos and sin of pos * inv_freq, each in two parts (hi + lo).  The product is formed and reduced
-// to [-pi/4, pi/4] in 64 bits (at position 30,000 a 32-bit product alone is off by 1e-3 rad) and
-// the Taylor series there end with a remainder below 2e-14.
-struct Turn {
-  float ch, sh, cl, sl;
+// cos and sin of pos * inv_freq in 64 bits.  The product is formed and reduced to [-pi/4, pi/4] in
+// 64 bits (at position 30,000 a 32-bit product alone is off by 1e-3 rad) and the Taylor series there
+// end with a remainder below 2e-14.  Keys are rotated in 64 bits too, so that each lands on the code
+// of its exact value: two products an element, less than fp32 arithmetic in two parts (12
+// operations).
+struct __align__(16) Turn {
+  double c, s;
 };
 __device__ __forceinline__ Turn turn_of(int64_t pos, float inv_freq) {
   const double a = static_cast<double>(pos) * static_cast<double>(inv_freq);
@@ -62,23 +64,14 @@ __device__ __forceinline__ Turn turn_of(int64_t pos, float inv_freq) {
     s = -s;
     c = -c;
   }
-  Turn t;
-  t.ch = static_cast<float>(c);
-  t.cl = static_cast<float>(c - t.ch);
-  t.sh = static_cast<float>(s);
-  t.sl = static_cast<float>(s - t.sh);
-  return t;
+  return Turn{c, s};
 }
 
-// x * c + y * s rounded once from twice fp32's precision (products split by fma, two-sum), so that
-// a rotated key lands on the same code as its 64-bit value.
-__device__ __forceinline__ float mul_add2(float x, float ch, float cl, float y, float sh, float sl) {
-  const float p = __fmul_rn(x, ch), q = __fmul_rn(y, sh);
-  const float e = fmaf(x, cl, fmaf(x, ch, -p)) + fmaf(y, sl, fmaf(y, sh, -q));
-  const float d = __fadd_rn(p, q);
-  const float bb = __fsub_rn(d, p);
-  const float err = __fadd_rn(__fsub_rn(p, __fsub_rn(d, bb)), __fsub_rn(q, bb));
-  return __fadd_rn(d, err + e);
+// Rotates the pair (x, y) and rounds it once to fp32.
+__device__ __forceinline__ void rotate(const Turn& t, float& x, float& y) {
+  const double u = x, v = y;
+  x = static_cast<float>(u * t.c - v * t.s);
+  y = static_cast<float>(v * t.c + u * t.s);
 }
 
 // Smallest power of two s with amax <= 448 s (448 = 1.75 * 2^8), at least 2^-100.
@@ -96,6 +89,7 @@ __device__ __forceinline__ bool is_pow2(float s) {
 struct RowList {
   int32_t row[kChunkRows];
   int32_t off[kChunkRows];
+  bool last[kChunkRows];  // the last of the list's rows with its slot
   int32_t n;
   int32_t next;  // row to go on from
 };
@@ -154,7 +148,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_fp8_kernel(AppendFp8Arg
     for (int w = tid; w < (r1 - r0) * half; w += kAppendThreads) {
       const int r = w / half, i = w - r * half;
       const Turn t = turn_of(a.positions[r0 + r], a.inv_freq[i]);
-      cs[w] = make_float2(t.ch, t.sh);
+      cs[w] = make_float2(static_cast<float>(t.c), static_cast<float>(t.s));
     }
     __syncthreads();
     const int per_row = a.hq * half;
@@ -224,10 +218,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_fp8_kernel(AppendFp8Arg
         const T* k = static_cast<const T*>(a.key) + list.row[r] * a.k_stok + h * a.k_shead;
         x1 = to_f32<T>(k[d]);
         if (ROPE) {
-          const float y = to_f32<T>(k[d + half]);
-          const Turn w = cs[r * half + d];
-          x2 = mul_add2(y, w.ch, w.cl, x1, w.sh, w.sl);
-          x1 = mul_add2(x1, w.ch, w.cl, -y, w.sh, w.sl);
+          x2 = to_f32<T>(k[d + half]);
+          rotate(cs[r * half + d], x1, x2);
         }
       }
     };
@@ -349,10 +341,8 @@ __device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
   reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-// Two values' codes; what is not finite becomes NaN.
+// Two values' codes (no infinities among them).
 __device__ __forceinline__ uint32_t codes2(float x, float y) {
-  x = fabsf(x) < INFINITY ? x : NAN;
-  y = fabsf(y) < INFINITY ? y : NAN;
   return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
 }
 
@@ -388,7 +378,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4)
     float2* cs = reinterpret_cast<float2*>(sm);  // [q_rows][kHalf]
     for (int w = tid; w < rows * kHalf; w += kAppendThreads) {
       const Turn t = turn_of(a.positions[r0 + w / kHalf], a.inv_freq[w % kHalf]);
-      cs[w / kHalf * kHalf + place(w % kHalf)] = make_float2(t.ch, t.sh);
+      cs[w / kHalf * kHalf + place(w % kHalf)] = make_float2(static_cast<float>(t.c), static_cast<float>(t.s));
     }
     __syncthreads();
     const int c = tid % LPR, row = (tid / LPR) % q_rows, groups = kAppendThreads / (LPR * q_rows);
@@ -454,6 +444,9 @@ __global__ void __launch_bounds__(kAppendThreads, 4)
       if (tid < list.n) {
         atomicOr(&written[list.off[tid] >> 5], 1u << (list.off[tid] & 31));
         if (list.off[tid] == 0) fresh_s = 1;
+        bool last = true;
+        for (int k = tid + 1; k < list.n; ++k) last &= list.off[k] != list.off[tid];
+        list.last[tid] = last;
       }
       if (ROPE) {
         for (int w = tid; w < list.n * kHalf; w += kAppendThreads)
@@ -483,28 +476,31 @@ __global__ void __launch_bounds__(kAppendThreads, 4)
           const int r = r0 + p * RPP + rs;
           if (r < list.n) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const Turn w = cs[r * kHalf + i * LPR + c];
-              const float u = x[p][0][i], v = x[p][1][i];
-              x[p][0][i] = mul_add2(u, w.ch, w.cl, -v, w.sh, w.sl);
-              x[p][1][i] = mul_add2(v, w.ch, w.cl, u, w.sh, w.sl);
-            }
+            for (int i = 0; i < 8; ++i) rotate(cs[r * kHalf + i * LPR + c], x[p][0][i], x[p][1][i]);
           }
         }
       }
     };
-    const auto largest = [&](const float (&x)[P][2][8]) {
+    // the warp's largest finite |x|; infinities become NaN on the way, which is what they are held as
+    const auto largest = [&](float (&x)[P][2][8]) {
       float m = 0.f;
+      for (int again = 0; again < 2; ++again) {
+        m = 0.f;
 #pragma unroll
-      for (int p = 0; p < P; ++p)
+        for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float u = fabsf(x[p][0][i]), v = fabsf(x[p][1][i]);
-          if (u < INFINITY) m = fmaxf(m, u);  // false for NaN too
-          if (v < INFINITY) m = fmaxf(m, v);
-        }
+          for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(x[p][0][i]), fabsf(x[p][1][i])));  // NaN apart
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (m < INFINITY) break;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[p][0][i] = fabsf(x[p][0][i]) < INFINITY ? x[p][0][i] : NAN;
+            x[p][1][i] = fabsf(x[p][1][i]) < INFINITY ? x[p][1][i] : NAN;
+          }
+      }
       return m;
     };
     const int64_t cache_blk = static_cast<int64_t>(a.layer) * a.nb + blk;
@@ -555,11 +551,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4)
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         const int r = r0 + p * RPP + rs;
-        bool live = r < list.n;
-        // of rows with one slot only the last is stored
-        if (live)
-          for (int k = r + 1; k < list.n; ++k) live &= list.off[k] != list.off[r];
-        if (!live) continue;
+        if (r >= list.n || !list.last[r]) continue;
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const float(&y)[8] = x[p][hf];
@@ -621,8 +613,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4)
           for (int h0 = 0; h0 < kChunkRows; h0 += kChunkRows / 2) {
             float x[P][2][8];
             load(task, h0, x);
+            const float m = largest(x);
             if (pass == 0) {
-              const float m = largest(x);
               if (lane == 0) amax[task] = fmaxf(amax[task], m);
             } else {
               store(task, h0, amax[task], x);
