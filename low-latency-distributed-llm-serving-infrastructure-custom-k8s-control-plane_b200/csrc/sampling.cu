@@ -611,6 +611,10 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
   };
   const auto sum32_all = [&]() { return static_cast<double>(head->sum32) * 0x1p-38; };
   const auto finish = [&](int token, double sum_all) {
+    if (token < 0 || token >= V) {  // none was found: left to sample_row_kernel
+      a.tokens[row] = kTodo;
+      return;
+    }
     a.tokens[row] = token;
     if (a.logprobs) {
       const float v = logit<T>(x0[token]);

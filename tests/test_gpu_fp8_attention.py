@@ -195,6 +195,65 @@ def test_decode_streams_and_graphs_share_a_workspace(ops):
             _close(out, torch.bfloat16, s[5], s[4], D, 11)
 
 
+@pytest.mark.parametrize("dtype", ALL)
+def test_more_sequences_than_one_launch_takes(ops, dtype):
+    g = torch.Generator().manual_seed(5)
+    ctx = torch.randint(0, 40, (2300,), generator=g).tolist()
+    q, cache, tables, cu, lens = _batch(ctx, [1] * 2300, 4, 2, 64, 16, dtype, seed=1)
+    ref = R.attend(q, *cache, 0, tables, cu, ctx, 0.125)
+    dev = [t.cuda() for t in cache]
+    got = ops.paged_decode_fp8(q.cuda(), *dev, 0, tables.cuda(), lens.cuda(), 0.125, 40)
+    _close(got, dtype, ref, ctx, 64, DECODE_BITS[dtype])
+    rows = torch.randperm(2300, generator=g).int()
+    back = torch.empty_like(q)
+    back[rows.long()] = q
+    got = ops.paged_decode_fp8(back.cuda(), *dev, 0, tables.cuda(), lens.cuda(), 0.125, 40, query_rows=rows.cuda())
+    _close(got[rows.long().cuda()], dtype, ref, ctx, 64, DECODE_BITS[dtype])
+    # a mixed step of as many: every 100th sequence has a chunk of new tokens
+    new = [min(c, 7) if i % 100 == 50 else min(c, 1) for i, c in enumerate(ctx)]
+    cu = torch.tensor([0] + new).cumsum(0)
+    q = torch.randn(int(cu[-1]), 4, 64, generator=g).to(dtype)
+    ref = R.attend(q, *cache, 0, tables, cu, ctx, 0.125)
+    got = ops.paged_prefill_fp8(q.cuda(), *dev, 0, tables.cuda(), cu.cuda(), lens.cuda(), 0.125, 7, 40)
+    _close(got, dtype, ref, ctx, 64, PREFILL_BITS[dtype])
+
+
+def test_captured_append_and_prefill(ops):
+    """An append of over 1024 rows and the prefill that reads it, captured and replayed on new values."""
+    hq, H, D, BS, n = 8, 2, 64, 16, 1300
+    kc, vc = (torch.zeros(1, 90, BS, H, D, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+    ks, vs = (torch.zeros(1, 90, H, device="cuda") for _ in range(2))
+    cache = (kc, vc, ks, vs, 0)
+    table = torch.randperm(90, device="cuda").int()[None, :82].contiguous()
+    pos = torch.arange(n, device="cuda")
+    slots = table[0].long()[pos // BS] * BS + pos % BS
+    inv = 1.0 / (10000.0 ** (torch.arange(0, D, 2, dtype=torch.float32, device="cuda") / D))
+    cu, ctx = torch.tensor([0, n], device="cuda"), torch.tensor([n], dtype=torch.int32, device="cuda")
+    qkv = torch.zeros(n, (hq + 2 * H) * D, device="cuda", dtype=torch.bfloat16)
+
+    def step():
+        q = ops.rope_reshape_and_cache_fp8(qkv, pos, inv, hq, *cache, slots)
+        return q, ops.paged_prefill_fp8(q, *cache, table, cu, ctx, 0.125, n, n, prefill_blocks=82)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, out = step()
+    for seed in range(2):
+        qkv.copy_(torch.randn(qkv.shape, generator=torch.Generator().manual_seed(seed)).bfloat16())
+        graph.replay()
+        ref = R.attend(q.cpu(), *[t.cpu() for t in cache[:4]], 0, table.cpu(), [0, n], [n], 0.125)
+        _close(out, torch.bfloat16, ref, [n], D, PREFILL_BITS[torch.bfloat16])
+        want = R.rotate(qkv.cpu().view(n, -1, D)[:, hq:hq + H], pos.cpu(), inv.cpu())
+        k, _ = ops.gather_cache_fp8(*cache, slots, torch.float32)
+        assert ((k.cpu().double() - want).abs() <= want.abs() * 2.0 ** -4 + 2.0 ** -14).all()
+    assert ops.read_status(torch.device("cuda")) == 0
+
+
 def test_decode_results_repeat(ops):
     q, cache, tables, cu, lens = _batch([9000, 300, 4000], [1] * 3, 8, 2, 128, 16, torch.bfloat16, seed=3)
     args = (q.cuda(), *[t.cuda() for t in cache], 0, tables.cuda(), lens.cuda(), 0.09, 9000)

@@ -59,6 +59,29 @@ def test_random_rows(sampling, dtype, vocab):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_lists_and_flat_rows(sampling, dtype):
+    """Top-k beyond what is counted out, beyond what is sorted and beyond one step; rows so flat that a
+    step holds thousands of tokens; temperatures from 0.05 to 50."""
+    rng = np.random.default_rng(7)
+    x = torch.from_numpy(rng.normal(0, 2.5, (20, 60000)).astype(np.float32)).to(dtype)
+    x[10:] *= 0.1
+    u = rng.random(20, dtype=np.float32).tolist()
+    k = [300, 384, 385, 400, 700, 1000, 1024, 1025, 5000, 59999] * 2
+    _check(sampling, x, u, k=k)
+    _check(sampling, x, u, k=k, p=[0.9] * 20)
+    _check(sampling, x, u, t=[float(t) for t in np.geomspace(0.05, 50, 20)], p=[0.97] * 20)
+    _check(sampling, x, u, p=[0.5, 0.9, 0.99, 0.999, 0.9999, 0.99999, 1 - 2.0 ** -23, 0.01, 1e-6, 0.7] * 2)
+    _check(sampling, x, u, t=[0.3] * 20, k=[2000] * 20, p=[0.95] * 20, m=[1e-4] * 20)
+
+
+def test_vocabularies_beyond_the_clusters_memory(sampling):
+    rng = np.random.default_rng(3)
+    x = torch.from_numpy(rng.normal(0, 3, (3, 500001)).astype(np.float32))
+    _check(sampling, x, [0.2, 0.6, 0.9], k=[0, 50, 0], p=[0.8, 1.0, 1.0])
+    _check(sampling, x[:, :392000], [0.2, 0.6, 0.9], k=[0, 50, 0], p=[0.8, 1.0, 1.0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_ties_go_to_the_lowest_index(sampling, dtype):
     x = torch.zeros(40, 2000)
     x[:, 500:1500] = 1.0
@@ -131,6 +154,22 @@ def test_strided_rows_and_graph(sampling):
         g.replay()
         now = sampling.sample(x, u, top_p=p)
         assert torch.equal(got[0], now[0]) and torch.equal(got[1], now[1])
+
+
+def test_two_streams_at_once(sampling):
+    x = [torch.randn(40, 30000 + i).cuda() for i in range(2)]
+    u = torch.rand(40).cuda()
+    p = torch.full((40,), 0.9).cuda()
+    want = [sampling.sample(t, u, top_p=p)[0] for t in x]
+    streams = [torch.cuda.Stream() for _ in x]
+    for _ in range(20):
+        got = []
+        for st, t in zip(streams, x):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append(sampling.sample(t, u, top_p=p)[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_draws_follow_the_distribution(sampling):
