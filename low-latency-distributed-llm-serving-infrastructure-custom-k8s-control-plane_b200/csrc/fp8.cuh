@@ -97,7 +97,6 @@ struct ExpandFp8Args {
   const int64_t* cu_q;
   int32_t S, max_ctx;
   int32_t scratch_blocks, scratch_stride;
-  int32_t* offsets;        // (S + 1): first scratch block of each sequence
   int32_t* scratch_ctx;    // (S)
   int32_t* scratch_table;  // (S, scratch_stride)
   void* k16;

@@ -216,7 +216,7 @@ struct PrefillPlan {
   bool tensor_cores;
   DecodePlan decode;
   int32_t blocks, stride, max_ctx;
-  size_t off_offsets, off_ctx, off_table, off_chunks, chunk_bytes, off_k, off_v, total;
+  size_t off_ctx, off_table, off_chunks, chunk_bytes, off_k, off_v, total;
 };
 
 // The 16-bit prefill's parameters over the copy at `ws`.
@@ -270,7 +270,6 @@ PrefillPlan prefill_plan(const B200AttentionFp8Params& p) {
     off += align256(bytes);
     return at;
   };
-  pl.off_offsets = take((static_cast<size_t>(p.num_seqs) + 1) * 4);
   pl.off_ctx = take(static_cast<size_t>(p.num_seqs) * 4);
   pl.off_table = take(static_cast<size_t>(p.num_seqs) * pl.stride * 4);
   pl.off_chunks = take(pl.chunk_bytes);
@@ -304,7 +303,6 @@ int run_prefill(const B200AttentionFp8Params& p, const PrefillPlan& pl, char* ws
   a.max_ctx = pl.max_ctx;
   a.scratch_blocks = pl.blocks;
   a.scratch_stride = pl.stride;
-  a.offsets = reinterpret_cast<int32_t*>(ws + pl.off_offsets);
   a.scratch_ctx = reinterpret_cast<int32_t*>(ws + pl.off_ctx);
   a.scratch_table = reinterpret_cast<int32_t*>(ws + pl.off_table);
   a.k16 = ws + pl.off_k;

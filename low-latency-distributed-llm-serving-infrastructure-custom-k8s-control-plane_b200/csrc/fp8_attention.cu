@@ -3,7 +3,6 @@
 #include <type_traits>
 
 #include "api_common.cuh"
-#include "cache_ops.cuh"
 #include "fp8.cuh"
 
 namespace b200 {
@@ -151,34 +150,6 @@ cudaError_t launch_row_t(const AttnFp8Args& a, int rows, cudaStream_t stream) {
 
 // ---- the 16-bit copy of a prefill's pages -----------------------------------------------------
 
-// Scratch blocks of each sequence with more than one new token: one CTA.
-__global__ void __launch_bounds__(1024) expand_plan_kernel(ExpandFp8Args a) {
-  __shared__ int64_t warp_buf[32];
-  __shared__ int64_t total;
-  int64_t carry = 0;
-  for (int base = 0; base < a.S; base += 1024) {
-    const int s = base + threadIdx.x;
-    int64_t n = 0;
-    if (s < a.S) {
-      int32_t ctx = a.ctx_lens[s];
-      if (ctx > a.max_ctx) {
-        flag_status(a.status, B200_DEVICE_BAD_OP);
-        ctx = a.max_ctx;
-      }
-      a.scratch_ctx[s] = ctx;
-      if (a.cu_q[s + 1] - a.cu_q[s] > 1 && ctx > 0) n = (ctx + a.bs - 1) / a.bs;
-    }
-    const int64_t before = block_exclusive_scan_1024(n, warp_buf, &total) + carry;
-    if (s < a.S) a.offsets[s] = static_cast<int32_t>(before < a.scratch_blocks ? before : a.scratch_blocks);
-    carry += total;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    if (carry > a.scratch_blocks) flag_status(a.status, B200_DEVICE_BAD_STEP);
-    a.offsets[a.S] = static_cast<int32_t>(carry < a.scratch_blocks ? carry : a.scratch_blocks);
-  }
-}
-
 // 16 codes at scale s in 16 bits: exact for bf16 with power-of-two scales; f16 values beyond its
 // range become +-65504.
 template <typename T>
@@ -200,26 +171,78 @@ __device__ __forceinline__ void widen16(uint4 c, float s, uint4 (&out)[2]) {
   out[1] = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
-// Each CTA copies an equal share of the scratch blocks, 16 codes per thread and step.  Bound by
-// memory: 1 byte read and 2 written per entry.
+// Each CTA copies an equal share of the scratch blocks, 16 codes per thread and step.  Every CTA
+// sums up the sequences' blocks by itself, 256 sequences at a time (1 us for a few hundred; a
+// kernel of its own for the sums took 4 us and a launch).  Bound by memory: 1 byte read and 2
+// written per entry.
 template <typename T>
 __global__ void __launch_bounds__(256) expand_kernel(ExpandFp8Args a) {
-  const int total = a.offsets[a.S];
-  const int per = (total + gridDim.x - 1) / gridDim.x;
-  const int b0 = blockIdx.x * per, b1 = min(total, b0 + per);
-  if (b0 >= b1) return;
-  int lo = 0, hi = a.S - 1;  // the sequence of b0: the last one that begins at or before it
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.offsets[mid] <= b0) lo = mid; else hi = mid - 1;
+  __shared__ int32_t warp_n[8];
+  __shared__ int32_t found_s, before_s;  // the sequence of the share's first block, its own first
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const auto blocks_of = [&](int s) -> int32_t {
+    const int32_t ctx = min(a.ctx_lens[s], a.max_ctx);
+    return a.cu_q[s + 1] - a.cu_q[s] > 1 && ctx > 0 ? (ctx + a.bs - 1) / a.bs : 0;
+  };
+  int64_t total = 0;
+  for (int s = tid; s < a.S; s += 256) {
+    total += blocks_of(s);
+    if (blockIdx.x == 0) {
+      if (a.ctx_lens[s] > a.max_ctx) flag_status(a.status, B200_DEVICE_BAD_OP);
+      a.scratch_ctx[s] = min(a.ctx_lens[s], a.max_ctx);
+    }
   }
-  int seq = lo;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  __shared__ int64_t warp_total[8];
+  if (lane == 0) warp_total[warp] = total;
+  if (tid == 0) found_s = -1;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < 8; ++w) total += warp_total[w];
+  if (total > a.scratch_blocks) {
+    if (blockIdx.x == 0 && tid == 0) flag_status(a.status, B200_DEVICE_BAD_STEP);
+    total = a.scratch_blocks;
+  }
+  const int per = static_cast<int>((total + gridDim.x - 1) / gridDim.x);
+  const int b0 = static_cast<int>(min(total, static_cast<int64_t>(blockIdx.x) * per));
+  const int b1 = static_cast<int>(min(total, static_cast<int64_t>(b0) + per));
+  if (b0 >= b1) return;
+  // the sequence of block b0
+  int64_t carry = 0;
+  for (int base = 0; base < a.S; base += 256) {
+    const int s = base + tid;
+    const int32_t n = s < a.S ? blocks_of(s) : 0;
+    int32_t x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t t = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += t;
+    }
+    if (lane == 31) warp_n[warp] = x;
+    __syncthreads();
+    int64_t before = carry + x - n;
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) before += warp_n[w];
+      carry += warp_n[w];
+    }
+    if (n > 0 && before <= b0 && b0 < before + n) {
+      found_s = s;
+      before_s = static_cast<int32_t>(before);
+    }
+    __syncthreads();
+    if (found_s >= 0) break;
+  }
+  int seq = found_s, first = before_s, held = blocks_of(seq);
   const int64_t block_bytes = static_cast<int64_t>(a.bs) * a.hkv * a.head_dim;
   const int chunks = static_cast<int>(block_bytes / 16);
   const int head_chunks = a.head_dim / 16;
   for (int b = b0; b < b1; ++b) {
-    while (a.offsets[seq + 1] <= b) ++seq;
-    const int j = b - a.offsets[seq];
+    while (b >= first + held) {
+      first += held;
+      held = blocks_of(++seq);
+    }
+    const int j = b - first;
     int32_t src = a.bt[static_cast<int64_t>(seq) * a.bt_stride + j];
     const bool good = src >= 0 && src < a.nb;
     if (threadIdx.x == 0) {
@@ -255,9 +278,6 @@ __global__ void __launch_bounds__(256) expand_kernel(ExpandFp8Args a) {
 }  // namespace
 
 cudaError_t launch_expand_fp8(const ExpandFp8Args& a, int dtype, int num_sms, cudaStream_t stream) {
-  expand_plan_kernel<<<1, 1024, 0, stream>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   const int grid = a.scratch_blocks < num_sms * 8 ? a.scratch_blocks : num_sms * 8;
   if (dtype == B200_DTYPE_BF16) expand_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a);
   else if (dtype == B200_DTYPE_F16) expand_kernel<__half><<<grid, 256, 0, stream>>>(a);
