@@ -36,8 +36,12 @@ constexpr int kWarps = 4;  // consumer warps
 constexpr int kCtasPerSm = 3;
 constexpr int kThreads = 32 * (kWarps + 1);  // the last warp loads for the others
 constexpr int kUnit = 32;      // tokens
-constexpr int kMinShare = 4;   // places on the line per warp at least: a shorter share costs more in the merge
-constexpr int kItemCost = 3;   // what beginning an item costs, in units: part of its length on the line
+// Places on the line per warp at least.  In us, for 1 | 2 | 4: one sequence of 512 tokens 11.0 | 10.7 |
+// 12.5, of 4096 28 | 14 | 17, four of 1000 16 | 12.4 | 14.4; large batches are not affected.
+constexpr int kMinShare = 2;
+// What beginning an item costs, in units: part of its length on the line (256 sequences of 16 to 4096
+// tokens take 145 us with 1, 140 with 3 and 140.5 with 6; eight of up to 512 13.3, 11.9 and 11.9).
+constexpr int kItemCost = 3;
 constexpr float kUnset = 0x1p+126f;  // F before a page with a nonzero value scale: any scale moves it
 constexpr float kLazy = 8.f;   // log2 of how far p may exceed 1 before the reference moves
 
@@ -728,12 +732,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 // CTA per warp of the decode, for the item that ended in that warp's share after beginning in an
 // earlier one; the warp has left what there is to know about it.  Launched while the decode still
 // runs: its first statement waits for the decode's results.
-constexpr int kMergeWarps = 8;
+//
+// W warps (at least as many as an item has heads) with U parts in flight each.  Most items of a
+// large batch have two or three parts, and what counts is how many CTAs an SM holds: 4 warps and 4
+// parts (8 warps for more than 4 heads).  Up to kFewItems items have many (222 for one sequence of
+// 32768 tokens with 8 KV heads): 16 warps and 8 parts.  Decode and merge with 4 heads an item:
+//   4 / 4:   256 sequences of 512 61 us, 16 of 1000 16.2, 4 of 1000 14.2, 1 of 32768 52
+//   16 / 8:  256 sequences of 512 71 us, 16 of 1000 18.3, 4 of 1000 12.6, 1 of 32768 29
+constexpr int kFewItems = 64;
 
-template <typename T, int D>
-__global__ void __launch_bounds__(32 * kMergeWarps) merge_fp8_kernel(DecodeFp8Args a) {
-  __shared__ float4 o_s[kMergeWarps][D / 4];
-  __shared__ float2 ml_s[kMergeWarps];
+template <typename T, int D, int W, int U>
+__global__ void __launch_bounds__(32 * W) merge_fp8_kernel(DecodeFp8Args a) {
+  __shared__ float4 o_s[W][D / 4];
+  __shared__ float2 ml_s[W];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const MergeItem it = a.merge[blockIdx.x];
   if (it.n == 0) return;
@@ -743,7 +754,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_fp8_kernel(DecodeFp8Ar
   // warps: heads first, then groups that take every groups-th part; with D = 64 a warp's halves
   // are groups of their own
   constexpr int kVec = D / 4, kPer = 32 / kVec;
-  const int hh = warp % nh, grp = warp / nh, groups = kMergeWarps / nh;
+  const int hh = warp % nh, grp = warp / nh, groups = W / nh;
   const int e = lane % kVec;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float M = -INFINITY, L = 0.f;
@@ -759,7 +770,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_fp8_kernel(DecodeFp8Ar
     M = N;
   };
   if (grp < groups) {
-    constexpr int U = 4;
+    // U parts at a time, all their loads in flight together
     const int step = groups * kPer;
     for (int i0 = grp * kPer + lane / kVec; i0 < it.n; i0 += U * step) {
       float2 ml[U];
@@ -772,8 +783,26 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_fp8_kernel(DecodeFp8Ar
         v[u] = i < it.n ? *reinterpret_cast<const float4*>(a.part_o + (sl * 8 + hh) * D + e * 4)
                         : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+      float N = M;
 #pragma unroll
-      for (int u = 0; u < U; ++u) add(ml[u], v[u]);
+      for (int u = 0; u < U; ++u) N = fmaxf(N, ml[u].x);
+      const float Nu = N == -INFINITY ? 0.f : N;
+      const float wa = fast_exp2(M - Nu);
+      o.x *= wa;
+      o.y *= wa;
+      o.z *= wa;
+      o.w *= wa;
+      L *= wa;
+      M = N;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = fast_exp2(ml[u].x - Nu);
+        o.x += v[u].x * w;
+        o.y += v[u].y * w;
+        o.z += v[u].z * w;
+        o.w += v[u].w * w;
+        L += ml[u].y * w;
+      }
     }
     if (kPer == 2)
       add(make_float2(__shfl_xor_sync(0xffffffffu, M, 16), __shfl_xor_sync(0xffffffffu, L, 16)),
@@ -820,8 +849,16 @@ cudaError_t launch_t(const CUtensorMap& km, const CUtensorMap& vm, const DecodeF
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   cfg.gridDim = dim3(grid * kWarps);
-  cfg.blockDim = dim3(32 * kMergeWarps);
-  return cudaLaunchKernelEx(&cfg, merge_fp8_kernel<T, D>, a);
+  if (static_cast<int64_t>(a.S) * a.hkv * a.nchunks <= kFewItems) {
+    cfg.blockDim = dim3(32 * 16);
+    return cudaLaunchKernelEx(&cfg, merge_fp8_kernel<T, D, 16, 8>, a);
+  }
+  if (a.group > 4) {
+    cfg.blockDim = dim3(32 * 8);
+    return cudaLaunchKernelEx(&cfg, merge_fp8_kernel<T, D, 8, 4>, a);
+  }
+  cfg.blockDim = dim3(32 * 4);
+  return cudaLaunchKernelEx(&cfg, merge_fp8_kernel<T, D, 4, 4>, a);
 }
 
 template <typename T, bool SPLIT>

@@ -95,6 +95,25 @@ def test_decode(ops, dtype, case):
     assert ops.read_status(torch.device("cuda")) == 0
 
 
+# sequences and KV heads on both sides of 64 items, query heads per KV head on both sides of 4 and 8,
+# and contexts that many warps share
+JOINS = [([5000], 8, 2), ([1, 2600], 16, 16), ([3000, 31], 24, 2), ([900] * 3, 14, 2), ([640] * 17, 16, 4),
+         ([700] * 33, 10, 2), ([400] * 9, 64, 8), ([1200] * 5, 27, 3), ([330] * 22, 9, 3)]
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("case", range(len(JOINS)))
+def test_decode_joins_parts(ops, dtype, D, case):
+    ctx, hq, H = JOINS[case]
+    if len(ctx) * H > 64:
+        ctx = [c - 7 * i for i, c in enumerate(ctx)]
+    q, cache, tables, cu, lens = _batch(ctx, [1] * len(ctx), hq, H, D, 16, dtype, seed=case)
+    ref = R.attend(q, *cache, 1, tables, cu, ctx, 1 / math.sqrt(D))
+    got = ops.paged_decode_fp8(q.cuda(), *[t.cuda() for t in cache], 1, tables.cuda(), lens.cuda(), 1 / math.sqrt(D), max(ctx))
+    _close(got, dtype, ref, ctx, D, DECODE_BITS[dtype])
+
+
 @pytest.mark.parametrize("dtype", ALL)
 def test_decode_scales_and_queries_of_any_size(ops, dtype):
     """Block scales 2^-40 .. 2^20 apart and queries far from 1: every score and output still has its
