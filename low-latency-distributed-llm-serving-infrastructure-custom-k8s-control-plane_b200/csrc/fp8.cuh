@@ -13,7 +13,9 @@
 namespace b200 {
 
 // Rows of a call up to which each row's block is looked up by scanning the call's slots (no
-// scratch, one launch); above it a marking kernel counts the rows of each block first.
+// scratch, one launch); above it a marking kernel counts the rows of each block first.  Rows in
+// blocks of their own, scanned and marked: 256 rows 6.8 and 10.5 us, 1024 16.6 and 19.0, 2048 36.9
+// and 31.8; whole blocks: 1024 rows 18.1 and 17.1, 4096 75 and 26.
 constexpr int kAppendScanRows = 1024;
 
 struct AppendFp8Args {
