@@ -358,6 +358,7 @@ struct ClusterShared {
     unsigned long long list[kList];  // key << 32 | ~index (descending: larger logit, lower index first)
   };
   unsigned long long red[3][kMaxClWarps];
+  unsigned long long warp_kept[kMaxClWarps];  // top-p: each warp's kept sum
   uint64_t loaded[4];  // barriers of the slice's quarters
   double table[64];
   float warp_x[kMaxClWarps];
@@ -573,8 +574,10 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
   weight.set(sh.table, mx, t, a.shift);
   const double one = static_cast<double>(1ull << a.shift);
   const bool top_k = rp.k < V && rp.k > 1, top_p = rp.p < 1.f && rp.k > 1;
+  const double mp = static_cast<double>(rp.mp);
   // each warp's tokens of the slice: [w0, w1), in index order over warps and ranks
-  const int wper = ((n + kClWarps - 1) / kClWarps + 31) & ~31;
+  const auto warp_tokens = [](int n) { return ((n + kClWarps - 1) / kClWarps + 31) & ~31; };
+  const int wper = warp_tokens(n);
   const int w0 = min(n, warp * wper), w1 = min(n, w0 + wper);
 
   uint32_t cut_key = 0, cut_idx = 0xffffffffu;  // kept: larger keys, and this key up to this index
@@ -736,7 +739,6 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       const int m = sh.list_n;
       if (state == 1) {
         // everything else on the list: its first k tokens, of these top-p's, and the draw
-        const double mp = static_cast<double>(rp.mp);
         if (m <= kCounted) {
           constexpr int kPer = (kCounted + kClThreads - 1) / kClThreads;
           order_list(m);
@@ -894,6 +896,7 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
         }
       });
     }
+    unsigned long long mine = mp > 0.0 ? 0 : above;  // of the kept tokens above the border's step
     total = cta_sum<kClThreads>(total, sh.red[1]);
     above = cta_sum<kClThreads>(above, sh.red[2]);  // its barriers order the steps' sums too
     if (tid == 0) {
@@ -905,8 +908,8 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
         if (sh.bins[i]) atomicAdd(&head->bins[i], sh.bins[i]);
     cluster.sync();
     if (rank == 0) {
-      // the border's step: the first one that reaches the target (step lo where rounding left it just
-      // behind); each thread looks at kPer steps in a row
+      // the border's step: the first one that reaches the target; each thread looks at kPer steps in a
+      // row
       constexpr int kPer = kBracket / kClThreads;
       const int steps = few ? hi - lo + 1 : 0;
       unsigned long long h[kPer], own = 0;
@@ -931,7 +934,7 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       for (int w = 0; w < warp; ++w) up += sh.red[0][w];
       for (int j = 0; j < kPer; ++j) {
         const int b = kPer * tid + j;
-        if (b < steps && (static_cast<double>(up) < target || b == 0) && static_cast<double>(up + h[j]) >= target) {
+        if (b < steps && static_cast<double>(up) < target && static_cast<double>(up + h[j]) >= target) {
           sh.bin = lo + b;
           sh.above_bin = up;
           sh.state = held[j] <= kList ? 2 : 3;
@@ -946,7 +949,30 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       cluster.sync();
       return;
     }
-    gather(scale, bin, bin);
+    // The border step's tokens into rank 0's list.  What the draw needs of the others is the sum of
+    // each warp's tokens above that step: the exact pass has it but for the steps from lo on, few of
+    // the tokens (with min-p, which the exact pass leaves out, all are looked at again).
+    {
+      const float from = mp > 0.0 ? -1.f : static_cast<float>(lo), at_bin = static_cast<float>(bin);
+      const float to = bin == kBins - 1 ? INFINITY : static_cast<float>(bin + 1);
+      each([&](float v, int i) {
+        const float at_step = place_of(v, scale);
+        if (at_step < from || (at_step >= to && to < INFINITY)) return;
+        const uint32_t key = key_of(v), idx = begin + i;
+        if (!kept(key, idx)) return;
+        if (at_step < at_bin) {
+          const double w = weight(v);
+          if (w >= mp) mine += weight.fixed(w);
+        } else {
+          const int at = atomicAdd(&head->list_n, 1);
+          if (at < kList) head->list[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - idx);
+        }
+      });
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      if (lane == 0) sh.warp_kept[warp] = mine;
+    }
+    cluster.sync();
     if (rank == 0) {
       const int m = sh.list_n;
       const double target = static_cast<double>(rp.p) * static_cast<double>(sh.all_total);
@@ -977,6 +1003,16 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
           }
         }
       }
+      __syncthreads();
+      // what is kept of the list, to the sums of the warps that hold it
+      for (int i = tid; i < m; i += kClThreads) {
+        const uint32_t key = static_cast<uint32_t>(sh.list[i] >> 32), idx = 0xffffffffu - static_cast<uint32_t>(sh.list[i]);
+        if (key < sh.cut_key || (key == sh.cut_key && idx > sh.cut_idx)) continue;
+        const double w = weight(float_of(key));
+        if (w < mp) continue;
+        const int r = static_cast<int>(idx) / per, at = static_cast<int>(idx) - r * per;
+        atomicAdd(&cluster.map_shared_rank(&sh, r)->warp_kept[at / warp_tokens(min(V - r * per, per))], weight.fixed(w));
+      }
     }
     cluster.sync();
     cut_key = head->cut_key;
@@ -984,23 +1020,26 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
   }
 
   // ---- 5. draw -----------------------------------------------------------------------------------
-  const double mp = static_cast<double>(rp.mp);
   const bool filtered = top_k || top_p;
   unsigned long long mine = 0, all = 0;
-  if (!filtered && mp <= 0.0) {
+  if (top_p) {
+    mine = sh.warp_kept[warp];
+  } else if (!filtered && mp <= 0.0) {
     each([&](float v, int) { mine += weight.fixed(weight(v)); });
     all = mine;
   } else {
     each([&](float v, int i) {
-      if (filtered && !kept(key_of(v), begin + i)) return;
+      if (top_k && !kept(key_of(v), begin + i)) return;
       const double w = weight(v);
       const unsigned long long f = weight.fixed(w);
       all += f;
       if (w >= mp) mine += f;
     });
   }
+  if (!top_p) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  }
   __syncthreads();
   if (lane == 0) sh.red[0][warp] = mine;
   all = cta_sum<kClThreads>(all, sh.red[1]);
