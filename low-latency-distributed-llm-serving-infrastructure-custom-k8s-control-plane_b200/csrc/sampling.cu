@@ -344,9 +344,12 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
 constexpr int kMaxClWarps = 16;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;
-constexpr int kCounted = 384;  // entries up to which a list's order is counted out instead of sorted
+// Entries up to which a list's order is counted out instead of sorted (lists of 240: 10,600 cycles
+// counted, 7,700 sorted; of 60 with top-k 50: the two are alike, and the sort comes twice).
+constexpr int kCounted = 128;
 constexpr int kBracket = 512;       // steps that can hold a top-p border
 constexpr float kBinScale = 64.f;
+constexpr int kFine = 128;          // parts that few steps are divided into (32 and 512: the same time)
 
 struct ClusterShared {
   union {  // the counts are read before the sums are written
@@ -370,6 +373,7 @@ struct ClusterShared {
   // what rank 0 decides
   int32_t bin, lo, hi, list_n, state, token;
   unsigned long long above_bin;
+  double last;  // the open step's share
   uint32_t cut_key;
   uint32_t cut_idx;
 };
@@ -389,16 +393,33 @@ __device__ __forceinline__ unsigned long long cta_sum(unsigned long long v, unsi
   return v;
 }
 
-// Descending bitonic sort of n <= kList entries, padded with zeros to a power of two.
+// Descending bitonic sort of n <= kList entries, padded with zeros to a power of two.  Exchanges over
+// less than 32 places are done in registers, a warp per 32 entries; only longer ones go through shared
+// memory with a barrier each (512 entries: 15 barriers instead of 45).
 template <int kClThreads>
 __device__ void sort_list(unsigned long long* v, int n) {
-  int size = 2;
+  const int tid = threadIdx.x;
+  int size = 32;
   while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += kClThreads) v[i] = 0;
+  for (int i = n + tid; i < size; i += kClThreads) v[i] = 0;
   __syncthreads();
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int p = threadIdx.x; p < size / 2; p += kClThreads) {
+  const auto within_warps = [&](int k_first, int k_last) {
+    for (int i = tid; i < size; i += kClThreads) {  // size is a multiple of 32: whole warps
+      unsigned long long own = v[i];
+      for (int k = k_first; k <= k_last; k <<= 1)
+        for (int j = k < 32 ? k >> 1 : 16; j > 0; j >>= 1) {
+          const unsigned long long other = __shfl_xor_sync(0xffffffffu, own, j);
+          const bool larger = ((i & j) == 0) == ((i & k) == 0);
+          own = (other > own) == larger ? other : own;
+        }
+      v[i] = own;
+    }
+    __syncthreads();
+  };
+  within_warps(2, 32);
+  for (int k = 64; k <= size; k <<= 1) {
+    for (int j = k >> 1; j >= 32; j >>= 1) {
+      for (int p = tid; p < size / 2; p += kClThreads) {
         const int lo = 2 * p - (p & (j - 1)), hi = lo + j;
         const bool down = (lo & k) == 0;
         const unsigned long long a = v[lo], b = v[hi];
@@ -409,6 +430,8 @@ __device__ void sort_list(unsigned long long* v, int n) {
       }
       __syncthreads();
     }
+    within_warps(k, k);
+  }
 }
 
 // Exclusive prefix sums of n <= kList entries in place; returns their sum.  Whole CTA.
@@ -595,6 +618,25 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
     }
     for (; i < w1; i += 32) f(logit<T>(s[i]), i);
   };
+  // f(logit, w in fixed point, token) likewise; the four weights are worked out side by side
+  const auto each_weight = [&](auto f) {
+    constexpr int U = 4;
+    int i = w0 + lane;
+    for (; i + 32 * (U - 1) < w1; i += 32 * U) {
+      float v[U];
+      unsigned long long w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = logit<T>(s[i + 32 * u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = weight.fixed(weight(v[u]));
+#pragma unroll
+      for (int u = 0; u < U; ++u) f(v[u], w[u], i + 32 * u);
+    }
+    for (; i < w1; i += 32) {
+      const float v = logit<T>(s[i]);
+      f(v, weight.fixed(weight(v)), i);
+    }
+  };
   // Sum of w where only the log probability asks for it: exact for the terms above 2^-10, in fp32
   // (4e-7 off at most, either way) for the many small ones behind them.
   const float c32 = static_cast<float>(1.4426950408889634 / t);
@@ -671,28 +713,55 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
     return;
   }
 
-  // Of up to kCounted entries of the list, by comparing all with all: how many are ahead of this
-  // thread's, and their weights' sum; every entry's weight into sums.  Whole CTA.
-  int place[(kCounted + kClThreads - 1) / kClThreads];
-  unsigned long long ahead[(kCounted + kClThreads - 1) / kClThreads];
+  // Sums over the entries of the list that `before` puts ahead of an entry, for each of its m <=
+  // kCounted entries: a warp takes four entries at a time, its lanes side by side through the list.
+  // What is counted and summed goes to take(entry, count, sum), in lane 0.  Whole CTA.
+  const auto compare_all = [&](int m, auto before, auto take) {
+    constexpr int E = 4;
+    for (int e0 = warp * E; e0 < m; e0 += kClWarps * E) {
+      unsigned long long own[E], sum[E];
+      uint32_t count[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        own[e] = sh.list[min(e0 + e, m - 1)];
+        sum[e] = 0;
+        count[e] = 0;
+      }
+#pragma unroll 2
+      for (int o = lane; o < m; o += 32) {
+        const unsigned long long other = sh.list[o], w = sh.sums[o];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const bool ahead = before(other, own[e]);
+          count[e] += ahead ? 1 : 0;
+          sum[e] += ahead ? w : 0;
+        }
+      }
+      // a lane's sum is below 2^50 (up to 12 weights of at most 2^46): in two parts of 26 bits
+      static_assert(kCounted <= 32 * 63, "a lane's sum stays below 2^52");
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        count[e] = __reduce_add_sync(0xffffffffu, count[e]);
+        const uint32_t low = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(sum[e]) & 0x3ffffffu);
+        const uint32_t high = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(sum[e] >> 26));
+        if (lane == 0 && e0 + e < m) take(e0 + e, static_cast<int>(count[e]), (static_cast<unsigned long long>(high) << 26) + low);
+      }
+    }
+    __syncthreads();
+  };
+  // Order of the list's entries: each one's weight into sums, how many are ahead of it into place, and
+  // their weights' sum into ahead (behind the entries that the two arrays hold).
+  unsigned long long* const ahead = sh.sums + kCounted;
+  unsigned long long* const place = sh.list + kCounted;
   const auto order_list = [&](int m) {
     for (int i = tid; i < m; i += kClThreads)
       sh.sums[i] = weight.fixed(weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32))));
     __syncthreads();
-    for (int j = 0; j < static_cast<int>(sizeof(place) / sizeof(place[0])); ++j) {
-      const int i = tid + j * kClThreads;
-      place[j] = 0;
-      ahead[j] = 0;
-      if (i >= m) continue;
-      const unsigned long long own = sh.list[i];
-#pragma unroll 4
-      for (int o = 0; o < m; ++o)
-        if (sh.list[o] > own) {
-          ++place[j];
-          ahead[j] += sh.sums[o];
-        }
-    }
-    __syncthreads();
+    compare_all(m, [](unsigned long long other, unsigned long long own) { return other > own; },
+                [&](int e, int count, unsigned long long sum) {
+                  place[e] = count;
+                  ahead[e] = sum;
+                });
   };
 
   if (top_k) {
@@ -740,38 +809,31 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       if (state == 1) {
         // everything else on the list: its first k tokens, of these top-p's, and the draw
         if (m <= kCounted) {
-          constexpr int kPer = (kCounted + kClThreads - 1) / kClThreads;
           order_list(m);
-          unsigned long long w[kPer], total = 0, sum = 0;
-          for (int j = 0; j < kPer; ++j) {
-            const int i = tid + j * kClThreads;
-            w[j] = i < m ? sh.sums[i] : 0;
-            if (i < m && place[j] < rp.k) total += w[j];
-          }
+          unsigned long long total = 0, sum = 0;
+          for (int i = tid; i < m; i += kClThreads)
+            if (static_cast<int>(place[i]) < rp.k) total += sh.sums[i];
           total = cta_sum<kClThreads>(total, sh.red[0]);
           const double target = static_cast<double>(rp.p) * static_cast<double>(total);
-          for (int j = 0; j < kPer; ++j) {
-            const int i = tid + j * kClThreads;
-            if (i >= m) continue;
-            const bool in = place[j] < rp.k &&
-                            (!top_p || place[j] == 0 || static_cast<double>(ahead[j]) < target) &&
+          for (int i = tid; i < m; i += kClThreads) {
+            const bool in = static_cast<int>(place[i]) < rp.k &&
+                            (!top_p || place[i] == 0 || static_cast<double>(ahead[i]) < target) &&
                             weight(float_of(static_cast<uint32_t>(sh.list[i] >> 32))) >= mp;
-            if (!in) w[j] = 0;
-            sh.sums[i] = w[j];
-            sum += w[j];
+            if (!in) sh.sums[i] = 0;
+            sum += sh.sums[i];
           }
           sum = cta_sum<kClThreads>(sum, sh.red[0]);
           const unsigned long long goal =
               static_cast<unsigned long long>(static_cast<double>(rp.u) * static_cast<double>(sum));
-          for (int j = 0; j < kPer; ++j) {
-            const int i = tid + j * kClThreads;
-            if (i >= m || w[j] == 0) continue;
-            const uint32_t own = static_cast<uint32_t>(sh.list[i]);  // ~index: larger for lower ones
-            unsigned long long before = 0;
-            for (int o = 0; o < m; ++o)
-              if (static_cast<uint32_t>(sh.list[o]) > own) before += sh.sums[o];
-            if (before <= goal && goal < before + w[j]) sh.token = static_cast<int32_t>(0xffffffffu - own);
-          }
+          // the low words are ~index: larger for lower ones
+          compare_all(m,
+                      [](unsigned long long other, unsigned long long own) {
+                        return static_cast<uint32_t>(other) > static_cast<uint32_t>(own);
+                      },
+                      [&](int e, int, unsigned long long before) {
+                        if (before <= goal && goal < before + sh.sums[e])
+                          sh.token = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(sh.list[e]));
+                      });
         } else {
           sort_list<kClThreads>(sh.list, m);
           const int keep_k = min(m, rp.k);
@@ -835,12 +897,15 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
     if (rank == 0) {
       // the border's steps: where p times the sum can lie, with a step's sum known to e^(1/64)
       const int per_t = kBins / kClThreads;
-      double mine[per_t], sum = 0.0;
+      constexpr double kStep = 0.9844964370054085;  // e^(-1/64)
+      double mine[per_t], sum = 0.0, most_w = exp(-static_cast<double>(tid * per_t) / 64.0), last_w = 0.0;
       for (int j = 0; j < per_t; ++j) {
-        const int b = tid * per_t + j;
-        mine[j] = sh.hist[b] * exp(-static_cast<double>(b) / 64.0);  // at most this
+        mine[j] = sh.hist[tid * per_t + j] * most_w;  // at most this
         sum += mine[j];
+        last_w = mine[j];
+        most_w *= kStep;
       }
+      if (tid == kClThreads - 1) sh.last = last_w;
       double x = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -864,16 +929,23 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       // where the sum from the top reaches p times the whole, and where the sum behind it is at most
       // 1 - p times the whole: for p near 1 the latter says far more.
       constexpr double kLow = 0.98447, kUp = 1.00001;
-      const double last = sh.hist[kBins - 1] * exp(-static_cast<double>(kBins - 1) / 64.0);
+      const double last = sh.last;
       const double p = static_cast<double>(rp.p), most = all * kUp, least = (all - last) * kLow;
+      int first_may = kBins - 1, first_must = kBins - 1;
       for (int j = 0; j < per_t; ++j) {
         const int b = tid * per_t + j;
         const double after = before + mine[j], tail = fmax(all - after, 0.0);
         const bool may = after * kUp >= p * least && (tail - last) * kLow <= (1.0 - p) * most;
         const bool must = (b == kBins - 1 ? 0.0 : after * kLow) >= p * most || tail * kUp + 1e-12 * all <= (1.0 - p) * least;
-        if (may) atomicMin(&sh.lo, b);
-        if (must) atomicMin(&sh.hi, b);
+        if (may) first_may = min(first_may, b);
+        if (must) first_must = min(first_must, b);
         before = after;
+      }
+      first_may = __reduce_min_sync(0xffffffffu, first_may);
+      first_must = __reduce_min_sync(0xffffffffu, first_must);
+      if (lane == 0) {
+        atomicMin(&sh.lo, first_may);
+        atomicMin(&sh.hi, first_must);
       }
     }
     cluster.sync();
@@ -881,19 +953,20 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
     // exact sums: all kept tokens, those above the border's steps, each of these steps
     unsigned long long total = 0, above = 0;
     const bool few = hi - lo < kBracket;
+    // the steps in parts, so that few tokens share one with the border
+    int split = 1;
+    while ((hi - lo + 1) * split * 2 <= kFine) split *= 2;
+    const float parts = static_cast<float>(split);
     if (few) {
-      const float from = static_cast<float>(lo);
-      each([&](float v, int i) {
-        if (top_k && !kept(key_of(v), begin + i)) return;
-        const unsigned long long w = weight.fixed(weight(v));
+      const float from = static_cast<float>(lo), last_part = static_cast<float>(kBins * split - 1);
+      const float behind = hi == kBins - 1 ? INFINITY : static_cast<float>(hi + 1);
+      each_weight([&](float v, unsigned long long w, int i) {
+        if (top_k && !kept(key_of(v), begin + i)) w = 0;
         total += w;
         const float at_step = place_of(v, scale);
-        if (at_step < from) {
-          above += w;
-        } else {
-          const int b = static_cast<int>(fminf(at_step, static_cast<float>(kBins - 1)));
-          if (b <= hi) atomicAdd(&sh.bins[b - lo], w);
-        }
+        above += at_step < from ? w : 0;
+        if (!(at_step < from) && !(at_step >= behind && behind < INFINITY))
+          atomicAdd(&sh.bins[static_cast<int>(fminf(at_step * parts, last_part)) - lo * split], w);
       });
     }
     unsigned long long mine = mp > 0.0 ? 0 : above;  // of the kept tokens above the border's step
@@ -904,20 +977,18 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       atomicAdd(&head->all_above, above);
     }
     if (rank != 0 && few)
-      for (int i = tid; i <= hi - lo; i += kClThreads)
+      for (int i = tid; i < (hi - lo + 1) * split; i += kClThreads)
         if (sh.bins[i]) atomicAdd(&head->bins[i], sh.bins[i]);
     cluster.sync();
     if (rank == 0) {
-      // the border's step: the first one that reaches the target; each thread looks at kPer steps in a
+      // the border's part: the first one that reaches the target; each thread looks at kPer parts in a
       // row
       constexpr int kPer = kBracket / kClThreads;
-      const int steps = few ? hi - lo + 1 : 0;
+      const int steps = few ? (hi - lo + 1) * split : 0;
       unsigned long long h[kPer], own = 0;
-      uint32_t held[kPer];
       for (int j = 0; j < kPer; ++j) {
         const int b = kPer * tid + j;
         h[j] = b < steps ? sh.bins[b] : 0;
-        held[j] = b < steps ? sh.hist[lo + b] : 0;
         own += h[j];
       }
       unsigned long long x = own;
@@ -935,9 +1006,9 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       for (int j = 0; j < kPer; ++j) {
         const int b = kPer * tid + j;
         if (b < steps && static_cast<double>(up) < target && static_cast<double>(up + h[j]) >= target) {
-          sh.bin = lo + b;
+          sh.bin = lo * split + b;
           sh.above_bin = up;
-          sh.state = held[j] <= kList ? 2 : 3;
+          sh.state = 2;
         }
         up += h[j];
       }
@@ -949,12 +1020,12 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       cluster.sync();
       return;
     }
-    // The border step's tokens into rank 0's list.  What the draw needs of the others is the sum of
-    // each warp's tokens above that step: the exact pass has it but for the steps from lo on, few of
+    // The border part's tokens into rank 0's list.  What the draw needs of the others is the sum of
+    // each warp's tokens above it: the exact pass has it but for the steps from lo on, few of
     // the tokens (with min-p, which the exact pass leaves out, all are looked at again).
     {
-      const float from = mp > 0.0 ? -1.f : static_cast<float>(lo), at_bin = static_cast<float>(bin);
-      const float to = bin == kBins - 1 ? INFINITY : static_cast<float>(bin + 1);
+      const float from = mp > 0.0 ? -1.f : static_cast<float>(lo), at_bin = static_cast<float>(bin) / parts;
+      const float to = bin == kBins * split - 1 ? INFINITY : static_cast<float>(bin + 1) / parts;
       each([&](float v, int i) {
         const float at_step = place_of(v, scale);
         if (at_step < from || (at_step >= to && to < INFINITY)) return;
@@ -973,17 +1044,20 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       if (lane == 0) sh.warp_kept[warp] = mine;
     }
     cluster.sync();
+    if (head->list_n > kList) {  // left to sample_row_kernel
+      if (rank == 0 && tid == 0) a.tokens[row] = kTodo;
+      cluster.sync();
+      return;
+    }
     if (rank == 0) {
       const int m = sh.list_n;
       const double target = static_cast<double>(rp.p) * static_cast<double>(sh.all_total);
       if (m <= kCounted) {
         order_list(m);
-        for (int j = 0; j < static_cast<int>(sizeof(place) / sizeof(place[0])); ++j) {
-          const int i = tid + j * kClThreads;
-          if (i >= m) continue;
+        for (int i = tid; i < m; i += kClThreads) {
           // the last token that is kept: the sum ahead of it is short of the target, with it it is not
-          const unsigned long long up = sh.above_bin + ahead[j];
-          if (static_cast<double>(up) < target && (static_cast<double>(up + sh.sums[i]) >= target || place[j] == m - 1)) {
+          const unsigned long long up = sh.above_bin + ahead[i];
+          if (static_cast<double>(up) < target && (static_cast<double>(up + sh.sums[i]) >= target || static_cast<int>(place[i]) == m - 1)) {
             sh.cut_key = static_cast<uint32_t>(sh.list[i] >> 32);
             sh.cut_idx = 0xffffffffu - static_cast<uint32_t>(sh.list[i]);
           }
@@ -1025,7 +1099,7 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
   if (top_p) {
     mine = sh.warp_kept[warp];
   } else if (!filtered && mp <= 0.0) {
-    each([&](float v, int) { mine += weight.fixed(weight(v)); });
+    each_weight([&](float, unsigned long long w, int) { mine += w; });
     all = mine;
   } else {
     each([&](float v, int i) {
