@@ -11,7 +11,8 @@ namespace {
 
 constexpr int kRowWarps = 8;
 
-// One CTA per (query row, KV head, up to 8 query heads): each warp takes every kRowWarps-th
+// For what the tensor-core kernels do not take (fp32 prefill, head dims other than 64 and 128, odd block
+// sizes).  One CTA per (query row, KV head, up to 8 query heads): each warp takes every kRowWarps-th
 // position, the running (max, sum, output) of the warps are merged at the end.
 template <typename T, int NPL>
 __global__ void __launch_bounds__(kRowWarps * 32) row_fp8_kernel(AttnFp8Args a, int nchunks) {
@@ -174,7 +175,7 @@ __device__ __forceinline__ void widen16(uint4 c, float s, uint4 (&out)[2]) {
 // Each CTA copies an equal share of the scratch blocks, 16 codes per thread and step.  Every CTA
 // sums up the sequences' blocks by itself, 256 sequences at a time (1 us for a few hundred; a
 // kernel of its own for the sums took 4 us and a launch).  Bound by memory: 1 byte read and 2
-// written per entry.
+// written per entry; 67 MB of codes take 44 us, of which 30 at the copy rate.
 template <typename T>
 __global__ void __launch_bounds__(256) expand_kernel(ExpandFp8Args a) {
   __shared__ int32_t warp_n[8];

@@ -14,6 +14,13 @@
 // kAppendScanRows rows every row's CTA scans the call's slots for its block (the CTA of the first
 // such row goes on, the others leave); larger calls first count the rows of each block and list
 // the rows where a run of rows of one block starts.
+//
+// Bound: HBM.  A step of 16 prompt chunks and 240 single rows (14,200 rows, GQA 32/8, D 128, bf16, with
+// rotation): 76 us for rows, codes and rotated queries (49 us at the copy rate; 44 % of the DRAM rate),
+// 22 us for the read-back; one element per thread and memory pass took 427 us for both, against 108.  256
+// decode rows take 6.3 us, of which a launch and the chain slot -> block -> scale -> codes are the most.
+// Rows that have a block to themselves are what keeps a large call from the DRAM rate: 8192 of them take
+// 115 us, 8192 rows of whole blocks 48.
 #include "fp8.cuh"
 
 namespace b200 {

@@ -329,6 +329,12 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
 
 // ---- a cluster of CTAs per row ----------------------------------------------------------------------
 //
+// Bound by instructions: an exact weight takes some 20, 12 of them on the 64-bit pipe.  256 rows of
+// 128256: temperature alone 74 us in bf16 (64 % of the issue slots, 10 % of the DRAM rate) and 122 in
+// fp32, top-k 50 113 and 156, top-p 0.95 188 and 262; one CTA per row that reads it once per pass took
+// 933 us for temperature alone and 2963 for all filters (186 before the draw lost its pass after
+// top-p, 168 now).  One row of 128256: 13, 18 and 28 us.
+//
 // The CTAs of a cluster hold a row in their shared memory, each a slice, so it is read from memory
 // once; what follows are passes over shared memory, joined through the cluster's.
 //   1. the maximum, while the slice is loaded
@@ -492,8 +498,8 @@ __device__ __forceinline__ float largest_of<__half>(uint4 u) {
 }
 
 // kClThreads: 256 for 16-bit logits (four CTAs an SM) and 512 for fp32 (two, as their slices are
-// twice the size): 256 x 128256 with every row's own parameters takes 170 us with 256 threads and
-// 205 with 512 in bf16, 255 (32 KB slices, 16 CTAs a row) and 234 in fp32.
+// twice the size): when it was chosen, 256 x 128256 with every row's own parameters took 170 us with
+// 256 threads and 205 with 512 in bf16, 255 (32 KB slices, 16 CTAs a row) and 234 in fp32.
 template <typename T, int kClThreads>
 __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_kernel(SampleArgs a) {
   constexpr int kClWarps = kClThreads / 32;
