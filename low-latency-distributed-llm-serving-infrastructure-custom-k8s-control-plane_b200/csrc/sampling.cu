@@ -955,13 +955,13 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
       }
     }
     cluster.sync();
-    const int lo = head->lo, hi = head->hi;
+    const int lo = head->lo, hi = max(lo, head->hi);
     // exact sums: all kept tokens, those above the border's steps, each of these steps
     unsigned long long total = 0, above = 0;
     const bool few = hi - lo < kBracket;
     // the steps in parts, so that few tokens share one with the border
     int split = 1;
-    while ((hi - lo + 1) * split * 2 <= kFine) split *= 2;
+    while (split < kFine && (hi - lo + 1) * split * 2 <= kFine) split *= 2;
     const float parts = static_cast<float>(split);
     if (few) {
       const float from = static_cast<float>(lo), last_part = static_cast<float>(kBins * split - 1);

@@ -74,6 +74,23 @@ def test_long_lists_and_flat_rows(sampling, dtype):
     _check(sampling, x, u, t=[0.3] * 20, k=[2000] * 20, p=[0.95] * 20, m=[1e-4] * 20)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [900, 40001])
+def test_top_p_borders_with_few_and_many_equal_tokens(sampling, dtype, vocab):
+    """From one to thousands of tokens of one logit at the border, spread over a cluster; with min-p
+    above and below the border; temperatures down to subnormal ones."""
+    rng = np.random.default_rng(11)
+    grid = [1, 3, 8, 20, 50, 120, 300, 1000, 1e6]
+    x = torch.from_numpy(np.stack([np.round(rng.normal(0, 2, vocab) * q) / q for q in grid]).astype(np.float32)).to(dtype)
+    n = len(grid)
+    for p in (0.05, 0.3, 0.8, 0.95, 0.999):
+        u = rng.random(n, dtype=np.float32).tolist()
+        _check(sampling, x, u, p=[p] * n)
+        _check(sampling, x, u, p=[p] * n, m=[0.3, 0.1, 0.01, 1e-3, 1e-5, 1.0, 0.03, 0.2, 0.5])
+        _check(sampling, x, u, t=[0.2, 1e-3, 1e-20, 1e-37, 1e-40, 0.7, 5.0, 100.0, 1e30], p=[p] * n)
+        _check(sampling, x, u, k=[100, 500, 2000, 0, 800, 128, 129, 1024, 1025], p=[p] * n, m=[1e-4] * n)
+
+
 def test_vocabularies_beyond_the_clusters_memory(sampling):
     rng = np.random.default_rng(3)
     x = torch.from_numpy(rng.normal(0, 3, (3, 500001)).astype(np.float32))
