@@ -155,8 +155,8 @@ int code_map(const void* cache, const B200Fp8Cache& c, int box_rows, CUtensorMap
 }
 
 // cu_q: mixed batch, only sequences with exactly one new token are decoded (row cu_q[s]).
-int run_decode(const B200AttentionFp8Params& p, const DecodePlan& pl, const int64_t* cu_q, char* ws,
-               cudaStream_t st) {
+int run_decode(const B200AttentionFp8Params& p, const DecodePlan& pl, const int64_t* cu_q,
+               bool decodes_only, char* ws, cudaStream_t st) {
   const B200Fp8Cache& c = p.cache;
   CUtensorMap km, vm;
   const int box_rows = c.block_size >= 16 ? 16 : 8;
@@ -180,6 +180,7 @@ int run_decode(const B200AttentionFp8Params& p, const DecodePlan& pl, const int6
   a.scale_log2 = p.scale * b200::kLog2e;
   a.o_srow = p.o_stride_row;
   a.o_shead = p.o_stride_head;
+  a.decodes_only = decodes_only ? 1 : 0;
   a.status = p.status_word;
   a.merge = reinterpret_cast<b200::MergeItem*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + pl.off_ml);
@@ -285,8 +286,10 @@ PrefillPlan prefill_plan(const B200AttentionFp8Params& p) {
 // decode 130 us, copy 44, plan 9, prefill 458 (0.95 PFLOP/s); a CTA per query row took 121 ms, and one
 // prompt of 8192 150 ms against 0.53.
 int run_prefill(const B200AttentionFp8Params& p, const PrefillPlan& pl, char* ws, cudaStream_t st) {
-  int rc = run_decode(p, pl.decode, p.cu_seqlens, ws, st);
-  if (rc != B200_OK || p.num_tokens < 2 || p.max_query_len < 2 || p.prefill_blocks == 0) return rc;
+  // by the caller's bounds there is nothing but decodes
+  const bool decodes_only = p.num_tokens < 2 || p.max_query_len < 2 || p.prefill_blocks == 0;
+  const int rc = run_decode(p, pl.decode, p.cu_seqlens, decodes_only, ws, st);
+  if (rc != B200_OK || decodes_only) return rc;
   const B200Fp8Cache& c = p.cache;
   b200::ExpandFp8Args a{};
   a.kc = static_cast<const uint8_t*>(c.key_cache);
@@ -447,7 +450,7 @@ int b200_paged_decode_fp8(const B200AttentionFp8Params* p, void* workspace,
   if (pl.tensor_cores) {
     rc = check_workspace(workspace, workspace_bytes, pl.total);
     if (rc != B200_OK) return rc;
-    return run_decode(*p, pl, nullptr, static_cast<char*>(workspace), st);
+    return run_decode(*p, pl, nullptr, false, static_cast<char*>(workspace), st);
   }
   b200::AttnFp8Args a = attention_args(*p);
   a.query_rows = p->query_rows;

@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   // decoded sequences without context: zeros
   for (int s = blockIdx.x; s < a.S; s += gridDim.x) {
     if (tid == 0 && a.ctx_lens[s] > a.max_ctx) flag_status(a.status, B200_DEVICE_BAD_OP);
+    if (tid == 0 && a.decodes_only && a.cu_q[s + 1] - a.cu_q[s] > 1) flag_status(a.status, B200_DEVICE_BAD_STEP);
     if (cu[s + 1] != cu[s] || (a.cu_q != nullptr && a.cu_q[s + 1] - a.cu_q[s] != 1)) continue;
     const int64_t row = a.cu_q ? a.cu_q[s] : (a.query_rows ? a.query_rows[s] : s);
     const int hq = a.hkv * a.group;

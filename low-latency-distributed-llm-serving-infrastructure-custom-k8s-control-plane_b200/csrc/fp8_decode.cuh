@@ -19,6 +19,7 @@ struct DecodeFp8Args {
   int32_t vec_q;  // query rows and heads are aligned to four elements
   const int32_t* query_rows;
   const int64_t* cu_q;  // mixed batch: only sequences with exactly one new token, row cu_q[s]
+  int32_t decodes_only;  // the caller says that there are no others: flagged where there are
   const float* ks;
   const float* vs;
   int32_t layer, nb, bs, hkv, head_dim, group, nchunks;

@@ -341,6 +341,8 @@ def test_prefill_bound_too_small_is_flagged(ops):
     got = ops.paged_prefill_fp8(*args, prefill_blocks=5)  # ten blocks are needed
     assert ops.read_status(torch.device("cuda")) & N.DEVICE_BAD_STEP
     _close(got[:40], torch.bfloat16, tuple(t[:40] for t in ref), ctx, 64, PREFILL_BITS[torch.bfloat16])
+    ops.paged_prefill_fp8(*args, prefill_blocks=0)  # none, it says
+    assert ops.read_status(torch.device("cuda")) & N.DEVICE_BAD_STEP
     got = ops.paged_prefill_fp8(*args, prefill_blocks=10)
     assert ops.read_status(torch.device("cuda")) == 0
     _close(got, torch.bfloat16, ref, ctx, 64, PREFILL_BITS[torch.bfloat16])
