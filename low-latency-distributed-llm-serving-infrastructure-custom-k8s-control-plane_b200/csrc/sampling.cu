@@ -350,8 +350,8 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
 constexpr int kMaxClWarps = 16;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;
-// Entries up to which a list's order is counted out instead of sorted (lists of 240: 10,600 cycles
-// counted, 7,700 sorted; of 60 with top-k 50: the two are alike, and the sort comes twice).
+// Entries up to which a list's order is counted out instead of sorted: lists of 240 take 10,600 cycles
+// counted and 7,700 sorted; with top-k 50 (lists of about 60) bounds of 64 and 128 are alike.
 constexpr int kCounted = 128;
 constexpr int kBracket = 512;       // steps that can hold a top-p border
 constexpr float kBinScale = 64.f;
