@@ -17,8 +17,9 @@
 // weights are split in two f16 parts (22 bits), each with its own product.
 // The weights of P: p = 2^(x - m) with a lazily moved reference m (p <= 2^8), stored for the
 // product as p * vs * F: vs is the page's value scale and F a power of two per head that keeps the
-// products inside f16's normal range whatever the scales are (11 bits of every weight that is
-// within 2^-22 of the head's largest).
+// head's largest product between 1 and 2^15 whatever the scales are, also where the scores move on to
+// pages of far smaller values (11 bits of every product within 2^-14 of the largest, an error of at
+// most 2^-25 of the largest for smaller ones).
 //
 // Bound: HBM (4 * G flop per byte).  A unit is 64 * D bytes.  Measured with GQA 32/8, D 128, bf16
 // queries: 256 sequences of 16 to 4096 tokens (677 MB) 128-139 us, 4.9-5.3 TB/s; 14 of 8192 to 32768
@@ -611,12 +612,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           w0 = fmaxf(w0, __shfl_xor_sync(0xffffffffu, w0, o));
           w1 = fmaxf(w1, __shfl_xor_sync(0xffffffffu, w1, o));
         }
-        // F changes when unset or when a product would pass 2^15
+        // F changes when unset, when a product would pass 2^15, and when the unit's largest one falls below
+        // 1: the reference has then moved to pages of smaller values, whose products f16 would hold in
+        // fewer bits.  Sums held so far are below 2^55 (products of 2^15, codes of 448, 2^31
+        // tokens); what raises F leaves them below 2^115.
         const auto refit = [](float w, float& F, float& al) {
-          if (!(w > 0.f) || (F != kUnset && w * F <= 32768.f)) return;
+          if (!(w > 0.f) || (F != kUnset && w * F >= 1.f && w * F <= 32768.f)) return;
           const float f = pow2_inverse(w, 8);  // p * vs * F in [2^8, 2^9)
-          al *= f / F;
-          F = f;
+          const int up = static_cast<int>(__float_as_uint(f) >> 23) - static_cast<int>(__float_as_uint(F) >> 23);
+          const int most = 60 + 127 - static_cast<int>(__float_as_uint(al) >> 23);
+          const int by = al > 0.f ? min(up, most) : up;
+          F = __uint_as_float(__float_as_uint(F) + (static_cast<uint32_t>(by) << 23));
+          al = ldexpf(al, by);
         };
         refit(w0, F0, al0);
         refit(w1, F1, al1);
