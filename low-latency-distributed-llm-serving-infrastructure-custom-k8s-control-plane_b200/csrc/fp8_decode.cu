@@ -50,7 +50,9 @@ constexpr int kMinShare = 2;
 // What beginning an item costs, in units: part of its length on the line (256 sequences of 16 to 4096
 // tokens take 145 us with 1, 140 with 3 and 140.5 with 6; eight of up to 512 13.3, 11.9 and 11.9).
 constexpr int kItemCost = 3;
-constexpr float kUnset = 0x1p+126f;  // F before a page with a nonzero value scale: any scale moves it
+// F before a page with a nonzero value scale: any of 2^-111 or more moves it.  Set ones are smaller, so p * F
+// stays finite for p <= 2^8, and times a scale it is 0 where the weight or the scale is.
+constexpr float kUnset = 0x1p+118f;
 constexpr float kLazy = 8.f;   // log2 of how far p may exceed 1 before the reference moves
 
 template <int D>
@@ -618,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         // tokens); what raises F leaves them below 2^115.
         const auto refit = [](float w, float& F, float& al) {
           if (!(w > 0.f) || (F != kUnset && w * F >= 1.f && w * F <= 32768.f)) return;
-          const float f = pow2_inverse(w, 8);  // p * vs * F in [2^8, 2^9)
+          const float f = fminf(pow2_inverse(w, 8), 0.5f * kUnset);  // p * vs * F in [2^8, 2^9)
           const int up = static_cast<int>(__float_as_uint(f) >> 23) - static_cast<int>(__float_as_uint(F) >> 23);
           const int most = 60 + 127 - static_cast<int>(__float_as_uint(al) >> 23);
           const int by = al > 0.f ? min(up, most) : up;
@@ -642,10 +644,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         float p0 = fast_exp2(y[j][0]), p1 = fast_exp2(y[j][1]), p2 = fast_exp2(y[j][2]), p3 = fast_exp2(y[j][3]);
         l0 += p0 + p2;
         l1 += p1 + p3;
-        p0 *= va * F0;
-        p1 *= va * F1;
-        p2 *= vc * F0;
-        p3 *= vc * F1;
+        p0 = p0 * F0 * va;
+        p1 = p1 * F1 * va;
+        p2 = p2 * F0 * vc;
+        p3 = p3 * F1 * vc;
         const uint32_t ph0 = pack_f16(p0, p1), ph1 = pack_f16(p2, p3);
         pb[j][0] = movmatrix_trans(ph0);
         pb[j][1] = movmatrix_trans(ph1);

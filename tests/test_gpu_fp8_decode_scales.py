@@ -45,6 +45,20 @@ def _batch(D, dtype, nats, value_scales, S=256, H=8, seed=0):
     return q, cache, tables
 
 
+def _flushed(q, cache, tables, ctx):
+    """Sum of p|v| over the tokens with a weight p below 2^-118 of the largest one's.  The kernel forms a
+    weight from fp32 exponentials of (score - reference of the moment) <= 2^8 and (older reference - newer
+    one, or a part's - the item's); where one of them is below 2^-126 it is 0 and with it the weight,
+    which is then below 2^8 * 2^-126."""
+    S, H, D = q.shape
+    at = tables.long()
+    k, v = (cache[i][0, at].double() * cache[i + 2][0, at].double()[:, :, None, :, None] for i in (0, 1))
+    k, v = (t.flatten(1, 2)[:, :ctx] for t in (k, v))
+    p = torch.einsum("shd,sthd->sht", q.double(), k)
+    p = (p - p.amax(-1, keepdim=True)).exp()
+    return torch.einsum("sht,sthd->shd", torch.where(p < 2.0 ** -118, p, 0.0), v.abs())
+
+
 def _check(ops, dtype, D, nats, value_scales, zero_pages=()):
     q, cache, tables = _batch(D, dtype, nats, value_scales)
     for j in zero_pages:
@@ -54,6 +68,8 @@ def _check(ops, dtype, D, nats, value_scales, zero_pages=()):
     ref = R.attend(q, *cache, 0, tables, torch.arange(S + 1), lens, 1.0)
     got = ops.paged_decode_fp8(q.cuda(), *[t.cuda() for t in cache], 0, tables.cuda(), lens.cuda(), 1.0, ctx)
     tol = R.attention_tolerance(dtype, *ref, ctx, D, BITS[dtype])
+    if zero_pages:
+        tol = tol + _flushed(q, cache, tables, ctx)
     err = (got.cpu().double() - ref[0]).abs()
     assert (err <= tol).all(), float((err / tol).max())
     assert ops.read_status(torch.device("cuda")) == 0
@@ -79,3 +95,25 @@ def test_scores_jump_towards_pages_of_small_values(ops, dtype, D, case):
     if dtype == torch.float16:  # the outputs within its range
         vs = [v * 2.0 ** -4 / min(vs) for v in vs]
     _check(ops, dtype, D, nats, vs)
+
+
+# a page without values (all zero: the append gives it the scale 2^-100; a caller may give it 0) that takes
+# all the weight, and pages of large values that carry next to none or none
+EMPTY = [
+    ([79.5, 79.5, 0, 0, 0, 0], [2.0 ** -100] * 2 + [2.0 ** 20] * 4),
+    ([85.0, 85, 0, 0, 0, 0], [2.0 ** -100] * 2 + [2.0 ** 21] * 4),
+    ([85.0, 0, 0, 0, 0, 0], [2.0 ** -100] + [2.0 ** 22] * 5),
+    ([105.0, 105, 0, 0, 0, 0], [2.0 ** -100] * 2 + [2.0 ** 30] * 4),
+    ([105.0, 0, 0, 0, 0, 0], [0.0] + [4.0] * 5),
+    ([105.0, 0, 0, 0, 0, 0], [0.0] + [2.0 ** -120] * 5),
+    ([105.0, 105, 110, 110, 0, 0], [0.0, 0, 0, 0, 2.0 ** 10, 2.0 ** 10]),
+    ([0.0, 0, 0, 0, 0, 0], [0.0, 0, 0, 0, 2.0 ** -5, 2.0 ** -5]),
+]
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("case", range(len(EMPTY)))
+def test_pages_without_values_before_large_ones(ops, dtype, D, case):
+    nats, vs = EMPTY[case]
+    _check(ops, dtype, D, nats, vs, zero_pages=[j for j, v in enumerate(vs) if v in (0.0, 2.0 ** -100)])
