@@ -645,7 +645,8 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
   };
   // Sum of w where only the log probability asks for it: exact for the terms above 2^-10, in fp32
   // (4e-7 off at most, either way) for the many small ones behind them.
-  const float c32 = static_cast<float>(1.4426950408889634 / t);
+  // finite at subnormal temperatures too: the maximum's own term is 2^(0 * c32) = 1
+  const float c32 = fminf(static_cast<float>(1.4426950408889634 / t), 3.402823466e38f);
   double sum_large = 0.0;
   float sum_small = 0.f;
   const auto sum32 = [&](float v) {
