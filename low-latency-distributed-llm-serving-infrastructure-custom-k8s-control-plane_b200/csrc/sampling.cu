@@ -598,6 +598,13 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
     cluster.sync();  // no CTA leaves while its peers read from it
     return;
   }
+  // Differences of logits are taken in fp32 below.  One that passes its range stands for a weight of
+  // e^-256 or less up to this temperature, and for one that counts beyond: left to sample_row_kernel.
+  if (rp.t > 0x1p+120f) {
+    if (rank == 0 && tid == 0) a.tokens[row] = kTodo;
+    cluster.sync();
+    return;
+  }
   const double t = rp.greedy ? 1.0 : static_cast<double>(rp.t);
   Weights weight;
   weight.set(sh.table, mx, t, a.shift);

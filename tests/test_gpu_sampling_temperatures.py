@@ -28,3 +28,20 @@ def test_top_k_at_subnormal_temperatures(sampling, dtype, vocab):
     for k in (2, 50, 300):
         _check(sampling, x, u, t=ts, k=[k] * len(ts))
         _check(sampling, x, u, t=ts, k=[k] * len(ts), p=[0.9] * len(ts), m=[0.1] * len(ts))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [600, 40001])
+def test_logits_and_temperatures_at_the_largest_numbers(sampling, dtype, vocab):
+    """Differences of two logits pass fp32's range while the weights do not vanish."""
+    rng = np.random.default_rng(6)
+    ts = [1e36, 5e36, 1e37, 5e37, 1e38, 3e38]
+    x = torch.from_numpy(rng.uniform(-3.2e38, 3.2e38, (len(ts), vocab)).astype(np.float32)).to(dtype)
+    x[:, 3], x[:, 4] = 3.2e38, -3.2e38
+    u = rng.random(len(ts), dtype=np.float32).tolist()
+    _check(sampling, x, u, t=ts)
+    _check(sampling, x, u, t=ts, k=[500] * len(ts))
+    _check(sampling, x, u, t=ts, m=[0.3] * len(ts))
+    for p in (0.05, 0.5, 0.9, 0.999):
+        _check(sampling, x, u, t=ts, p=[p] * len(ts))
+        _check(sampling, x, u, t=ts, k=[400] * len(ts), p=[p] * len(ts))
