@@ -256,7 +256,7 @@ def sampling_rows(seqs: List[Sequence], floats: np.ndarray, top_k: np.ndarray) -
     floats[1, :n] = [p.temperature if p else 0.0 for p in params]
     floats[2, :n] = [p.top_p if p else 1.0 for p in params]
     floats[3, :n] = [p.min_p if p else 0.0 for p in params]
-    top_k[:n] = [min(p.top_k, 0x7FFFFFFF) if p else 0 for p in params]
+    top_k[:n] = [min(max(p.top_k, 0), 0x7FFFFFFF) if p else 0 for p in params]
 
 
 class _DecodeGraph:

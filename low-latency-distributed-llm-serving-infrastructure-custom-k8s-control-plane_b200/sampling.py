@@ -3,6 +3,7 @@ draw by given uniform numbers (so a run is reproduced by its random numbers).  O
 libb200paged.so; raises if a tensor is not on a CUDA device."""
 from __future__ import annotations
 
+import numbers
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -15,7 +16,8 @@ from .paged_ops import _DTYPES, _on, _one_device, _ptr, _raw_stream, _status_ptr
 @dataclass
 class SamplingParams:
     """How a request's tokens are drawn.  ``temperature`` 0: the most likely token.  ``top_k`` 0
-    or less: no limit.  ``seed`` starts the request's own sequence of random numbers."""
+    or less: no limit.  ``seed`` starts the request's own sequence of random numbers.  The
+    temperature has to be finite in fp32, in which it is used."""
     temperature: float = 1.0
     top_k: int = 0
     top_p: float = 1.0
@@ -23,8 +25,20 @@ class SamplingParams:
     seed: int = 0
 
     def __post_init__(self) -> None:
-        if not 0.0 <= self.temperature < float("inf"):
-            raise ValueError(f"temperature must be finite and at least 0, got {self.temperature}")
+        for name in ("temperature", "top_p", "min_p"):
+            if not isinstance(getattr(self, name), numbers.Real):
+                raise ValueError(f"{name} must be a number, got {getattr(self, name)!r}")
+            try:
+                setattr(self, name, float(getattr(self, name)))
+            except OverflowError:
+                raise ValueError(f"{name} is beyond a float's range") from None
+        for name in ("top_k", "seed"):
+            if not isinstance(getattr(self, name), numbers.Integral):
+                raise ValueError(f"{name} must be a whole number, got {getattr(self, name)!r}")
+            setattr(self, name, int(getattr(self, name)))
+        # numbers from half a step above the largest fp32 number on become infinite
+        if not 0.0 <= self.temperature < 2.0 ** 128 - 2.0 ** 103:
+            raise ValueError(f"temperature must be finite in fp32 and at least 0, got {self.temperature}")
         if not 0.0 < self.top_p <= 1.0:
             raise ValueError(f"top_p must be in (0, 1], got {self.top_p}")
         if not 0.0 <= self.min_p <= 1.0:
