@@ -64,6 +64,7 @@ class Sequence:
         self.eos_token_id = eos_token_id
         self.sampling = sampling  # None: greedy
         self.status = SequenceStatus.WAITING
+        self.error: Optional[str] = None  # why the request ended before its last token
         self.block_table = None
         self.arrival = 0.0
         self.first_token_time: Optional[float] = None
@@ -333,7 +334,9 @@ class Engine:
         self._graph_ws = None
 
     def step(self) -> Dict[str, List[Sequence]]:
-        """One continuous-batching step.  NVTX ranges mark its phases on a timeline profile:
+        """One continuous-batching step.  A sampled step in which no token can be drawn for a request
+        (all its logits NaN or -inf) ends that request: it is among the finished ones, with its
+        ``error`` set.  NVTX ranges mark its phases on a timeline profile:
         ``engine.step`` around it, ``schedule``, then ``decode_graph`` (replay of a captured
         decode step) or ``eager_step`` (prefill or mixed batch); the C library adds one range per
         kernel-launching call inside them."""
@@ -362,13 +365,14 @@ class Engine:
             nvtx.range_pop()
         now = time.perf_counter()
         for s, t in zip(seqs, next_tokens):
-            if t < 0:
-                raise RuntimeError(f"Sequence {s.seq_id}: no token can be drawn (its logits are "
-                                   "all NaN or -inf)")
+            if t < 0:  # ends this request, the others go on
+                s.error = "no token can be drawn (its logits are all NaN or -inf)"
+                s.status = SequenceStatus.FINISHED
+                continue
             if s.first_token_time is None:
                 s.first_token_time = now
             s.append_token(int(t))
-        self.tokens_generated += len(seqs)
+            self.tokens_generated += 1
         self.steps += 1
         finished = [s for s in seqs if s.is_finished()]
         for s in finished:

@@ -21,3 +21,50 @@ def test_every_top_k_reaches_the_device(pkg, top_k):
     floats, ks = np.zeros((4, 1), np.float32), np.full(1, 7, np.int32)
     sampling_rows([s], floats, ks)
     assert ks[0] == (0 if top_k < 0 else 2 ** 31 - 1) and floats[1, 0] == 0.5
+
+
+def _host_engine():
+    """The engine over the host allocator; its model's step is replaced by ``answer``."""
+    import torch
+    from llm_serving_b200 import llm_allocator_cpp as la
+    from llm_serving_b200.engine import Engine, Scheduler
+    from test_engine_host import HostKV
+
+    class KV(HostKV):
+        torch_device = torch.device("cpu")
+
+    class Model:
+        class shape:
+            head_dim = 64
+
+    kv = KV(la, 64, 4)
+    eng = Engine(Model, kv, Scheduler(kv, max_batch_size=8, max_model_len=100), cuda_graphs=False)
+    # a request's n-th token is 10 * its first prompt token + n; without one from its `dies`-th on
+    eng.dies = {}
+    eng._eager_step = lambda out: [
+        -1 if len(s.output_token_ids) >= eng.dies.get(s.seq_id, 99) else 10 * s.prompt_token_ids[0] + len(s.output_token_ids)
+        for s in out.scheduled_prefills + out.scheduled_decodes]
+    return eng
+
+
+@pytest.mark.parametrize("dies", [{2: 0}, {1: 3}, {1: 2, 3: 2}, {4: 1, 2: 1, 3: 1, 1: 1}, {2: 4}])
+def test_a_row_without_a_token_ends_its_own_request_only(pkg, dies):
+    def run(dies):
+        eng = _host_engine()
+        eng.dies = dies
+        seqs = [eng.add_request([k + 1] * (k + 2), max_tokens=4 + k) for k in range(4)]
+        finished = []
+        for _ in range(20):
+            finished += eng.step()["finished"]
+        assert not eng.has_unfinished_requests()
+        assert sorted(s.seq_id for s in finished) == [1, 2, 3, 4]
+        assert eng.kv.allocator.get_num_free_blocks() == 64
+        assert eng.tokens_generated == sum(len(s.output_token_ids) for s in seqs)
+        return seqs
+
+    whole, got = run({}), run(dies)
+    assert all(s.error is None for s in whole)
+    for a, b in zip(whole, got):
+        n = dies.get(b.seq_id, 99)
+        assert b.output_token_ids == a.output_token_ids[:n]
+        assert (b.error is not None) == (n < len(a.output_token_ids)) and b.is_finished()
