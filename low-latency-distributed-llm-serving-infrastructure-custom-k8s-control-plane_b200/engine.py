@@ -13,8 +13,9 @@ Differences that are the point of the rebuild: block allocation goes to the devi
 mixed forward, and sampling runs on the device with one host read per step (instead of one
 ``int(argmax)`` per sequence, llm_engine.py:200-204): a greedy argmax, or, in steps with a request
 that asks for it (``SamplingParams``), temperature, top-k, top-p and min-p for every row by its own
-parameters.  A request's random numbers come from its seed and the index of the output token, so
-they do not depend on the batch it runs in, on preemption or on the tensor-parallel size.
+parameters.  A request's random numbers come from its seed (its own, or one made from the engine's
+``sampling_seed`` and the request's number) and the index of the output token, so they do not depend
+on the batch it runs in, on preemption or on the tensor-parallel size.
 The KV cache may be 8 bits wide (``build_engine(kv_dtype=torch.float8_e4m3fn)``).
 
 Pure decode steps replay a CUDA graph captured per batch-size bucket (step metadata, the whole
@@ -51,10 +52,22 @@ class SequenceStatus(Enum):
     FINISHED = "FINISHED"
 
 
+_MASK64 = 0xFFFFFFFFFFFFFFFF
+
+
+def request_seed(sampling_seed: int, seq_id: int) -> int:
+    """Seed of a request that names none: 64 bits mixed from the engine's sampling seed and the
+    request's number (the splitmix64 finaliser, Steele et al. 2014)."""
+    z = (sampling_seed * 0xD1342543DE82EF95 + seq_id * 0x9E3779B97F4A7C15) & _MASK64
+    z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & _MASK64
+    z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & _MASK64
+    return z ^ (z >> 31)
+
+
 class Sequence:
     def __init__(self, seq_id: int, prompt_token_ids: List[int], max_tokens: int = 128,
                  eos_token_id: Optional[int] = None,
-                 sampling: Optional[SamplingParams] = None) -> None:
+                 sampling: Optional[SamplingParams] = None, sampling_seed: int = 0) -> None:
         if not prompt_token_ids:
             raise ValueError(f"Sequence {seq_id}: Prompt and prompt_token_ids cannot be both empty.")
         self.seq_id = seq_id
@@ -63,6 +76,10 @@ class Sequence:
         self.max_tokens = max_tokens
         self.eos_token_id = eos_token_id
         self.sampling = sampling  # None: greedy
+        self.seed = 0  # of the request's random numbers
+        if sampling is not None:
+            self.seed = (request_seed(sampling_seed, seq_id) if sampling.seed is None
+                         else sampling.seed & _MASK64)
         self.status = SequenceStatus.WAITING
         self.error: Optional[str] = None  # why the request ended before its last token
         self.block_table = None
@@ -252,8 +269,7 @@ def sampling_rows(seqs: List[Sequence], floats: np.ndarray, top_k: np.ndarray) -
     and min-p, ``top_k`` (rows,).  Greedy requests have temperature 0."""
     n = len(seqs)
     params = [s.sampling for s in seqs]
-    floats[0, :n] = uniforms([p.seed & 0xFFFFFFFFFFFFFFFF if p else 0 for p in params],
-                             [len(s.output_token_ids) for s in seqs])
+    floats[0, :n] = uniforms([s.seed for s in seqs], [len(s.output_token_ids) for s in seqs])
     floats[1, :n] = [p.temperature if p else 0.0 for p in params]
     floats[2, :n] = [p.top_p if p else 1.0 for p in params]
     floats[3, :n] = [p.min_p if p else 0.0 for p in params]
@@ -287,8 +303,9 @@ class _DecodeGraph:
 
 class Engine:
     def __init__(self, model, kv_cache_manager: PagedKVCacheManager, scheduler: Scheduler,
-                 cuda_graphs: bool = True) -> None:
+                 cuda_graphs: bool = True, sampling_seed: int = 0) -> None:
         self.model = model
+        self.sampling_seed = sampling_seed  # of the requests that name no seed of their own
         self.kv = kv_cache_manager
         self.scheduler = scheduler
         self.device = kv_cache_manager.torch_device
@@ -310,9 +327,11 @@ class Engine:
     def add_request(self, prompt_token_ids: List[int], max_tokens: int = 128,
                     eos_token_id: Optional[int] = None, arrival: float = 0.0,
                     sampling: Optional[SamplingParams] = None) -> Sequence:
-        """``sampling``: how the request's tokens are drawn (None: greedy)."""
+        """``sampling``: how the request's tokens are drawn (None: greedy).  Without a seed of its own
+        it draws by one made from the engine's ``sampling_seed`` and its number."""
         self.seq_counter += 1
-        seq = Sequence(self.seq_counter, prompt_token_ids, max_tokens, eos_token_id, sampling)
+        seq = Sequence(self.seq_counter, prompt_token_ids, max_tokens, eos_token_id, sampling,
+                       self.sampling_seed)
         seq.arrival = arrival
         self.scheduler.add_sequence(seq)
         return seq
@@ -547,9 +566,10 @@ def build_engine(shape, total_blocks: int, block_size: int = 16, rank: int = 0, 
                  device=None, dtype=torch.bfloat16, seed: int = 0, max_batch_size: int = 256,
                  max_num_batched_tokens: int = 16384, max_model_len: int = 8192,
                  full_init: bool = False, group=None, cuda_graphs: bool = True,
-                 kv_dtype: Optional[torch.dtype] = None) -> Engine:
+                 kv_dtype: Optional[torch.dtype] = None, sampling_seed: int = 0) -> Engine:
     """``kv_dtype``: the KV cache's type where it is not the model's; torch.float8_e4m3fn holds it
-    in 8 bits."""
+    in 8 bits.  ``sampling_seed``: starts the random numbers of sampled requests that name no seed of
+    their own; the same on every rank of a tensor-parallel group, another on every replica."""
     from .model import TPLlama
     device = torch.device(device or "cuda")
     model = TPLlama(shape, rank, world, device, dtype, seed, full_init=full_init, group=group)
@@ -559,4 +579,4 @@ def build_engine(shape, total_blocks: int, block_size: int = 16, rank: int = 0, 
                              device=device, max_seqs=max(16 * max_batch_size, 4096),
                              max_blocks_per_seq=max_blocks)
     sched = Scheduler(kv, max_batch_size, max_num_batched_tokens, max_model_len)
-    return Engine(model, kv, sched, cuda_graphs=cuda_graphs)
+    return Engine(model, kv, sched, cuda_graphs=cuda_graphs, sampling_seed=sampling_seed)

@@ -16,13 +16,14 @@ from .paged_ops import _DTYPES, _on, _one_device, _ptr, _raw_stream, _status_ptr
 @dataclass
 class SamplingParams:
     """How a request's tokens are drawn.  ``temperature`` 0: the most likely token.  ``top_k`` 0
-    or less: no limit.  ``seed`` starts the request's own sequence of random numbers.  The
-    temperature has to be finite in fp32, in which it is used."""
+    or less: no limit.  ``seed`` starts the request's own sequence of random numbers (None:
+    the engine gives each request one).  The temperature has to be finite in fp32, in which it is
+    used."""
     temperature: float = 1.0
     top_k: int = 0
     top_p: float = 1.0
     min_p: float = 0.0
-    seed: int = 0
+    seed: Optional[int] = None
 
     def __post_init__(self) -> None:
         for name in ("temperature", "top_p", "min_p"):
@@ -33,6 +34,8 @@ class SamplingParams:
             except OverflowError:
                 raise ValueError(f"{name} is beyond a float's range") from None
         for name in ("top_k", "seed"):
+            if name == "seed" and self.seed is None:
+                continue
             if not isinstance(getattr(self, name), numbers.Integral):
                 raise ValueError(f"{name} must be a whole number, got {getattr(self, name)!r}")
             setattr(self, name, int(getattr(self, name)))

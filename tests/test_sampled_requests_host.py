@@ -68,3 +68,42 @@ def test_a_row_without_a_token_ends_its_own_request_only(pkg, dies):
         n = dies.get(b.seq_id, 99)
         assert b.output_token_ids == a.output_token_ids[:n]
         assert (b.error is not None) == (n < len(a.output_token_ids)) and b.is_finished()
+
+
+def _draws(seq, n=64):
+    """The uniform numbers of a request's first n tokens."""
+    from llm_serving_b200.engine import sampling_rows
+    out = []
+    floats, ks = np.zeros((4, 1), np.float32), np.zeros(1, np.int32)
+    seq.max_tokens = n + 1
+    for i in range(n):
+        sampling_rows([seq], floats, ks)
+        out.append(float(floats[0, 0]))
+        seq.append_token(i)
+    return out
+
+
+def test_requests_without_a_seed_draw_their_own_numbers(pkg):
+    from llm_serving_b200.sampling import SamplingParams
+    params = SamplingParams()  # shared by the requests
+    eng = _host_engine()
+    draws = [_draws(eng.add_request([1, 2], max_tokens=8, sampling=params)) for _ in range(50)]
+    assert len({u for d in draws for u in d}) > 0.99 * 50 * 64
+    # the correlation of two requests' numbers, within five standard deviations
+    z = np.array(draws) - 0.5
+    assert abs((z[1:] * z[:-1]).mean()) < 5 / 12 / (49 * 64) ** 0.5
+    # another engine of the same sampling seed (another rank) draws the same, one of another seed does not
+    same, other = _host_engine(), _host_engine()
+    other.sampling_seed = 1
+    assert _draws(same.add_request([5], max_tokens=8, sampling=params)) == draws[0]
+    assert not set(_draws(other.add_request([5], max_tokens=8, sampling=params))) & set(draws[0])
+
+
+def test_requests_with_a_seed_draw_as_before(pkg):
+    from llm_serving_b200.engine import Sequence, uniforms
+    from llm_serving_b200.sampling import SamplingParams
+    eng = _host_engine()
+    for seed in (0, 7, -3, 2 ** 64 + 7):
+        want = uniforms([seed % 2 ** 64] * 64, range(64)).tolist()
+        assert _draws(eng.add_request([1], max_tokens=8, sampling=SamplingParams(seed=seed))) == want
+        assert _draws(Sequence(9, [1], sampling=SamplingParams(seed=seed))) == want
