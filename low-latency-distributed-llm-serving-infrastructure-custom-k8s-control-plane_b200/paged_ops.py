@@ -65,16 +65,25 @@ def cache_geometry(key_cache: torch.Tensor) -> N.CacheGeometry:
     return N.CacheGeometry(L, NB, BS, Hkv, D, _DTYPES[key_cache.dtype])
 
 
+def _capturing(device: torch.device) -> bool:
+    with _on(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class Workspace:
     """Grow-only device scratch buffer per (device, stream), 256-byte aligned.  Keyed by stream
     because the kernels of one call use the scratch until they finish: two streams sharing one
     buffer would race, and a buffer replaced by a larger one is released in the order of the
-    stream that used it."""
+    stream that used it.  A call under capture gets memory of its own, which belongs to the graph:
+    the graph keeps using its address, also when the shared buffer has been replaced, and beside
+    other graphs."""
 
     def __init__(self):
         self._buf = {}
 
     def get(self, device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
+        if _capturing(device):
+            return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
         key = (device.type, device.index, stream)
         buf = self._buf.get(key)
         if buf is None or buf.numel() < nbytes:
