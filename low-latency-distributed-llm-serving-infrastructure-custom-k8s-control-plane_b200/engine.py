@@ -76,16 +76,20 @@ class Sequence:
         self.max_tokens = max_tokens
         self.eos_token_id = eos_token_id
         self.sampling = sampling  # None: greedy
-        self.seed = 0  # of the request's random numbers
-        if sampling is not None:
-            self.seed = (request_seed(sampling_seed, seq_id) if sampling.seed is None
-                         else sampling.seed & _MASK64)
+        self._own_seed = request_seed(sampling_seed, seq_id)
         self.status = SequenceStatus.WAITING
         self.error: Optional[str] = None  # why the request ended before its last token
         self.block_table = None
         self.arrival = 0.0
         self.first_token_time: Optional[float] = None
         self.finish_time: Optional[float] = None
+
+    @property
+    def seed(self) -> int:
+        """Starts the request's random numbers."""
+        if self.sampling is None:
+            return 0
+        return self._own_seed if self.sampling.seed is None else self.sampling.seed & _MASK64
 
     @property
     def total_len(self) -> int:

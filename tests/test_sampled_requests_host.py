@@ -107,3 +107,12 @@ def test_requests_with_a_seed_draw_as_before(pkg):
         want = uniforms([seed % 2 ** 64] * 64, range(64)).tolist()
         assert _draws(eng.add_request([1], max_tokens=8, sampling=SamplingParams(seed=seed))) == want
         assert _draws(Sequence(9, [1], sampling=SamplingParams(seed=seed))) == want
+
+
+def test_sampling_that_is_set_later_counts(pkg):
+    from llm_serving_b200.engine import Sequence, uniforms
+    from llm_serving_b200.sampling import SamplingParams
+    s = Sequence(3, [1])
+    assert s.seed == 0
+    s.sampling = SamplingParams(seed=11)
+    assert _draws(s) == uniforms([11] * 64, range(64)).tolist()
