@@ -418,7 +418,8 @@ int b200_reshape_and_cache_fp8(const B200Fp8Cache* cache, int32_t dtype, const v
 
 /* b200_rope_reshape_and_cache into an 8-bit cache: rotated q of `dtype` to q_out, rotated k and
  * v to their slots as above.  Unlike the 16-bit form, angles are formed and reduced in 64 bits
- * (exact at far positions) and rotated keys are rounded once, to their codes. */
+ * (exact at far positions); keys are rotated in 64 bits, rounded to fp32 and from there to their
+ * codes, not to `dtype` in between. */
 int b200_rope_reshape_and_cache_fp8(const B200Fp8Cache* cache, int32_t dtype, const void* qkv,
                                     int64_t qkv_stride_token, int32_t num_tokens,
                                     int32_t num_query_heads, const int64_t* positions,
@@ -455,24 +456,33 @@ typedef struct {
   int32_t num_tokens;         /* prefill                                                        */
   int32_t max_query_len;      /* prefill                                                        */
   int32_t prefill_blocks;     /* prefill: host upper bound of the cache blocks that sequences with
-                                 more than one new token hold together; < 0: not known          */
+                                 more than one new token hold together; < 0: not known, the
+                                 workspace is then for min(S, num_tokens / 2) sequences of
+                                 max_context_len                                                */
   int32_t* status_word;
 } B200AttentionFp8Params;
 
 size_t b200_paged_decode_fp8_workspace_bytes(const B200AttentionFp8Params* p);
 
 /* b200_paged_decode over an 8-bit cache.  A context of 0 gives zeros.  A page outside the pool
- * sets B200_DEVICE_BAD_BLOCK and its positions do not take part. */
+ * sets B200_DEVICE_BAD_BLOCK and its positions do not take part.  Head dims 64 and 128 with blocks of 8
+ * or a multiple of 16 slots run on the tensor cores, with the softmax weights in 11 bits (fp32
+ * queries: two parts of 11); other shapes take a slower kernel in fp32. */
 int b200_paged_decode_fp8(const B200AttentionFp8Params* p, void* workspace,
                           size_t workspace_bytes, void* stream);
 
 size_t b200_paged_prefill_fp8_workspace_bytes(const B200AttentionFp8Params* p);
 
 /* b200_paged_prefill over an 8-bit cache.  bf16 and f16 queries whose shapes the tensor-core prefill
- * covers run on it, over a 16-bit copy of the pages that the sequences with more than one new token
- * hold (exact for bf16 with power-of-two scales; f16 values beyond its range become +-65504); the
- * copy takes 4 bytes per cached entry of prefill_blocks blocks in the workspace.  If those
- * sequences hold more blocks than prefill_blocks, B200_DEVICE_BAD_STEP is set and the rows of the
+ * covers (head dim 64 or 128, blocks of a multiple of 16 slots, 1, 2, 4, 8 or 16 query heads per KV
+ * head, query rows and heads on 16-byte boundaries) run on it, with the softmax weights in the
+ * query's type, over a 16-bit copy of the pages that the sequences with more than one new token
+ * hold (exact for bf16 with power-of-two scales; f16 values beyond its range become +-65504, ones
+ * below 2^-14 are rounded to multiples of 2^-24); the copy takes 4 bytes per cached entry of
+ * prefill_blocks blocks in the workspace, and sequences with one new token run as in the decode.
+ * Every other call runs as a whole, its sequences with one new token among it, on a kernel with a
+ * CTA per query row, hundreds of times slower for long chunks.  If the sequences with more than one
+ * new token hold more blocks than prefill_blocks, B200_DEVICE_BAD_STEP is set and the rows of the
  * ones that do not fit are not meaningful.  A page outside the pool sets B200_DEVICE_BAD_BLOCK; the
  * rows of a sequence with such a page are not meaningful, the others are not touched by it.  Rows
  * of query behind the last sequence are left as they are in out. */
@@ -490,10 +500,12 @@ int b200_paged_prefill_fp8(const B200AttentionFp8Params* p, void* workspace,
  * min-p keeps tokens with w >= min_p; the first of all is always kept.  The token drawn is the
  * first in index order whose cumulative w exceeds uniform times the kept sum; temperature 0 takes
  * the first of all.  Parameters are device arrays of one entry per row; temperature, top_k, top_p
- * and min_p may be NULL (1, off, 1, 0).  NaN logits count as -inf.  logprobs (may be NULL): the
- * token's log probability at the row's temperature over the whole vocabulary.  A row in which no
- * token can be drawn (all logits -inf, or a parameter that is NaN or out of range) gives -1 and
- * NaN and sets B200_DEVICE_BAD_SAMPLE.  vocab <= 2^24.  Replaces the per-sequence host argmax of
+ * and min_p may be NULL (1, off, 1, 0).  NaN logits count as -inf, infinite ones as the largest
+ * fp32 number.  logprobs (may be NULL): the token's log probability at the row's temperature over
+ * the whole vocabulary.  A row in which no token can be drawn (all logits -inf, a parameter that is
+ * NaN, a uniform number outside [0, 1), a temperature that is negative or infinite) gives -1 and
+ * NaN and sets B200_DEVICE_BAD_SAMPLE; top_p and min_p outside [0, 1] act as the nearer end.
+ * vocab <= 2^24.  Replaces the per-sequence host argmax of
  * app/engine/llm_engine.py:200-204 for requests that are not greedy. */
 int b200_sample(const void* logits, int32_t dtype, int64_t stride_row, int32_t rows, int32_t vocab,
                 const float* uniform, const float* temperature, const int32_t* top_k,

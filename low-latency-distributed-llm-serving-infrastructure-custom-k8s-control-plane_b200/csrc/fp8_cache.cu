@@ -6,8 +6,8 @@
 //   new scale = need                    if R writes the block's first slot (the block begins anew)
 //             = max(old scale, need)    otherwise
 //   a held code c becomes rn(c * old / new) where the scale grew; a row's entry becomes rn(x / new).
-// Powers of two make both divisions exact, so each entry is rounded once (a held one again only
-// where it falls below e4m3's smallest normal number).
+// Powers of two make both divisions exact, so each entry is rounded to its code once (a held one again
+// only where it falls below e4m3's smallest normal number).
 //
 // One CTA owns a block: it lists the block's rows in the call, takes the maxima, rescales what the
 // block holds and writes the rows, so no two CTAs touch one scale.  In calls of up to
@@ -16,10 +16,10 @@
 // the rows where a run of rows of one block starts.
 //
 // Bound: HBM.  A step of 16 prompt chunks and 240 single rows (14,200 rows, GQA 32/8, D 128, bf16, with
-// rotation): 76 us for rows, codes and rotated queries (49 us at the copy rate; 44 % of the DRAM rate),
+// rotation): 76 us for rows, codes and rotated queries (275 MB move: 55 % of the copy rate),
 // 22 us for the read-back; one element per thread and memory pass took 427 us for both, against 108.  256
 // decode rows take 6.3 us, of which a launch and the chain slot -> block -> scale -> codes are the most.
-// Rows that have a block to themselves are what keeps a large call from the DRAM rate: 8192 of them take
+// Rows that have a block to themselves are what keeps a large call from the copy rate: 8192 of them take
 // 115 us, 8192 rows of whole blocks 48.
 #include "fp8.cuh"
 
@@ -34,9 +34,9 @@ constexpr int kMaxBlockSize = 1024;
 
 // cos and sin of pos * inv_freq in 64 bits.  The product is formed and reduced to [-pi/4, pi/4] in
 // 64 bits (at position 30,000 a 32-bit product alone is off by 1e-3 rad) and the Taylor series there
-// end with a remainder below 2e-14.  Keys are rotated in 64 bits too, so that each lands on the code
-// of its exact value: two products an element, less than fp32 arithmetic in two parts (12
-// operations).
+// end with a remainder below 2e-14.  Keys are rotated in 64 bits too and rounded to fp32 (an error of
+// 2^-24, against a code's 2^-4): two products an element, less than fp32 arithmetic in two parts
+// (12 operations).
 struct __align__(16) Turn {
   double c, s;
 };

@@ -22,10 +22,10 @@
 // most 2^-25 of the largest for smaller ones).
 //
 // Bound: HBM (4 * G flop per byte).  A unit is 64 * D bytes.  Measured with GQA 32/8, D 128, bf16
-// queries: 256 sequences of 16 to 4096 tokens (677 MB) 128-139 us, 4.9-5.3 TB/s; 14 of 8192 to 32768
-// (616 MB) 115-127 us; 66-68 % of the DRAM rate and 43 % of the issue slots while the warps run, so
-// what bounds it now is how many loads the 12 consumers an SM (128 registers a thread) keep in flight
-// beside their conversions and products.
+// queries: 256 sequences of 16 to 4096 tokens (677 MB) 133-137 us, 4.9-5.1 TB/s; 14 of 8192 to 32768
+// (616 MB) 120-123 us, the merge (6 and 12 us) included.  While the warps run: 5.3 and 5.6 TB/s, 81 and
+// 85 % of the copy rate, and 42 % of the issue slots, so what bounds it now is how many loads the 12
+// consumers an SM (128 registers a thread) keep in flight beside their conversions and products.
 // What the parts brought (256 sequences | 14 long ones, us): a CTA per row on the CUDA cores 2337 | 6022;
 // tensor cores and equal shares of 16-token units 173 | 148; the warps of a CTA on adjacent heads 151 |
 // 135; 32-token units, 12 warps an SM with 16 KB rings 133 | 125; a loading warp per CTA 134 | 118.

@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
 // ---- a cluster of CTAs per row ----------------------------------------------------------------------
 //
 // Bound by instructions: an exact weight takes some 20, 12 of them on the 64-bit pipe.  256 rows of
-// 128256: temperature alone 74 us in bf16 (64 % of the issue slots, 10 % of the DRAM rate) and 122 in
+// 128256: temperature alone 79 us in bf16 (64 % of the issue slots, 12 % of the copy rate) and 122 in
 // fp32, top-k 50 113 and 156, top-p 0.95 188 and 262; one CTA per row that reads it once per pass took
 // 933 us for temperature alone and 2963 for all filters (186 before the draw lost its pass after
 // top-p, 168 now).  One row of 128256: 13, 18 and 28 us.
@@ -751,7 +751,7 @@ __global__ void __launch_bounds__(kClThreads, 1024 / kClThreads) sample_cluster_
           sum[e] += ahead ? w : 0;
         }
       }
-      // a lane's sum is below 2^50 (up to 12 weights of at most 2^46): in two parts of 26 bits
+      // a lane's sum is at most 2^48 (kCounted / 32 = 4 weights of at most 2^46): in two parts of 26 bits
       static_assert(kCounted <= 32 * 63, "a lane's sum stays below 2^52");
 #pragma unroll
       for (int e = 0; e < E; ++e) {

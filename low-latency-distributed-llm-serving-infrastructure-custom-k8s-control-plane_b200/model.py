@@ -180,7 +180,8 @@ class TPLlama:
         return g[best, 1, torch.arange(g.shape[2], device=g.device)].long()
 
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
-        """Full logits (for tests): gathers the vocab shards."""
+        """Full fp32 logits, for steps with sampled requests and for tests: gathers the vocab
+        shards."""
         lg = F.linear(hidden, self.lm_head).float()
         if self.world == 1:
             return lg

@@ -437,7 +437,7 @@ def rope_reshape_and_cache_fp8(qkv: torch.Tensor, positions: torch.Tensor, inv_f
     """``rope_reshape_and_cache`` into an 8-bit cache: qkv (Ntok, (Hq + 2*Hkv) * D) rows
     [q | k | v] of any float type; rotated k and v go to their slots as
     ``reshape_and_cache_fp8`` stores them; returns the rotated q (Ntok, Hq, D) of qkv's type.
-    Angles are formed in 64 bits and a rotated key is rounded once, to its code."""
+    Angles are formed in 64 bits; a rotated key is rounded to fp32 and from there to its code."""
     c = fp8_cache(key_cache, value_cache, key_scale, value_scale, layer_idx)
     if qkv.dim() != 2 or qkv.stride(1) != 1:
         raise ValueError("qkv must be (tokens, row) with unit stride inside a row")
@@ -585,7 +585,10 @@ def paged_prefill_fp8(query: torch.Tensor, key_cache: torch.Tensor, value_cache:
                       prefill_blocks: Optional[int] = None) -> torch.Tensor:
     """``paged_prefill`` over an 8-bit cache (prefill chunks and mixed steps): query (Ntok, Hq, D)
     of any float type.  ``prefill_blocks``: how many cache blocks the sequences with more than one
-    new token hold together, where the caller knows it; it bounds the call's scratch memory."""
+    new token hold together, where the caller knows it; it bounds the call's scratch memory, which
+    otherwise is for min(S, Ntok / 2) sequences of max_context_len (4 * Hkv * D bytes a token).  What the tensor-core prefill does not cover (fp32
+    queries, head dims other than 64 and 128, block sizes that are no multiple of 16, other than 1,
+    2, 4, 8 or 16 query heads per KV head) runs on a far slower kernel, decodes included."""
     if out is None:
         out = torch.empty_like(query)
     p = attention_fp8_params(query, key_cache, value_cache, key_scale, value_scale, layer_idx,

@@ -68,8 +68,9 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor,
 
     Returns (tokens int64, log-probabilities fp32): the latter of the whole vocabulary's softmax
     at the row's temperature (at 1 for temperature 0), before the filters.  A row in which no
-    token can be drawn (every logit masked, or a parameter that is NaN or out of range) gives
-    token -1, NaN and the status bit DEVICE_BAD_SAMPLE."""
+    token can be drawn (every logit masked, a parameter that is NaN, a uniform number outside [0, 1),
+    a temperature that is negative or infinite) gives token -1, NaN and the status bit
+    DEVICE_BAD_SAMPLE.  top_p and min_p outside [0, 1] act as the nearer end."""
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be (rows, vocab) with unit stride along a row")
     if logits.dtype not in _DTYPES:
