@@ -66,6 +66,8 @@ def cache_geometry(key_cache: torch.Tensor) -> N.CacheGeometry:
 
 
 def _capturing(device: torch.device) -> bool:
+    if device.type != "cuda":
+        return False
     with _on(device):
         return torch.cuda.is_current_stream_capturing()
 
