@@ -615,20 +615,34 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           w1 = fmaxf(w1, __shfl_xor_sync(0xffffffffu, w1, o));
         }
         // F changes when unset, when a product would pass 2^15, and when the unit's largest one falls below
-        // 1: the reference has then moved to pages of smaller values, whose products f16 would hold in
-        // fewer bits.  Sums held so far are below 2^55 (products of 2^15, codes of 448, 2^31
-        // tokens); what raises F leaves them below 2^115.
-        const auto refit = [](float w, float& F, float& al) {
+        // 1: the reference may have moved to pages of smaller values, whose products f16 would hold in
+        // fewer bits.  What raises F leaves the sums held so far below 2^101; those of a unit that
+        // would need more are 2^-90 of them at most.
+        const auto low = [](float w, float F) { return w > 0.f && F != kUnset && w * F < 1.f; };
+        float held0 = 0.f, held1 = 0.f;
+        if (__any_sync(0xffffffffu, low(w0, F0) || low(w1, F1))) {
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            held0 = fmaxf(held0, fmaxf(fabsf(acc[k][0]), fabsf(acc[k][2])));
+            held1 = fmaxf(held1, fmaxf(fabsf(acc[k][1]), fabsf(acc[k][3])));
+          }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            held0 = fmaxf(held0, __shfl_xor_sync(0xffffffffu, held0, o));
+            held1 = fmaxf(held1, __shfl_xor_sync(0xffffffffu, held1, o));
+          }
+        }
+        const auto exponent = [](float x) { return static_cast<int>(__float_as_uint(x) >> 23); };
+        const auto refit = [&](float w, float held, float& F, float& al) {
           if (!(w > 0.f) || (F != kUnset && w * F >= 1.f && w * F <= 32768.f)) return;
           const float f = fminf(pow2_inverse(w, 8), 0.5f * kUnset);  // p * vs * F in [2^8, 2^9)
-          const int up = static_cast<int>(__float_as_uint(f) >> 23) - static_cast<int>(__float_as_uint(F) >> 23);
-          const int most = 60 + 127 - static_cast<int>(__float_as_uint(al) >> 23);
-          const int by = al > 0.f ? min(up, most) : up;
+          int by = exponent(f) - exponent(F);
+          if (by > 0) by = min(by, max(227 - exponent(held * al), 0));
           F = __uint_as_float(__float_as_uint(F) + (static_cast<uint32_t>(by) << 23));
           al = ldexpf(al, by);
         };
-        refit(w0, F0, al0);
-        refit(w1, F1, al1);
+        refit(w0, held0, F0, al0);
+        refit(w1, held1, F1, al1);
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           acc[k][0] *= al0;

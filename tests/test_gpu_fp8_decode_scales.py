@@ -117,3 +117,20 @@ EMPTY = [
 def test_pages_without_values_before_large_ones(ops, dtype, D, case):
     nats, vs = EMPTY[case]
     _check(ops, dtype, D, nats, vs, zero_pages=[j for j, v in enumerate(vs) if v in (0.0, 2.0 ** -100)])
+
+
+# pages of large values, then pages without values whose scores pass theirs step by step
+LATER = [
+    ([0.0] * 6 + [6.0, 12.0], [2.0 ** 40] * 6 + [2.0 ** -100] * 2),
+    ([0.0] * 6 + [6.0, 12.0], [2.0 ** 90] * 6 + [2.0 ** -100] * 2),
+    ([0.0] * 4 + [7.0, 7, 14, 14, 21, 21], [2.0 ** 30] * 4 + [0.0, 0, 2.0 ** -100, 2.0 ** -100, 0, 2.0 ** -100]),
+    ([0.0] * 4 + [7.0, 7, 14, 14, 0, 0], [2.0 ** 30] * 4 + [2.0 ** -100] * 4 + [2.0 ** 28] * 2),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("case", range(len(LATER)))
+def test_pages_without_values_after_large_ones(ops, dtype, D, case):
+    nats, vs = LATER[case]
+    _check(ops, dtype, D, nats, vs, zero_pages=[j for j, v in enumerate(vs) if v in (0.0, 2.0 ** -100)])
