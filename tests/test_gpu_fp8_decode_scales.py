@@ -45,18 +45,20 @@ def _batch(D, dtype, nats, value_scales, S=256, H=8, seed=0):
     return q, cache, tables
 
 
-def _flushed(q, cache, tables, ctx):
-    """Sum of p|v| over the tokens with a weight p below 2^-118 of the largest one's.  The kernel forms a
-    weight from fp32 exponentials of (score - reference of the moment) <= 2^8 and (older reference - newer
-    one, or a part's - the item's); where one of them is below 2^-126 it is 0 and with it the weight,
-    which is then below 2^8 * 2^-126."""
-    S, H, D = q.shape
+def _attend(q, cache, tables, ctx):
+    """``R.attend`` for S contexts of one length, a query head per KV head and a scale of 1, all
+    sequences side by side; and the sum of p|v| over the tokens with a weight p below 2^-118 of the
+    largest one's.  The kernel forms a weight from fp32 exponentials of (score - reference of the
+    moment) <= 2^8 and (older reference - newer one, or a part's - the item's); where one of them is
+    below 2^-126 it is 0 and with it the weight, which is then below 2^8 * 2^-126."""
     at = tables.long()
-    k, v = (cache[i][0, at].double() * cache[i + 2][0, at].double()[:, :, None, :, None] for i in (0, 1))
-    k, v = (t.flatten(1, 2)[:, :ctx] for t in (k, v))
-    p = torch.einsum("shd,sthd->sht", q.double(), k)
-    p = (p - p.amax(-1, keepdim=True)).exp()
-    return torch.einsum("sht,sthd->shd", torch.where(p < 2.0 ** -118, p, 0.0), v.abs())
+    k, v = ((cache[i][0, at].double() * cache[i + 2][0, at].double()[:, :, None, :, None])
+            .flatten(1, 2)[:, :ctx].transpose(1, 2) for i in (0, 1))  # (S, H, ctx, D)
+    q = q.double()[:, :, None]
+    p = (q @ k.mT)[:, :, 0].softmax(-1)[:, :, None]
+    low = torch.where(p < 2.0 ** -118 * p.amax(-1, keepdim=True), p, 0.0)
+    big = (q.abs() @ k.abs().mT).amax(-1)
+    return ((p @ v)[:, :, 0], (p @ v.abs())[:, :, 0], big), (low @ v.abs())[:, :, 0]
 
 
 def _check(ops, dtype, D, nats, value_scales, zero_pages=()):
@@ -65,11 +67,11 @@ def _check(ops, dtype, D, nats, value_scales, zero_pages=()):
         cache[1].view(torch.uint8)[:, tables[:, j].long()] = 0
     S, ctx = q.shape[0], len(nats) * BS - 3
     lens = torch.full((S,), ctx, dtype=torch.int32)
-    ref = R.attend(q, *cache, 0, tables, torch.arange(S + 1), lens, 1.0)
+    ref, flushed = _attend(q, cache, tables, ctx)
     got = ops.paged_decode_fp8(q.cuda(), *[t.cuda() for t in cache], 0, tables.cuda(), lens.cuda(), 1.0, ctx)
     tol = R.attention_tolerance(dtype, *ref, ctx, D, BITS[dtype])
     if zero_pages:
-        tol = tol + _flushed(q, cache, tables, ctx)
+        tol = tol + flushed
     err = (got.cpu().double() - ref[0]).abs()
     assert (err <= tol).all(), float((err / tol).max())
     assert ops.read_status(torch.device("cuda")) == 0
