@@ -571,7 +571,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       for (int p = 1; p < NP; ++p) vmax = fmaxf(vmax, vs[p]);
 #pragma unroll
       for (int e = 1; e < 8; ++e) top = fmaxf(top, y[e >> 2][e & 3]);
-      // (a fitted F leaves pages of the same scale below 2^7)
       const bool move = top > kLazy || vmax * fmaxf(F0, F1) > 128.f;
       if (__any_sync(0xffffffffu, move)) {
         float t0 = m0, t1 = m1;
@@ -617,8 +616,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
         // F changes when unset, when a product would pass 2^15, and when the unit's largest one falls below
         // 1: the reference may have moved to pages of smaller values, whose products f16 would hold in
-        // fewer bits.  What raises F leaves the sums held so far below 2^101; the products of a unit
-        // that would need more are 2^-90 of them at most.
+        // fewer bits.  What raises F leaves the sums held so far below 2^101; those of a unit that
+        // would need more are 2^-90 of them at most.
         const auto low = [](float w, float F) { return w > 0.f && F != kUnset && w * F < 1.f; };
         float held0 = 0.f, held1 = 0.f;
         if (__any_sync(0xffffffffu, low(w0, F0) || low(w1, F1))) {
@@ -636,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         const auto exponent = [](float x) { return static_cast<int>(__float_as_uint(x) >> 23); };
         const auto refit = [&](float w, float held, float& F, float& al) {
           if (!(w > 0.f) || (F != kUnset && w * F >= 1.f && w * F <= 32768.f)) return;
-          const float f = fminf(pow2_inverse(w, 6), 0.5f * kUnset);  // p * vs * F in [2^6, 2^7)
+          const float f = fminf(pow2_inverse(w, 8), 0.5f * kUnset);  // p * vs * F in [2^8, 2^9)
           int by = exponent(f) - exponent(F);
           if (by > 0) by = min(by, max(227 - exponent(held * al), 0));
           F = __uint_as_float(__float_as_uint(F) + (static_cast<uint32_t>(by) << 23));
