@@ -498,13 +498,16 @@ int b200_paged_prefill_fp8(const B200AttentionFp8Params* p, void* workspace,
  * index first) and w = exp((logit - max) / temperature): top-k keeps the first k (<= 0: all);
  * top-p keeps of those each token whose predecessors' sum of w is below top_p times their sum;
  * min-p keeps tokens with w >= min_p; the first of all is always kept.  The token drawn is the
- * first in index order whose cumulative w exceeds uniform times the kept sum; temperature 0 takes
+ * first in index order whose cumulative w exceeds uniform times the kept sum; w is worked out to
+ * 5e-14 and held in steps of 2^-46 (2^-(62 - b) for vocabularies of up to 2^b tokens, b > 16), so a
+ * token of less than half a step is not drawn, by uniform 0 either; temperature 0 takes
  * the first of all.  Parameters are device arrays of one entry per row; temperature, top_k, top_p
  * and min_p may be NULL (1, off, 1, 0).  NaN logits count as -inf, infinite ones as the largest
  * fp32 number.  logprobs (may be NULL): the token's log probability at the row's temperature over
- * the whole vocabulary.  A row in which no token can be drawn (all logits -inf, a parameter that is
- * NaN, a uniform number outside [0, 1), a temperature that is negative or infinite) gives -1 and
- * NaN and sets B200_DEVICE_BAD_SAMPLE; top_p and min_p outside [0, 1] act as the nearer end.
+ * the whole vocabulary (for top-k and the first of all good to 2.7e-6 where tokens of less than
+ * 2^-10 of the first's probability hold most of it, else to fp32's rounding).  A row in which no
+ * token can be drawn (all logits -inf, a parameter that is NaN, a uniform number outside [0, 1), a
+ * temperature that is negative or infinite) gives -1 and NaN and sets B200_DEVICE_BAD_SAMPLE; top_p and min_p outside [0, 1] act as the nearer end.
  * vocab <= 2^24.  Replaces the per-sequence host argmax of
  * app/engine/llm_engine.py:200-204 for requests that are not greedy. */
 int b200_sample(const void* logits, int32_t dtype, int64_t stride_row, int32_t rows, int32_t vocab,

@@ -15,16 +15,19 @@
 //   S^T = K Q^T and O^T += V^T P^T, m16n8k16 with f16 operands and fp32 sums.
 // Q is scaled to f16 by a power of two per head (exact for bf16 and f16 queries); fp32 queries and
 // weights are split in two f16 parts (22 bits), each with its own product.
-// The weights of P: p = 2^(x - m) with a lazily moved reference m (p <= 2^8), stored for the
+// The weights of P: p = 2^(x - m) with a reference m that moves in units with a page whose value scale is
+// near the largest so far (nearly all) or with a score that passes it by more than 8 (p <= 2^8).  A
+// row's largest weight is then mostly 1, exact in f16; a reference that moves at scores alone takes 131 us
+// for 256 sequences against 134, with the rounding of the largest weights in every output.  P is stored for the
 // product as p * vs * F: vs is the page's value scale and F a power of two per head that keeps the
 // head's largest product between 1 and 2^15 whatever the scales are, also where the scores move on to
 // pages of far smaller values (11 bits of every product within 2^-14 of the largest, an error of at
 // most 2^-25 of the largest for smaller ones).
 //
 // Bound: HBM (4 * G flop per byte).  A unit is 64 * D bytes.  Measured with GQA 32/8, D 128, bf16
-// queries: 256 sequences of 16 to 4096 tokens (677 MB) 133-137 us, 4.9-5.1 TB/s; 14 of 8192 to 32768
-// (616 MB) 120-123 us, the merge (6 and 12 us) included.  While the warps run: 5.3 and 5.6 TB/s, 81 and
-// 85 % of the copy rate, and 42 % of the issue slots, so what bounds it now is how many loads the 12
+// queries: 256 sequences of 16 to 4096 tokens (677 MB) 134-140 us, 4.8-5.1 TB/s; 14 of 8192 to 32768
+// (616 MB) 121-125 us, the merge (8 and 13 us) included.  While the warps run: 5.3 and 5.5 TB/s, 81 and
+// 84 % of the copy rate, and 43 % of the issue slots, so what bounds it now is how many loads the 12
 // consumers an SM (128 registers a thread) keep in flight beside their conversions and products.
 // What the parts brought (256 sequences | 14 long ones, us): a CTA per row on the CUDA cores 2337 | 6022;
 // tensor cores and equal shares of 16-token units 173 | 148; the warps of a CTA on adjacent heads 151 |
@@ -552,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         for (int e = 0; e < 4; ++e) s[j][e] += sb[e];
       }
 
-      // ---- softmax with a lazily moved reference: y = score - m, in log2 units -------------------
+      // ---- softmax relative to the reference: y = score - m, in log2 units ----------------------
       float y[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -571,6 +574,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       for (int p = 1; p < NP; ++p) vmax = fmaxf(vmax, vs[p]);
 #pragma unroll
       for (int e = 1; e < 8; ++e) top = fmaxf(top, y[e >> 2][e & 3]);
+      // (a unit fitted to F has p * vs * F in [2^8, 2^9); without a move p is up to 2^8, the product to 2^15)
       const bool move = top > kLazy || vmax * fmaxf(F0, F1) > 128.f;
       if (__any_sync(0xffffffffu, move)) {
         float t0 = m0, t1 = m1;
@@ -616,8 +620,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
         // F changes when unset, when a product would pass 2^15, and when the unit's largest one falls below
         // 1: the reference may have moved to pages of smaller values, whose products f16 would hold in
-        // fewer bits.  What raises F leaves the sums held so far below 2^101; those of a unit that
-        // would need more are 2^-90 of them at most.
+        // fewer bits.  What raises F leaves the sums held so far below 2^101; the products of a unit
+        // that would need more are 2^-90 of them at most.
         const auto low = [](float w, float F) { return w > 0.f && F != kUnset && w * F < 1.f; };
         float held0 = 0.f, held1 = 0.f;
         if (__any_sync(0xffffffffu, low(w0, F0) || low(w1, F1))) {
